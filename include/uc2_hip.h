@@ -171,6 +171,34 @@ int uc2_gemm_fp8_drop_residual(int M, int N, int K, const void* A8, int lda, con
                                const float* scale_w, void* C, int ldc, const float* bias, const void* residual, int ldres,
                                float p_drop, const uint64_t* seed_ptr, uint64_t seed_imm, void* stream);
 
+/* ---- e4m3 under block scales: one power of two for each block of 128 (beside the per-tensor scales above, which follow a tensor's history;
+ *      these need none, so they also serve single calls, and an outlier costs its own block only) ---------------------------------------
+ *   block value = e4m3(x 2^-e) 2^e, e the smallest integer with max |x| <= 448 2^e, kept as the byte e + 127 (at least 1); infinities and
+ *   NaN become the e4m3 NaN.  Kp = K rounded up to a multiple of 128; the bytes behind K are zero.
+ *   rows (activations, output gradients): x [M, K] (row stride ldx elements, any alignment) -> out [M, Kp] bytes, scale = 32-bit words
+ *     [ceil(Kp / 512)][M], word (w, m) = the bytes of row m's blocks 4 w .. 4 w + 3.
+ *   square (weights): w [N, K] -> out [N, Kp], scale = bytes [ceil(N / 128)][Kp / 128], one per block of 128 x 128; optionally the transposed copy
+ *     out_t [K, Np] with scale_t [Kp / 128][Np / 128] (Np = N rounded up to 128), the operand of the input gradient dX = dY W: the same values. */
+int uc2_fp8_quant_rows(int dtype, int M, int K, const void* x, long long ldx, void* out, void* scale, void* stream);
+int uc2_fp8_quant_square(int dtype, int N, int K, const void* w, long long ldw, void* out, void* scale, void* out_t, void* scale_t, void* stream);
+/* C[M,N] (bf16) = A8 B8^T + bias[n] of a rows operand A8 [M, Kp] and a square operand B8 [N, Kp]; the scales are applied inside the matrix
+ * instruction, sums are fp32, one rounding to bf16.  lda, ldb multiples of 16 bytes, A8 and B8 16-byte aligned; rows_a = the row count of A8's scale words (>= M: the first rows
+ * of a longer operand may be multiplied); C of any alignment.  Any M, N, K; any number of rows including single ones. */
+int uc2_gemm_fp8_block(int M, int N, int K, const void* A8, int lda, const void* scale_a, int rows_a, const void* B8, int ldb,
+                       const void* scale_b, const float* bias, void* C, int ldc, void* stream);
+
+/* ---- root-mean-square norm of a residual stream (beside LayerNorm below) ------------------------------------------------------------------
+ *   sum = x + residual rounded to the tensors' type (both NULL: the norm reads x);  y = sum rstd gamma,  rstd = 1 / sqrt(mean(sum^2) + eps)
+ *   rows contiguous, any alignment, H <= 16384.  y, rstd optional (y or q_out is given); q_out / q_scale: y as a rows operand of
+ *   uc2_gemm_fp8_block, quantised from the fp32 values.
+ *   backward: dx = rstd (g - h mean(g h)) + dsum, g = dy gamma, h = sum rstd -- the gradient of x and of residual alike; dsum (gradient that
+ *   reaches the stream itself) may be NULL; dgamma [H] = sum over rows of dy h (written; may be NULL), in a fixed order through ws (uc2_rms_bwd_workspace). */
+int uc2_rms_fwd(int dtype, int M, int H, const void* x, const void* residual, const float* gamma, float eps, void* sum, void* y, float* rstd,
+                void* q_out, void* q_scale, void* stream);
+size_t uc2_rms_bwd_workspace(int M, int H);
+int uc2_rms_bwd(int dtype, int M, int H, const void* dy, const void* dsum, const void* sum, const float* gamma, const float* rstd, void* dx,
+                float* dgamma, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- One BertLayer per call (model/layer.py:159-170: BertAttention -> BertIntermediate -> BertOutput) ---------------------------
  * The launch sequence of uc2_amd/ops/layer.py BertLayerFn -- 7 launches forward, 8 backward -- enqueued by one C call per direction: the same
  * kernels with the same arguments in the same order as the per-kernel entry points above, hence the same bits.  It exists for the host:
@@ -305,6 +333,39 @@ int uc2_attn_general_bwd(int dtype, int B, int Lq, int Lk, int nh, int D, const 
 int uc2_attn_general_probs_mean(int dtype, int B, int Lq, int Lk, int nh, int D, const void* q, int ldq, const void* k, int ldk,
                                 const float* key_mask, const float* attn_mask, float scale, const float* lse, float* out,
                                 float drop_p, const uint64_t* seed_ptr, uint64_t seed_imm, void* stream);      /* (dropped weights, like the reference returns) */
+
+/* ---- attention from one sequence to the states of another (cross attention; beside the general form above, which serves
+ *      MultiheadAttention, model/attention.py:12-264) ----------------------------------------------------------------------------
+ *   q, out [B, Lq, nh, D], k, v [B, Lk, nkv, D], nkv dividing nh (heads h G .. h G + G - 1, G = nh / nkv, share key head h); D 32, 64 or
+ *   128; strides of batch / row / head in ELEMENTS, the head dimension contiguous; every pointer 16-byte aligned, every stride a
+ *   multiple of 16 bytes (slices of a fused projection are read in place).
+ *     out = softmax_key(scale q k^T + key_mask) v
+ *   k_lens [B] int32 on the device, or NULL: keys at and behind k_lens[b] (clamped to 0 .. Lk) take no part.  key_mask [B, Lk] fp32
+ *   additive (row stride key_mask_sb), or NULL: a key whose entry is <= -1e30 takes no part.  What the rows of such keys hold reaches
+ *   nothing (NaN included), their dk / dv are zero; a row without any key gives zeros and passes no gradient.  lse [B, nkv, Lq, G] fp32: base-2
+ *   log-sum-exp of each row (-inf: no key), for the backward; NULL in a forward that has none.  Dropout on the normalised weights, keep(row, key)
+ *   a function of (*seed + site, batch, head, query, key head, key) as in uc2_attn_general_fwd (the same mask where nkv == nh).
+ *   fp32 softmax and sums; bf16 rounds the weights (and their gradients) to bf16 where they enter the second matrix product.  No atomics:
+ *   results repeat bit for bit.  ws: uc2_xattn_workspace bytes (0: may be NULL), not shared by calls that may overlap. */
+typedef struct Uc2CrossAttn {
+  int dtype, B, Lq, Lk, nh, nkv, D;
+  float scale, drop_p;
+  const void *q, *k, *v;
+  long long q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
+  const float* key_mask; long long key_mask_sb;
+  const int* k_lens;
+  void* out; long long o_sb, o_sl, o_sh;
+  float* lse;
+  const uint64_t* seed; uint64_t site;
+} Uc2CrossAttn;
+typedef struct Uc2CrossAttnGrad {
+  const void* dout; long long dout_sb, dout_sl, dout_sh;
+  void *dq, *dk, *dv;
+  long long dq_sb, dq_sl, dq_sh, dk_sb, dk_sl, dk_sh, dv_sb, dv_sl, dv_sh;
+} Uc2CrossAttnGrad;
+size_t uc2_xattn_workspace(const Uc2CrossAttn* attn, int backward);
+int uc2_xattn_fwd(const Uc2CrossAttn* attn, void* ws, size_t ws_bytes, void* stream);
+int uc2_xattn_bwd(const Uc2CrossAttn* attn, const Uc2CrossAttnGrad* grad, void* ws, size_t ws_bytes, void* stream);
 
 /* ---- embeddings and sequence assembly (model/model.py:280-335, 352-364, 412-425) ---------------------------- */
 int uc2_position_ids(int B, int T, const int64_t* ids, int64_t pad, int64_t* out, void* stream);

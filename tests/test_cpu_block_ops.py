@@ -1,0 +1,127 @@
+"""What the block-scaled e4m3 operators, the root-mean-square norm and the cross attention refuse before anything is launched, and the test
+oracle's own arithmetic, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+import block_ref as R
+from uc2_amd import _lib, ops
+from uc2_amd.ops.cross import _CrossAttn, _CrossAttnGrad
+
+P = 4096                        # an aligned address; no check dereferences it
+
+
+def attn(**kw):
+    d = dict(dtype=1, B=2, Lq=3, Lk=5, nh=4, nkv=2, D=64, scale=0.125, drop_p=0.0, q=P, k=P, v=P, q_sb=768, q_sl=256, q_sh=64, k_sb=640, k_sl=128, k_sh=64, v_sb=640,
+             v_sl=128, v_sh=64, out=P, o_sb=768, o_sl=256, o_sh=64, lse=P)
+    d.update(kw)
+    return _CrossAttn(**d)
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=2), dict(D=48), dict(D=0), dict(nkv=3), dict(nkv=0), dict(B=-1), dict(Lq=-1), dict(Lk=-2), dict(drop_p=1.0), dict(drop_p=-0.5), dict(q=0),
+                                 dict(k=0), dict(out=0), dict(q=P + 2), dict(v=P + 8), dict(q_sl=257), dict(k_sh=4), dict(o_sb=-8), dict(Lq=1 << 30)])
+def test_cross_attention_argument_errors(bad):
+    lib = _lib.load()
+    assert lib.uc2_xattn_fwd(ctypes.byref(attn(**bad)), None, 0, None) == -1
+    assert lib.uc2_last_error()
+
+
+def test_cross_attention_backward_argument_errors():
+    lib = _lib.load()
+    g = dict(dout=P, dout_sb=768, dout_sl=256, dout_sh=64, dq=P, dk=P, dv=P, dq_sb=768, dq_sl=256, dq_sh=64, dk_sb=640, dk_sl=128, dk_sh=64, dv_sb=640, dv_sl=128, dv_sh=64)
+    need = lib.uc2_xattn_workspace(ctypes.byref(attn()), 1)
+    assert need > 0
+    for a, gb, ws, n in ((attn(lse=0), g, P, need), (attn(), dict(g, dq=0), P, need), (attn(), dict(g, dk=0), P, need), (attn(), dict(g, dout_sl=3), P, need),
+                         (attn(), dict(g, dv=P + 4), P, need), (attn(), g, None, need), (attn(), g, P, need - 1), (attn(), g, P + 4, need)):
+        assert lib.uc2_xattn_bwd(ctypes.byref(a), ctypes.byref(_CrossAttnGrad(**gb)), ws, n, None) == -1
+    assert lib.uc2_xattn_bwd(ctypes.byref(attn()), None, P, need, None) == -1
+    assert lib.uc2_xattn_fwd(None, None, 0, None) == -1
+    # a long axis split over workgroups needs its workspace
+    long = attn(B=1, Lq=1, Lk=100000, nkv=4, q_sl=256)
+    n = lib.uc2_xattn_workspace(ctypes.byref(long), 0)
+    assert n > 0 and lib.uc2_xattn_fwd(ctypes.byref(long), None, 0, None) == -1 and lib.uc2_xattn_fwd(ctypes.byref(long), P, n - 1, None) == -1
+    assert lib.uc2_xattn_workspace(ctypes.byref(attn(B=4000, Lk=64)), 0) == 0
+    assert lib.uc2_xattn_workspace(ctypes.byref(attn(D=7)), 0) == 0
+
+
+def test_empty_calls_launch_nothing():
+    lib = _lib.load()
+    assert lib.uc2_xattn_fwd(ctypes.byref(attn(B=0)), None, 0, None) == 0
+    assert lib.uc2_xattn_fwd(ctypes.byref(attn(Lq=0)), None, 0, None) == 0
+    assert lib.uc2_gemm_fp8_block(0, 5, 128, None, 128, None, 0, None, 128, None, None, None, 5, None) == 0
+    assert lib.uc2_fp8_quant_rows(1, 0, 128, None, 128, None, None, None) == 0
+    assert lib.uc2_rms_fwd(1, 0, 128, None, None, None, 1e-6, None, None, None, None, None, None) == 0
+
+
+def test_block_argument_errors():
+    lib = _lib.load()
+    ok = [4, 8, 256, P, 256, P, 4, P, 256, P, None, P, 8, None]
+    for i, bad in ((0, -1), (1, -1), (2, 0), (3, None), (3, P + 8), (4, 128), (4, 264), (5, None), (5, P + 2), (6, 3), (7, None), (7, P + 4), (8, 128), (9, None), (11, None), (11, P + 1),
+                   (12, 7), (10, P + 2)):
+        a = list(ok)
+        a[i] = bad
+        assert lib.uc2_gemm_fp8_block(*a) == -1, (i, bad)
+    for a in ((2, 4, 128, P, 128, P, P, None), (1, -1, 128, P, 128, P, P, None), (1, 4, 0, P, 128, P, P, None), (1, 4, 128, P, 127, P, P, None), (1, 4, 128, None, 128, P, P, None),
+              (1, 4, 128, P, 128, P + 4, P, None), (1, 4, 128, P, 128, P, P + 1, None)):
+        assert lib.uc2_fp8_quant_rows(*a) == -1
+    for a in ((3, 4, 128, P, 128, P, P, None, None, None), (1, 4, 128, P, 100, P, P, None, None, None), (1, 4, 128, P, 128, P, P, P, None, None), (1, 4, 128, P, 128, P, None, None, None, None),
+              (1, 4, 128, P, 128, P + 1, P, None, None, None), (1, 1 << 24, 128, P, 128, P, P, None, None, None)):
+        assert lib.uc2_fp8_quant_square(*a) == -1
+
+
+def test_rms_argument_errors():
+    lib = _lib.load()
+    ok = [1, 4, 128, P, P, P, 1e-6, P, P, P, P, P, None]
+    for i, bad in ((0, 5), (1, -1), (2, 0), (2, 16385), (3, None), (4, None), (5, None), (6, -1.0), (7, None), (10, None), (11, None), (10, P + 4), (11, P + 2)):
+        a = list(ok)
+        a[i] = bad
+        assert lib.uc2_rms_fwd(*a) == -1, (i, bad)
+    assert lib.uc2_rms_fwd(1, 4, 128, P, None, P, 1e-6, None, None, None, None, None, None) == -1     # no output at all
+    n = lib.uc2_rms_bwd_workspace(4, 128)
+    ok = [1, 4, 128, P, P, P, P, P, P, P, P, n, None]
+    for i, bad in ((0, 5), (1, -1), (2, 16385), (3, None), (5, None), (6, None), (7, None), (8, None), (10, None), (10, P + 2), (11, n - 1)):
+        a = list(ok)
+        a[i] = bad
+        assert lib.uc2_rms_bwd(*a) == -1, (i, bad)
+    assert lib.uc2_rms_bwd_workspace(0, 128) == 0 and lib.uc2_rms_bwd_workspace(4, 20000) == 0
+
+
+def test_cpu_tensors_are_refused():
+    x, w, g = torch.zeros(4, 128, dtype=torch.bfloat16), torch.zeros(8, 128), torch.ones(128)
+    q = torch.zeros(1, 2, 4, 64)
+    for f in (lambda: ops.fp8_quantize_block(x), lambda: ops.fp8_quantize_weight_block(w), lambda: ops.linear_fp8_block(x, w), lambda: ops.rms_norm(x, g), lambda: ops.rms_norm_fp8(x, g),
+              lambda: ops.cross_attention(q, q, q), lambda: ops.fp8_quantize_weight_block(g),
+              lambda: ops.gemm_fp8_block(ops.BlockRows(torch.zeros(4, 128, dtype=torch.uint8), torch.zeros(1, 4, dtype=torch.int32), 128),
+                                         ops.BlockWeight(torch.zeros(8, 128, dtype=torch.uint8), torch.zeros(1, 1, dtype=torch.uint8)))):
+        with pytest.raises(_lib.Uc2Error):
+            f()
+
+
+def test_structures_match_the_header():
+    """sizes as a C compiler lays the header's structures out (pointers of 8 bytes)"""
+    assert ctypes.sizeof(_CrossAttn) == 216 and ctypes.sizeof(_CrossAttnGrad) == 128
+
+
+def test_oracle_rounds_as_torch_does():
+    """block_ref's e4m3 against torch's own cast, and its exponents against their definition"""
+    x = torch.randn(4000, dtype=torch.float64) * torch.exp(2 * torch.randn(4000, dtype=torch.float64))
+    x = x[x.abs() <= 448].float()
+    assert torch.equal(R.e4m3(x.double()), x.to(torch.float8_e4m3fn).double())
+    every = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    every = every[torch.isfinite(every)]
+    assert torch.equal(R.e4m3(every), every)
+    e = R.block_exponents(torch.tensor([448.0, 448.1, 224.0, 1.75, 1.76, 0.0]))
+    assert e.tolist() == [127, 128, 126, 119, 120, 1]
+
+
+def test_oracle_attention_is_softmax():
+    q, k, v = torch.randn(2, 5, 4, 32), torch.randn(2, 7, 2, 32), torch.randn(2, 7, 2, 32)
+    dout = torch.randn(2, 5, 4, 32)
+    leaves = [t.double().requires_grad_() for t in (q, k, v)]
+    t = lambda a: a.repeat_interleave(4 // a.shape[2], 2).transpose(1, 2)  # noqa: E731
+    o = (torch.softmax(t(leaves[0]) @ t(leaves[1]).transpose(2, 3) * 0.2, -1) @ t(leaves[2])).transpose(1, 2)
+    want = [o, *torch.autograd.grad(o, leaves, dout.double())]
+    got, _ = R.attention(q, k, v, 0.2, None, None, dout)
+    for a, b in zip(got, want):
+        assert torch.allclose(a, b.detach(), atol=1e-12)

@@ -15,7 +15,7 @@ from .config import cfg
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = cfg.lib_path      # (UC2_LIB_PATH: A/B of two builds on one box)
 _lib = None
-ABI_VERSION = 13         # include/uc2_hip.h; bumped whenever a signature changes
+ABI_VERSION = 14         # include/uc2_hip.h; bumped whenever a signature changes
 
 P, I, F, U64, I64, SZ = c_void_p, c_int, c_float, c_uint64, c_int64, c_size_t
 
@@ -61,6 +61,15 @@ SIGNATURES = {
     "uc2_attn_general_fwd": (I, [I, I, I, I, I, I, P, I, P, I, P, I, P, P, F, P, I, P, F, P, U64, P]),
     "uc2_attn_general_bwd": (I, [I, I, I, I, I, I, P, I, P, I, P, I, P, P, F, P, P, I, P, P, P, I, P, I, P, I, F, P, U64, P]),
     "uc2_attn_general_probs_mean": (I, [I, I, I, I, I, I, P, I, P, I, P, P, F, P, P, F, P, U64, P]),
+    "uc2_xattn_workspace": (SZ, [P, I]),
+    "uc2_xattn_fwd": (I, [P, P, SZ, P]),
+    "uc2_xattn_bwd": (I, [P, P, P, SZ, P]),
+    "uc2_fp8_quant_rows": (I, [I, I, I, P, I64, P, P, P]),
+    "uc2_fp8_quant_square": (I, [I, I, I, P, I64, P, P, P, P, P]),
+    "uc2_gemm_fp8_block": (I, [I, I, I, P, I, P, I, P, I, P, P, P, I, P]),
+    "uc2_rms_fwd": (I, [I, I, I, P, P, P, F, P, P, P, P, P, P]),
+    "uc2_rms_bwd_workspace": (SZ, [I, I]),
+    "uc2_rms_bwd": (I, [I, I, I, P, P, P, P, P, P, P, P, SZ, P]),
     "uc2_position_ids": (I, [I, I, P, I64, P, P]),
     "uc2_embed_fwd": (I, [I, I, I, P, P, P, I, P, P, P, P, P]),
     "uc2_embed_bwd": (I, [I, I, I, P, P, P, P, P, P, P, I64, I64, P]),

@@ -1,0 +1,743 @@
+// Attention from one sequence to the states of another (cross attention): queries [B, Lq, nh, D], keys / values [B, Lk, nkv, D], every
+// tensor with its own batch / row / head strides (a fused projection's slices are read in place), nkv dividing nh.
+//   x = scale q k^T + key_mask[b, key];  p = softmax_key(x) over the keys that take part;  out = p v
+// A key takes no part behind its sequence's length k_lens[b] or where key_mask <= UC2_XATTN_REMOVED (-1e30, -inf included): whatever
+// its k / v rows hold (NaN of a padded buffer too) reaches nothing, its gradients are zero.  A row without any key gives zeros and
+// passes no gradient.  The softmax runs online in one pass over the keys; scores never reach memory, only one fp32 log2-sum-exp per row.
+//
+// One skeleton for the three kernels, on the 32 x 32 matrix instructions.  A wave OWNS 32 columns -- packed query rows
+// r = i G + g of the G = nh / nkv heads that share a key head (forward, dQ), or keys (dK / dV) -- whose vectors stay in registers as the
+// second operand.  The other side STREAMS through LDS in tiles of TT rows, double-buffered, staged through registers so that rows that take no
+// part become zeros on the way.  The product (streamed rows x owned columns) leaves a lane with ONE owned column (lane & 31) and 16
+// streamed rows per block: the softmax's maximum, sum and rescaling are lane-local but for one exchange between the wave's halves, and
+// the weights feed the second product (contraction over streamed rows) straight from the accumulator registers: the order in which that
+// product sums its rows is free, so the streamed tile is read transposed (ds_read_b64_tr_b16) in the accumulator's own row order.
+// dK / dV of a shared head sum over its G heads by streaming all their rows.  Sums are made in a fixed order: no atomics, same bits every run.
+//
+// When the owned tiles alone do not fill the chip (single tokens, short batches), the streamed axis is split over workgroups into fp32
+// partials (outputs with maximum and sum; gradients), joined by a second small kernel.
+#include "../../include/uc2_hip.h"
+#include "common.h"
+
+typedef __attribute__((ext_vector_type(4))) __bf16 xa_bf16x4;
+
+#define XA_LOG2E 1.4426950408889634f
+#define XA_REMOVED (-1e30f)
+
+struct XaView { const char* p; long long sb, sl, sh; };          // byte strides of batch, row, head
+struct XaOut { char* p; long long sb, sl, sh; };
+
+struct XaArgs {
+  int B, Lq, Lk, nkv, G, R;                                       // R = Lq G packed rows per (batch, key head)
+  int tiles, splits, BH;                                          // owned tiles per (batch, key head), splits of the streamed axis, B nkv
+  XaView q, k, v, o, dout;
+  XaOut out, dq, dk, dv;
+  const float* kmask; long long kmask_sb; const int* klens;
+  float scale, scale2;                                            // scale2 = scale log2 e
+  float* lse; float* delta;                                       // [B nkv][R], lse in base 2
+  float* part; float* pml;                                        // partials: [splits][B nkv][rows][..], maxima and sums [splits][B nkv][R][2]
+  uint32_t thresh; float keep_scale; const uint64_t* seed_ptr; uint64_t seed_imm; int nh;
+};
+
+template <typename T, int D> struct XaCfg {
+  static constexpr int RB = D * (int)sizeof(T);                   // bytes of a row
+  static constexpr int CPR = RB / 16;                             // 16-byte chunks of a row
+  // streamed rows per tile: 64 rows of 128 bytes or less, 32 longer ones: 32 KiB of LDS for two double-buffered tensors (64 KiB for fp32
+  // at D = 128), and at most 128 staging registers in a workgroup of one wave
+  static constexpr int TT = RB <= 128 ? 64 : 32;
+  static constexpr int NB = TT / 32;                              // 32-row blocks per tile
+  static constexpr int KS = sizeof(T) == 2 ? D / 16 : D / 8;      // chunks a lane holds of an owned vector
+  static constexpr int DB = D / 32;                               // 32-wide blocks of the head dimension
+};
+
+// chunk swizzle of a row: 8 consecutive rows of one chunk column fall on 8 distinct 16-byte bank groups (row reads), and so do the 4 rows x 2
+// chunks of a transposing read
+template <int CPR> __device__ __forceinline__ int xa_swz(int row) {
+  return CPR == 4 ? ((row & 2) | ((row >> 2) & 1)) : (((row & 3) << 1) | ((row >> 2) & 1));
+}
+
+template <typename T, int D> struct XaMma;
+template <int D> struct XaMma<bf16, D> {
+  typedef XaCfg<bf16, D> C;
+  typedef bf16x8 Frag;
+  // acc[16] = rows blk*32.. of the tile (lane's row: lane & 31) against the owned vectors
+  static __device__ __forceinline__ f32x16 rows(const char* lds, int blk, const Frag (&own)[C::KS], int lane) {
+    const int row = blk * 32 + (lane & 31), h = lane >> 5, sw = xa_swz<C::CPR>(row);
+    f32x16 acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < C::KS; ++s) {
+      const bf16x8 a = *reinterpret_cast<const bf16x8*>(lds + row * C::RB + (((2 * s + h) ^ sw) << 4));
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, own[s], acc, 0, 0, 0);
+    }
+    return acc;
+  }
+  // out[db] (head dimension x owned columns) += tile rows^T x w[16] (the accumulator order of rows())
+  static __device__ __forceinline__ void cols(const char* lds, int blk, const float (&w)[16], f32x16 (&out)[C::DB], int lane) {
+    const int h = lane >> 5, i = lane & 15, dh = (lane >> 4) & 1;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      bf16x8 b;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[j] = (bf16)w[8 * ks + j];
+      const int row0 = blk * 32 + 16 * ks + 4 * h + (i >> 2), row1 = row0 + 8;
+#pragma unroll
+      for (int db = 0; db < C::DB; ++db) {
+        const int c = 4 * db + 2 * dh + ((i >> 1) & 1), sub = (i & 1) * 8;
+        typedef __attribute__((address_space(3))) short4v* lp;
+        const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + row0 * C::RB + ((c ^ xa_swz<C::CPR>(row0)) << 4) + sub));
+        const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + row1 * C::RB + ((c ^ xa_swz<C::CPR>(row1)) << 4) + sub));
+        const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        out[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, out[db], 0, 0, 0);
+      }
+    }
+  }
+};
+template <int D> struct XaMma<float, D> {
+  typedef XaCfg<float, D> C;
+  typedef f32x4 Frag;
+  static __device__ __forceinline__ f32x16 rows(const char* lds, int blk, const Frag (&own)[C::KS], int lane) {
+    const int row = blk * 32 + (lane & 31), h = lane >> 5, sw = xa_swz<C::CPR>(row);
+    f32x16 acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < C::KS; ++s) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(lds + row * C::RB + (((2 * s + h) ^ sw) << 4));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], own[s][j], acc, 0, 0, 0);
+    }
+    return acc;
+  }
+  static __device__ __forceinline__ void cols(const char* lds, int blk, const float (&w)[16], f32x16 (&out)[C::DB], int lane) {
+    const int h = lane >> 5, l31 = lane & 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = blk * 32 + 8 * (r >> 2) + 4 * h + (r & 3), sw = xa_swz<C::CPR>(row);
+#pragma unroll
+      for (int db = 0; db < C::DB; ++db) {
+        const float a = *reinterpret_cast<const float*>(lds + row * C::RB + (((8 * db + (l31 >> 2)) ^ sw) << 4) + (l31 & 3) * 4);
+        out[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w[r], out[db], 0, 0, 0);
+      }
+    }
+  }
+};
+
+// position of packed row r: (query i, head g of the group)
+__device__ __forceinline__ void xa_split(const XaArgs& a, int r, int& i, int& g) {
+  if (a.G == 1) { i = r; g = 0; } else { i = (int)((unsigned)r / (unsigned)a.G); g = r - i * a.G; }
+}
+// rows of a key-like tensor (PACKED false) or of a query-like one (packed rows)
+template <bool PACKED> __device__ __forceinline__ const char* xa_row(const XaArgs& a, const XaView& x, int b, int kvh, int r) {
+  if (!PACKED) return x.p + b * x.sb + (long long)r * x.sl + kvh * x.sh;
+  int i, g;
+  xa_split(a, r, i, g);
+  return x.p + b * x.sb + (long long)i * x.sl + (long long)(kvh * a.G + g) * x.sh;
+}
+__device__ __forceinline__ float xa_key_bias(const XaArgs& a, int b, int key, int len) {     // base-2 additive mask; -inf: no part
+  if (key >= len) return -INFINITY;
+  if (!a.kmask) return 0.f;
+  const float m = a.kmask[b * a.kmask_sb + key];
+  return m <= XA_REMOVED ? -INFINITY : m * XA_LOG2E;
+}
+
+// staging of TT rows x D of two tensors by NT threads, through registers
+template <typename T, int D, int NT, bool PACKED> struct XaStage {
+  typedef XaCfg<T, D> C;
+  static constexpr int N = C::TT * C::CPR / NT;                  // chunks per thread and tensor
+  static_assert(N >= 1 && C::TT * C::CPR % NT == 0, "");
+  uint4 x[N], y[N];
+  __device__ __forceinline__ void load(const XaArgs& a, const XaView& X, const XaView& Y, int b, int kvh, int row0, int limit, int t) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int idx = t + n * NT, row = row0 + idx / C::CPR, c = idx % C::CPR;
+      bool take = row < limit;
+      if (!PACKED && take && a.kmask) take = !(a.kmask[b * a.kmask_sb + row] <= XA_REMOVED);
+      x[n] = uint4{0, 0, 0, 0}; y[n] = uint4{0, 0, 0, 0};
+      if (take) {
+        x[n] = *reinterpret_cast<const uint4*>(xa_row<PACKED>(a, X, b, kvh, row) + c * 16);
+        y[n] = *reinterpret_cast<const uint4*>(xa_row<PACKED>(a, Y, b, kvh, row) + c * 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* lx, char* ly, int t) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int idx = t + n * NT, row = idx / C::CPR, c = idx % C::CPR;
+      const int off = row * C::RB + ((c ^ xa_swz<C::CPR>(row)) << 4);
+      *reinterpret_cast<uint4*>(lx + off) = x[n];
+      *reinterpret_cast<uint4*>(ly + off) = y[n];
+    }
+  }
+};
+
+// owned vectors of the lane: column r (query row or key), zeros where it takes no part
+template <typename T, int D, bool PACKED>
+__device__ __forceinline__ void xa_own(const XaArgs& a, const XaView& X, int b, int kvh, int r, bool take, int lane, typename XaMma<T, D>::Frag (&f)[XaCfg<T, D>::KS]) {
+  typedef typename XaMma<T, D>::Frag Frag;
+  const int h = lane >> 5;
+  if (take) {
+    const char* p = xa_row<PACKED>(a, X, b, kvh, r);
+#pragma unroll
+    for (int s = 0; s < XaCfg<T, D>::KS; ++s) f[s] = *reinterpret_cast<const Frag*>(p + (2 * s + h) * 16);
+  } else {
+#pragma unroll
+    for (int s = 0; s < XaCfg<T, D>::KS; ++s) f[s] = __builtin_bit_cast(Frag, uint4{0, 0, 0, 0});
+  }
+}
+// 4 consecutive values of the head dimension
+__device__ __forceinline__ void xa_put4(bf16* p, float a, float b, float c, float d) {
+  *reinterpret_cast<xa_bf16x4*>(p) = xa_bf16x4{(bf16)a, (bf16)b, (bf16)c, (bf16)d};
+}
+__device__ __forceinline__ void xa_put4(float* p, float a, float b, float c, float d) { *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d); }
+template <typename T, int DB> __device__ __forceinline__ void xa_put_row(char* row, const f32x16 (&o)[DB], float mul, int lane) {
+  T* p = reinterpret_cast<T*>(row) + 4 * (lane >> 5);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) xa_put4(p + 32 * db + 8 * k, o[db][4 * k] * mul, o[db][4 * k + 1] * mul, o[db][4 * k + 2] * mul, o[db][4 * k + 3] * mul);
+}
+
+// block -> (batch and key head, owned tile, split): blocks go to the 8 XCDs in turn, the tiles and splits of one (batch, key head) share its
+// streamed rows, so they are put on one XCD and its L2 (worth nothing below 8 heads: plain order there)
+__device__ __forceinline__ bool xa_block(const XaArgs& a, int& bh, int& tile, int& split) {
+  const int per = a.tiles * a.splits;
+  int blk = blockIdx.x;
+  if (a.BH >= 8) {
+    const int x = blk & 7, n = blk >> 3, grp = n / per;
+    bh = grp * 8 + x;
+    blk = n - grp * per;
+  } else {
+    bh = blk / per;
+    blk -= bh * per;
+  }
+  tile = blk / a.splits;
+  split = blk - tile * a.splits;
+  return bh < a.BH;
+}
+__device__ __forceinline__ int xa_len(const XaArgs& a, int b) { return a.klens ? max(0, min(a.klens[b], a.Lk)) : a.Lk; }
+
+template <typename T, int D, int NS, bool DROP>
+__global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
+  typedef XaCfg<T, D> C;
+  typedef XaMma<T, D> M;
+  __shared__ __attribute__((aligned(16))) char lk[2][C::TT * C::RB], lv[2][C::TT * C::RB];
+  __shared__ __attribute__((aligned(16))) float lb[2][C::TT];
+  __shared__ __attribute__((aligned(16))) uint32_t lh[2][DROP ? C::TT : 4];
+  int bh, tile, split;
+  if (!xa_block(a, bh, tile, split)) return;
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, b = bh / a.nkv, kvh = bh - b * a.nkv;
+  const int r = (tile * NS + w) * 32 + (lane & 31);
+  const bool mine = r < a.R;
+  const int len = xa_len(a, b), nt = (len + C::TT - 1) / C::TT, per = (nt + a.splits - 1) / a.splits;
+  const int t0 = split * per, t1 = min(nt, t0 + per);
+  const uint64_t seed = DROP ? a.seed_imm + (a.seed_ptr ? *a.seed_ptr : 0ull) : 0ull;
+  uint32_t hq = 0;
+  if (DROP && mine) { int i, g; xa_split(a, r, i, g); hq = attn_line_hash(seed, b * a.nh + kvh * a.G + g, i, UC2_ATTN_SALT_Q); }
+
+  typename M::Frag q[C::KS];
+  xa_own<T, D, true>(a, a.q, b, kvh, r, mine, lane, q);
+  f32x16 o[C::DB];
+#pragma unroll
+  for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  XaStage<T, D, NS * 64, false> st;
+  float bias = 0.f; uint32_t hash = 0;
+  auto fetch = [&](int tt) __attribute__((always_inline)) {
+    st.load(a, a.k, a.v, b, kvh, tt * C::TT, len, t);
+    if (t < C::TT) {
+      bias = xa_key_bias(a, b, tt * C::TT + t, len);
+      if (DROP) hash = attn_line_hash(seed, bh, tt * C::TT + t, UC2_ATTN_SALT_K);
+    }
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+    st.store(lk[buf], lv[buf], t);
+    if (t < C::TT) { lb[buf][t] = bias; if (DROP) lh[buf][t] = hash; }
+  };
+  if (t0 < t1) { fetch(t0); put(0); }
+  __syncthreads();
+  int buf = 0;
+  for (int tt = t0; tt < t1; ++tt) {
+    if (tt + 1 < t1) fetch(tt + 1);
+    f32x16 s[C::NB];
+#pragma unroll
+    for (int n = 0; n < C::NB; ++n) s[n] = M::rows(lk[buf], n, q, lane);
+    // x = score in base 2, masked; its maximum over the tile
+    float mx = -INFINITY;
+    const bool masked = a.kmask != nullptr || (tt + 1) * C::TT > len;
+#pragma unroll
+    for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f32x4 bv = {0.f, 0.f, 0.f, 0.f};
+        if (masked) bv = *reinterpret_cast<const f32x4*>(&lb[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { s[n][4 * k + e] = fmaf(s[n][4 * k + e], a.scale2, bv[e]); mx = fmaxf(mx, s[n][4 * k + e]); }
+      }
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__any(mx > m)) {
+      const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= al;
+#pragma unroll
+      for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[db][e] *= al;
+      m = mn;
+    }
+    const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int n = 0; n < C::NB; ++n) {
+      float p[16];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint4 hk = {0, 0, 0, 0};
+        if (DROP) hk = *reinterpret_cast<const uint4*>(&lh[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+        const uint32_t hh[4] = {hk.x, hk.y, hk.z, hk.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = __builtin_amdgcn_exp2f(s[n][4 * k + e] - mu);
+          l += v;
+          p[4 * k + e] = DROP ? (attn_keep(hq, hh[e], a.thresh) ? v * a.keep_scale : 0.f) : v;
+        }
+      }
+      M::cols(lv[buf], n, p, o, lane);
+    }
+    if (tt + 1 < t1) put(buf ^ 1);
+    __syncthreads();
+    buf ^= 1;
+  }
+  l += __shfl_xor(l, 32);
+  if (!mine) return;
+  if (a.splits == 1) {
+    int i, g;
+    xa_split(a, r, i, g);
+    const float inv = l > 0.f ? 1.0f / l : (l == l ? 0.f : l);     // no key: zeros; NaN stays NaN
+    xa_put_row<T, C::DB>(a.out.p + b * a.out.sb + (long long)i * a.out.sl + (long long)(kvh * a.G + g) * a.out.sh, o, inv, lane);
+    if (a.lse && lane < 32) a.lse[(size_t)bh * a.R + r] = m + __log2f(l);
+  } else {
+    const size_t row = ((size_t)split * a.BH + bh) * a.R + r;
+    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.part + row * D), o, 1.0f, lane);
+    if (lane < 32) { a.pml[2 * row] = m; a.pml[2 * row + 1] = l; }
+  }
+}
+
+// joins the splits of the forward: a wave per row, lane = element (two per lane at D = 128, half the lanes idle at 32)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a) {
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (long long)a.BH * a.R;
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 63, bh = (int)(row / a.R), r = (int)(row - (long long)bh * a.R);
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.pml[2 * (s * rows + row)]);
+  const float mu = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[2] = {0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const size_t at = s * rows + row;
+    const float f = __builtin_amdgcn_exp2f(a.pml[2 * at] - mu);
+    l += f * a.pml[2 * at + 1];
+    if (D >= 64 || lane < D) o[0] += f * a.part[at * D + lane];
+    if (D == 128) o[1] += f * a.part[at * D + 64 + lane];
+  }
+  const float inv = l > 0.f ? 1.0f / l : (l == l ? 0.f : l);
+  const int b = bh / a.nkv, kvh = bh - b * a.nkv;
+  int i, g;
+  xa_split(a, r, i, g);
+  T* out = reinterpret_cast<T*>(a.out.p + b * a.out.sb + (long long)i * a.out.sl + (long long)(kvh * a.G + g) * a.out.sh);
+  if (D >= 64 || lane < D) out[lane] = from_f<T>(o[0] * inv);
+  if (D == 128) out[64 + lane] = from_f<T>(o[1] * inv);
+  if (a.lse && lane == 0) a.lse[row] = m + __log2f(l);
+}
+
+// dQ (owned query rows, streamed keys) and delta[r] = dout . out, which the dK / dV kernel reads
+//   dx = p (dp - delta),  dp = dout v^T (dropped as the forward's weights were),  dq = scale dx k
+template <typename T, int D, int NS, bool DROP>
+__global__ __launch_bounds__(NS * 64) void xattn_dq_kernel(XaArgs a) {
+  typedef XaCfg<T, D> C;
+  typedef XaMma<T, D> M;
+  __shared__ __attribute__((aligned(16))) char lk[2][C::TT * C::RB], lv[2][C::TT * C::RB];
+  __shared__ __attribute__((aligned(16))) float lb[2][C::TT];
+  __shared__ __attribute__((aligned(16))) uint32_t lh[2][DROP ? C::TT : 4];
+  int bh, tile, split;
+  if (!xa_block(a, bh, tile, split)) return;
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, b = bh / a.nkv, kvh = bh - b * a.nkv;
+  const int r = (tile * NS + w) * 32 + (lane & 31);
+  const bool mine = r < a.R;
+  const int len = xa_len(a, b), nt = (len + C::TT - 1) / C::TT, per = (nt + a.splits - 1) / a.splits;
+  const int t0 = split * per, t1 = min(nt, t0 + per);
+  const uint64_t seed = DROP ? a.seed_imm + (a.seed_ptr ? *a.seed_ptr : 0ull) : 0ull;
+  uint32_t hq = 0;
+  if (DROP && mine) { int i, g; xa_split(a, r, i, g); hq = attn_line_hash(seed, b * a.nh + kvh * a.G + g, i, UC2_ATTN_SALT_Q); }
+
+  typename M::Frag q[C::KS], go[C::KS];
+  xa_own<T, D, true>(a, a.q, b, kvh, r, mine, lane, q);
+  xa_own<T, D, true>(a, a.dout, b, kvh, r, mine, lane, go);
+  float delta = 0.f, lse = INFINITY;
+  {
+    typename M::Frag of[C::KS];
+    xa_own<T, D, true>(a, a.o, b, kvh, r, mine, lane, of);
+#pragma unroll
+    for (int s = 0; s < C::KS; ++s)
+#pragma unroll
+      for (int j = 0; j < (int)(16 / sizeof(T)); ++j) delta = fmaf((float)of[s][j], (float)go[s][j], delta);
+    delta += __shfl_xor(delta, 32);
+  }
+  if (mine) {
+    lse = a.lse[(size_t)bh * a.R + r];
+    if (lse == -INFINITY) lse = INFINITY;                          // a row without any key: p = 0
+    if (split == 0 && lane < 32) a.delta[(size_t)bh * a.R + r] = delta;
+  }
+  f32x16 dq[C::DB];
+#pragma unroll
+  for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dq[db][e] = 0.f;
+  XaStage<T, D, NS * 64, false> st;
+  float bias = 0.f; uint32_t hash = 0;
+  auto fetch = [&](int tt) __attribute__((always_inline)) {
+    st.load(a, a.k, a.v, b, kvh, tt * C::TT, len, t);
+    if (t < C::TT) {
+      bias = xa_key_bias(a, b, tt * C::TT + t, len);
+      if (DROP) hash = attn_line_hash(seed, bh, tt * C::TT + t, UC2_ATTN_SALT_K);
+    }
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+    st.store(lk[buf], lv[buf], t);
+    if (t < C::TT) { lb[buf][t] = bias; if (DROP) lh[buf][t] = hash; }
+  };
+  if (t0 < t1) { fetch(t0); put(0); }
+  __syncthreads();
+  int buf = 0;
+  for (int tt = t0; tt < t1; ++tt) {
+    if (tt + 1 < t1) fetch(tt + 1);
+    const bool masked = a.kmask != nullptr || (tt + 1) * C::TT > len;
+#pragma unroll
+    for (int n = 0; n < C::NB; ++n) {
+      const f32x16 s = M::rows(lk[buf], n, q, lane);
+      const f32x16 dp = M::rows(lv[buf], n, go, lane);
+      float ds[16];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f32x4 bv = {0.f, 0.f, 0.f, 0.f};
+        uint4 hk = {0, 0, 0, 0};
+        if (masked) bv = *reinterpret_cast<const f32x4*>(&lb[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+        if (DROP) hk = *reinterpret_cast<const uint4*>(&lh[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+        const uint32_t hh[4] = {hk.x, hk.y, hk.z, hk.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * k + e], a.scale2, bv[e]) - lse);
+          const float d = DROP ? (attn_keep(hq, hh[e], a.thresh) ? dp[4 * k + e] * a.keep_scale : 0.f) : dp[4 * k + e];
+          ds[4 * k + e] = p * (d - delta);
+        }
+      }
+      M::cols(lk[buf], n, ds, dq, lane);
+    }
+    if (tt + 1 < t1) put(buf ^ 1);
+    __syncthreads();
+    buf ^= 1;
+  }
+  if (!mine) return;
+  if (a.splits == 1) {
+    int i, g;
+    xa_split(a, r, i, g);
+    xa_put_row<T, C::DB>(a.dq.p + b * a.dq.sb + (long long)i * a.dq.sl + (long long)(kvh * a.G + g) * a.dq.sh, dq, a.scale, lane);
+  } else {
+    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.part + (((size_t)split * a.BH + bh) * a.R + r) * D), dq, a.scale, lane);
+  }
+}
+
+// dK, dV (owned keys, streamed packed query rows):  dv = p^T dout,  dk = scale dx^T q
+template <typename T, int D, int NS, bool DROP>
+__global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
+  typedef XaCfg<T, D> C;
+  typedef XaMma<T, D> M;
+  __shared__ __attribute__((aligned(16))) char lq[2][C::TT * C::RB], lg[2][C::TT * C::RB];
+  __shared__ __attribute__((aligned(16))) float ls[2][C::TT], ld[2][C::TT];
+  __shared__ __attribute__((aligned(16))) uint32_t lh[2][DROP ? C::TT : 4];
+  int bh, tile, split;
+  if (!xa_block(a, bh, tile, split)) return;
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, b = bh / a.nkv, kvh = bh - b * a.nkv;
+  const int key = (tile * NS + w) * 32 + (lane & 31);
+  const int len = xa_len(a, b);
+  const float bias = xa_key_bias(a, b, key, len);
+  const bool part = bias != -INFINITY;
+  const int nt = tile * NS * 32 < len ? (a.R + C::TT - 1) / C::TT : 0;          // a tile behind the length: zeros
+  const int per = (nt + a.splits - 1) / a.splits;
+  const int t0 = split * per, t1 = min(nt, t0 + per);
+  const uint64_t seed = DROP ? a.seed_imm + (a.seed_ptr ? *a.seed_ptr : 0ull) : 0ull;
+  const uint32_t hk = DROP ? attn_line_hash(seed, bh, key, UC2_ATTN_SALT_K) : 0u;
+
+  typename M::Frag kf[C::KS], vf[C::KS];
+  xa_own<T, D, false>(a, a.k, b, kvh, key, part, lane, kf);
+  xa_own<T, D, false>(a, a.v, b, kvh, key, part, lane, vf);
+  f32x16 dk[C::DB], dv[C::DB];
+#pragma unroll
+  for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) { dk[db][e] = 0.f; dv[db][e] = 0.f; }
+  XaStage<T, D, NS * 64, true> st;
+  float lse = 0.f, delta = 0.f; uint32_t hash = 0;
+  auto fetch = [&](int tt) __attribute__((always_inline)) {
+    st.load(a, a.q, a.dout, b, kvh, tt * C::TT, a.R, t);
+    if (t < C::TT) {
+      const int r = tt * C::TT + t;
+      lse = INFINITY; delta = 0.f;                                 // behind the last row, and rows without any key: p = 0
+      if (r < a.R) {
+        lse = a.lse[(size_t)bh * a.R + r];
+        if (lse == -INFINITY) lse = INFINITY;
+        delta = a.delta[(size_t)bh * a.R + r];
+        if (DROP) { int i, g; xa_split(a, r, i, g); hash = attn_line_hash(seed, b * a.nh + kvh * a.G + g, i, UC2_ATTN_SALT_Q); }
+      }
+    }
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+    st.store(lq[buf], lg[buf], t);
+    if (t < C::TT) { ls[buf][t] = lse; ld[buf][t] = delta; if (DROP) lh[buf][t] = hash; }
+  };
+  if (t0 < t1) { fetch(t0); put(0); }
+  __syncthreads();
+  int buf = 0;
+  for (int tt = t0; tt < t1; ++tt) {
+    if (tt + 1 < t1) fetch(tt + 1);
+#pragma unroll
+    for (int n = 0; n < C::NB; ++n) {
+      const f32x16 s = M::rows(lq[buf], n, kf, lane);
+      const f32x16 dp = M::rows(lg[buf], n, vf, lane);
+      float p[16], ds[16];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int at = n * 32 + 8 * k + 4 * (lane >> 5);
+        const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[buf][at]), dl = *reinterpret_cast<const f32x4*>(&ld[buf][at]);
+        uint4 hv = {0, 0, 0, 0};
+        if (DROP) hv = *reinterpret_cast<const uint4*>(&lh[buf][at]);
+        const uint32_t hh[4] = {hv.x, hv.y, hv.z, hv.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[4 * k + e], a.scale2, bias) - lv[e]);
+          float d = dp[4 * k + e], y = x;
+          if (DROP) { const bool keep = attn_keep(hh[e], hk, a.thresh); d = keep ? d * a.keep_scale : 0.f; y = keep ? x * a.keep_scale : 0.f; }
+          p[4 * k + e] = y;
+          ds[4 * k + e] = x * (d - dl[e]);
+        }
+      }
+      M::cols(lg[buf], n, p, dv, lane);
+      M::cols(lq[buf], n, ds, dk, lane);
+    }
+    if (tt + 1 < t1) put(buf ^ 1);
+    __syncthreads();
+    buf ^= 1;
+  }
+  if (key >= a.Lk) return;
+  if (a.splits == 1) {
+    xa_put_row<T, C::DB>(a.dk.p + b * a.dk.sb + (long long)key * a.dk.sl + kvh * a.dk.sh, dk, a.scale, lane);
+    xa_put_row<T, C::DB>(a.dv.p + b * a.dv.sb + (long long)key * a.dv.sl + kvh * a.dv.sh, dv, 1.0f, lane);
+  } else {
+    const size_t n = (size_t)a.BH * a.Lk, row = (size_t)bh * a.Lk + key;
+    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.part + (split * 2 * n + row) * D), dk, a.scale, lane);
+    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.part + ((split * 2 + 1) * n + row) * D), dv, 1.0f, lane);
+  }
+}
+
+// sum of the splits' gradients in split order.  which: 0 = dQ (packed rows), 1 = dK and dV
+template <typename T, int D>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(XaArgs a, int which, int len) {
+  const long long rows = (long long)a.BH * len, all = rows * (which ? 2 : 1);
+  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x, row = idx / (D / 4);
+  if (row >= all) return;
+  const int c = (int)(idx - row * (D / 4)) * 4;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < a.splits; ++k) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + ((size_t)k * all + row) * D + c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += v[e];
+  }
+  const long long lr = row >= rows ? row - rows : row;
+  const int bh = (int)(lr / len), r = (int)(lr - (long long)bh * len), b = bh / a.nkv, kvh = bh - b * a.nkv;
+  char* p;
+  if (which) {
+    const XaOut& x = row >= rows ? a.dv : a.dk;
+    p = x.p + b * x.sb + (long long)r * x.sl + kvh * x.sh;
+  } else {
+    int i, g;
+    xa_split(a, r, i, g);
+    p = a.dq.p + b * a.dq.sb + (long long)i * a.dq.sl + (long long)(kvh * a.G + g) * a.dq.sh;
+  }
+  xa_put4(reinterpret_cast<T*>(p) + c, s[0], s[1], s[2], s[3]);
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------------------
+static int xa_tt(int dtype, int D) { return D * (dtype ? 2 : 4) <= 128 ? 64 : 32; }
+// waves of a workgroup: as many 32-column waves as there are columns, up to 4 (they share the streamed tile); two at least for fp32
+// vectors of 128, whose staging by one wave alone spills
+static int xa_ns(int dtype, int D, int cols) { return cols <= 32 && !(dtype == 0 && D == 128) ? 1 : cols <= 64 ? 2 : 4; }
+// splits of the streamed axis: until the launch has about 2048 waves (8 per CU), each split at least two tiles
+static int xa_splits(const Uc2CrossAttn* p, int cols, int streamed) {
+  const int ns = xa_ns(p->dtype, p->D, cols), tt = xa_tt(p->dtype, p->D);
+  const long long bh = (long long)p->B * p->nkv;
+  const long long waves = bh * ((cols + 32 * ns - 1) / (32 * ns)) * ns, nt = (streamed + tt - 1) / tt;
+  long long s = waves > 0 ? 2048 / waves : 1;
+  if (s > nt / 2) s = nt / 2;
+  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+static size_t xa_up(size_t n) { return (n + 255) & ~(size_t)255; }
+struct XaPlan { int s_fwd, s_dq, s_dkv; size_t fwd, part_dq, part_dkv, delta, bwd; };
+static XaPlan xa_plan(const Uc2CrossAttn* p) {
+  XaPlan r{};
+  const long long bh = (long long)p->B * p->nkv, R = (long long)p->Lq * (p->nh / p->nkv);
+  r.s_fwd = r.s_dq = xa_splits(p, (int)R, p->Lk);
+  r.s_dkv = xa_splits(p, p->Lk, (int)R);
+  if (r.s_fwd > 1) r.fwd = xa_up((size_t)r.s_fwd * bh * R * p->D * 4) + xa_up((size_t)r.s_fwd * bh * R * 8);
+  r.delta = xa_up((size_t)bh * R * 4);
+  r.part_dq = r.s_dq > 1 ? (size_t)r.s_dq * bh * R * p->D * 4 : 0;
+  r.part_dkv = r.s_dkv > 1 ? (size_t)r.s_dkv * 2 * bh * p->Lk * p->D * 4 : 0;
+  r.bwd = r.delta + xa_up(r.part_dq > r.part_dkv ? r.part_dq : r.part_dkv);     // the two kernels follow one another: one area
+  return r;
+}
+static bool xa_str_ok(long long sb, long long sl, long long sh, int el) {      // 16-byte rows
+  return ((sb | sl | sh) & (16 / el - 1)) == 0 && sb >= 0 && sl >= 0 && sh >= 0;
+}
+static int xa_check(const Uc2CrossAttn* p) {
+  UC2_CHECK_ARG(p != nullptr);
+  UC2_CHECK_ARG(p->dtype == 0 || p->dtype == 1);
+  UC2_CHECK_ARG(p->D == 32 || p->D == 64 || p->D == 128);
+  UC2_CHECK_ARG(p->B >= 0 && p->Lq >= 0 && p->Lk >= 0 && p->nkv >= 1 && p->nh >= 1 && p->nh % p->nkv == 0);
+  UC2_CHECK_ARG((long long)p->Lq * (p->nh / p->nkv) < (1ll << 30) && p->Lk < (1 << 30));
+  UC2_CHECK_ARG((long long)p->B * p->nkv < (1ll << 24));
+  UC2_CHECK_ARG(p->drop_p >= 0.f && p->drop_p < 1.f);
+  return 0;
+}
+static int xa_ptrs(const Uc2CrossAttn* p) {
+  const int el = p->dtype ? 2 : 4;
+  UC2_CHECK_ARG(p->q && p->out && (p->Lk == 0 || (p->k && p->v)));
+  UC2_CHECK_ARG(xa_str_ok(p->q_sb, p->q_sl, p->q_sh, el) && xa_str_ok(p->k_sb, p->k_sl, p->k_sh, el) && xa_str_ok(p->v_sb, p->v_sl, p->v_sh, el));
+  UC2_CHECK_ARG(xa_str_ok(p->o_sb, p->o_sl, p->o_sh, el));
+  UC2_CHECK_ARG((((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->out) & 15) == 0);
+  return 0;
+}
+static XaArgs xa_args(const Uc2CrossAttn* p) {
+  const int el = p->dtype ? 2 : 4;
+  XaArgs a{};
+  a.B = p->B; a.Lq = p->Lq; a.Lk = p->Lk; a.nkv = p->nkv; a.nh = p->nh; a.G = p->nh / p->nkv; a.R = p->Lq * a.G; a.BH = p->B * p->nkv;
+  a.q = {(const char*)p->q, p->q_sb * el, p->q_sl * el, p->q_sh * el};
+  a.k = {(const char*)p->k, p->k_sb * el, p->k_sl * el, p->k_sh * el};
+  a.v = {(const char*)p->v, p->v_sb * el, p->v_sl * el, p->v_sh * el};
+  a.out = {(char*)p->out, p->o_sb * el, p->o_sl * el, p->o_sh * el};
+  a.o = {(const char*)p->out, p->o_sb * el, p->o_sl * el, p->o_sh * el};
+  a.kmask = p->key_mask; a.kmask_sb = p->key_mask_sb; a.klens = p->k_lens;
+  a.scale = p->scale; a.scale2 = p->scale * XA_LOG2E;
+  a.lse = p->lse;
+  a.thresh = drop_thresh(p->drop_p); a.keep_scale = 1.0f / (1.0f - p->drop_p); a.seed_ptr = p->seed; a.seed_imm = p->site;
+  return a;
+}
+static int xa_grid(XaArgs& a, int cols, int ns) {                  // blocks, or 0 where they pass a launch's limit
+  a.tiles = (cols + 32 * ns - 1) / (32 * ns);
+  const long long n = (long long)(a.BH >= 8 ? (a.BH + 7) / 8 * 8 : a.BH) * a.tiles * a.splits;
+  return n < (1ll << 31) ? (int)n : 0;
+}
+#define XA_LAUNCH(KERN, TT_, DD_, NN_, grid)                                                                                        \
+  do {                                                                                                                              \
+    if (a.thresh) hipLaunchKernelGGL((KERN<TT_, DD_, NN_, true>), dim3(grid), dim3(NN_ * 64), 0, st, a);                             \
+    else hipLaunchKernelGGL((KERN<TT_, DD_, NN_, false>), dim3(grid), dim3(NN_ * 64), 0, st, a);                                     \
+  } while (0)
+#define XA_NS(KERN, TT_, DD_)                                                                                                       \
+  do {                                                                                                                              \
+    if constexpr (DD_ * sizeof(TT_) <= 256) { if (ns == 1) { XA_LAUNCH(KERN, TT_, DD_, 1, grid); break; } }                          \
+    if (ns == 2) XA_LAUNCH(KERN, TT_, DD_, 2, grid); else XA_LAUNCH(KERN, TT_, DD_, 4, grid); \
+  } while (0)
+#define XA_TD(WHAT)                                                                                                                 \
+  do {                                                                                                                              \
+    if (p->dtype == 1) { if (p->D == 32) { WHAT(bf16, 32); } else if (p->D == 64) { WHAT(bf16, 64); } else { WHAT(bf16, 128); } }     \
+    else { if (p->D == 32) { WHAT(float, 32); } else if (p->D == 64) { WHAT(float, 64); } else { WHAT(float, 128); } }                \
+  } while (0)
+
+extern "C" size_t uc2_xattn_workspace(const Uc2CrossAttn* p, int backward) {
+  if (xa_check(p) != 0) return 0;
+  const XaPlan pl = xa_plan(p);
+  return backward ? pl.bwd : pl.fwd;
+}
+
+extern "C" int uc2_xattn_fwd(const Uc2CrossAttn* p, void* ws, size_t ws_bytes, void* stream) {
+  if (int e = xa_check(p)) return e;
+  if (p->B == 0 || p->Lq == 0) return 0;
+  if (int e = xa_ptrs(p)) return e;
+  const XaPlan pl = xa_plan(p);
+  UC2_CHECK_ARG(pl.fwd == 0 || (ws && ws_bytes >= pl.fwd && ((uintptr_t)ws & 15) == 0));
+  hipStream_t st = (hipStream_t)stream;
+  XaArgs a = xa_args(p);
+  a.splits = pl.s_fwd;
+  if (a.splits > 1) {
+    a.part = (float*)ws;
+    a.pml = (float*)((char*)ws + xa_up((size_t)a.splits * a.BH * a.R * p->D * 4));
+  }
+  const int ns = xa_ns(p->dtype, p->D, a.R), grid = xa_grid(a, a.R, ns);
+  UC2_CHECK_ARG(grid > 0);
+#define XA_GO(T_, D_) XA_NS(xattn_fwd_kernel, T_, D_)
+  XA_TD(XA_GO);
+#undef XA_GO
+  UC2_LAUNCH_CHECK();
+  if (a.splits > 1) {
+    const long long blocks = ((long long)a.BH * a.R + 3) / 4;
+    UC2_CHECK_ARG(blocks < (1ll << 31));
+#define XA_GO(T_, D_) hipLaunchKernelGGL((xattn_join_kernel<T_, D_>), dim3((unsigned)blocks), dim3(256), 0, st, a)
+    XA_TD(XA_GO);
+#undef XA_GO
+    UC2_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+extern "C" int uc2_xattn_bwd(const Uc2CrossAttn* p, const Uc2CrossAttnGrad* g, void* ws, size_t ws_bytes, void* stream) {
+  if (int e = xa_check(p)) return e;
+  UC2_CHECK_ARG(g != nullptr);
+  if (p->B == 0) return 0;
+  const int el = p->dtype ? 2 : 4;
+  UC2_CHECK_ARG(p->Lq == 0 || (g->dout && g->dq && p->lse));
+  UC2_CHECK_ARG(p->Lk == 0 || (g->dk && g->dv));
+  UC2_CHECK_ARG(xa_str_ok(g->dout_sb, g->dout_sl, g->dout_sh, el) && xa_str_ok(g->dq_sb, g->dq_sl, g->dq_sh, el));
+  UC2_CHECK_ARG(xa_str_ok(g->dk_sb, g->dk_sl, g->dk_sh, el) && xa_str_ok(g->dv_sb, g->dv_sl, g->dv_sh, el));
+  UC2_CHECK_ARG((((uintptr_t)g->dout | (uintptr_t)g->dq | (uintptr_t)g->dk | (uintptr_t)g->dv) & 15) == 0);
+  if (p->Lq > 0) { if (int e = xa_ptrs(p)) return e; }
+  const XaPlan pl = xa_plan(p);
+  UC2_CHECK_ARG(pl.bwd == 0 || (ws && ws_bytes >= pl.bwd && ((uintptr_t)ws & 15) == 0));
+  hipStream_t st = (hipStream_t)stream;
+  XaArgs a = xa_args(p);
+  a.dout = {(const char*)g->dout, g->dout_sb * el, g->dout_sl * el, g->dout_sh * el};
+  a.dq = {(char*)g->dq, g->dq_sb * el, g->dq_sl * el, g->dq_sh * el};
+  a.dk = {(char*)g->dk, g->dk_sb * el, g->dk_sl * el, g->dk_sh * el};
+  a.dv = {(char*)g->dv, g->dv_sb * el, g->dv_sl * el, g->dv_sh * el};
+  a.delta = (float*)ws;
+  a.part = (float*)((char*)ws + pl.delta);
+  if (p->Lq > 0) {
+    a.splits = pl.s_dq;
+    const int ns = xa_ns(p->dtype, p->D, a.R), grid = xa_grid(a, a.R, ns);
+    UC2_CHECK_ARG(grid > 0);
+#define XA_GO(T_, D_) XA_NS(xattn_dq_kernel, T_, D_)
+    XA_TD(XA_GO);
+#undef XA_GO
+    UC2_LAUNCH_CHECK();
+    if (a.splits > 1) {
+      const long long blocks = ((long long)a.BH * a.R * (p->D / 4) + 255) / 256;
+      UC2_CHECK_ARG(blocks < (1ll << 31));
+#define XA_GO(T_, D_) hipLaunchKernelGGL((xattn_sum_kernel<T_, D_>), dim3((unsigned)blocks), dim3(256), 0, st, a, 0, a.R)
+      XA_TD(XA_GO);
+#undef XA_GO
+      UC2_LAUNCH_CHECK();
+    }
+  }
+  if (p->Lk > 0) {
+    a.splits = pl.s_dkv;
+    const int ns = xa_ns(p->dtype, p->D, a.Lk), grid = xa_grid(a, a.Lk, ns);
+    UC2_CHECK_ARG(grid > 0);
+#define XA_GO(T_, D_) XA_NS(xattn_dkv_kernel, T_, D_)
+    XA_TD(XA_GO);
+#undef XA_GO
+    UC2_LAUNCH_CHECK();
+    if (a.splits > 1) {
+      const long long blocks = (2ll * a.BH * a.Lk * (p->D / 4) + 255) / 256;
+      UC2_CHECK_ARG(blocks < (1ll << 31));
+#define XA_GO(T_, D_) hipLaunchKernelGGL((xattn_sum_kernel<T_, D_>), dim3((unsigned)blocks), dim3(256), 0, st, a, 1, a.Lk)
+      XA_TD(XA_GO);
+#undef XA_GO
+      UC2_LAUNCH_CHECK();
+    }
+  }
+  return 0;
+}

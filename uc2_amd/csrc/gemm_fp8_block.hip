@@ -1,0 +1,181 @@
+// C[M, N] (bf16) = A B^T + bias of e4m3 operands with a power-of-two scale for each block of 128 (fp8_block.h): A [M, Kp] with 1 x 128 scales
+// (activations, output gradients), B [N, Kp] with 128 x 128 scales (weights; for the input gradient their transposed copy).
+//   C[m][n] = bias[n] + sum over k-blocks b of 2^(ea[m][b] + eb[n / 128][b]) sum_{k in b} a[m][k] b[n][k]
+// The scales are powers of two, so v_mfma_scale_f32_16x16x128_f8f6f4 applies both inside the matrix instruction (one k-block of 128 per
+// instruction): no second accumulator, no multiply per block; sums are fp32 throughout and rounded to bf16 once.
+#include "../../include/uc2_hip.h"
+#include "common.h"
+#include "fp8_block.h"
+
+typedef __attribute__((ext_vector_type(8))) int blk_i32x8;
+typedef __attribute__((ext_vector_type(4))) int blk_i32x4;
+
+struct BlkGemm {
+  int M, N, Kb, lda, ldb, ldc, lds_a, vec;                         // Kb = Kp / 128; lds_a: rows of A's scale words; vec: C takes 8-byte stores
+  const unsigned char *A, *B; const unsigned* sa; const unsigned char* sb;
+  const float* bias; bf16* C;
+};
+
+// the matrix instruction with A and B swapped: the accumulator block is [n][m], a lane holds row m = lane & 15 and columns 4 (lane >> 4) + 0..3
+__device__ __forceinline__ f32x4 blk_mfma(blk_i32x8 b, blk_i32x8 a, f32x4 c, int sb, int sa) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, sb, 0, sa);
+}
+__device__ __forceinline__ blk_i32x8 blk_cat(blk_i32x4 lo, blk_i32x4 hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ void blk_put(const BlkGemm& p, int m, int n, const f32x4& v) {
+  if (m >= p.M || n >= p.N) return;
+  bf16* c = p.C + (size_t)m * p.ldc + n;
+  if (n + 4 <= p.N) {
+    f32x4 x = v;
+    if (p.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += p.bias[n + e];
+    }
+    if (p.vec) { *reinterpret_cast<bf16x4*>(c) = bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]}; return; }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] = (bf16)x[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) if (n + e < p.N) c[e] = (bf16)(v[e] + (p.bias ? p.bias[n + e] : 0.f));
+  }
+}
+
+// ---- few rows: the weight's bytes are the work.  A workgroup owns 16 columns and 16 MB rows, its 8 waves take the k-blocks in turn -- both
+// operands straight from memory into the matrix instruction's registers, 32 bytes per lane and block -- and are added in wave order.
+template <int MB>
+__global__ __launch_bounds__(512) void gemm_fp8_block_rows_kernel(BlkGemm p) {
+  __shared__ f32x4 red[8][MB][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MB;
+  const unsigned char* b = p.B + (size_t)min(n0 + i, p.N - 1) * p.ldb + 32 * g;
+  const unsigned char* sb = p.sb + (size_t)(n0 >> 7) * p.Kb;
+  const unsigned char* a[MB];
+  int row[MB];
+#pragma unroll
+  for (int j = 0; j < MB; ++j) { row[j] = min(m0 + 16 * j + i, p.M - 1); a[j] = p.A + (size_t)row[j] * p.lda + 32 * g; }
+  f32x4 acc[MB];
+#pragma unroll
+  for (int j = 0; j < MB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int kt = w; kt < p.Kb; kt += 8) {
+    const blk_i32x4* bp = reinterpret_cast<const blk_i32x4*>(b + (size_t)kt * 128);
+    const blk_i32x8 bv = blk_cat(bp[0], bp[1]);
+    const int es = sb[kt];
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+      const blk_i32x4* ap = reinterpret_cast<const blk_i32x4*>(a[j] + (size_t)kt * 128);
+      const int ea = p.sa[(size_t)(kt >> 2) * p.lds_a + row[j]] >> (8 * (kt & 3));
+      acc[j] = blk_mfma(bv, blk_cat(ap[0], ap[1]), acc[j], es, ea);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < MB; ++j) red[w][j][lane] = acc[j];
+  __syncthreads();
+  for (int j = w; j < MB; j += 8) {
+    f32x4 s = red[0][j][lane];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += red[k][j][lane];
+    blk_put(p, m0 + 16 * j + i, n0 + 4 * g, s);
+  }
+}
+
+// ---- any size: WB x WB blocks of 16 per wave, 2 x 2 waves; k-tiles of one block (128 bytes) double-buffered in LDS through registers
+template <int WB>
+__global__ __launch_bounds__(256) void gemm_fp8_block_tile_kernel(BlkGemm p) {
+  constexpr int T = 32 * WB, NL = T * 8 / 256;                     // tile edge; 16-byte pieces per thread and operand
+  __shared__ __attribute__((aligned(16))) unsigned char la[2][T * 128], lb[2][T * 128];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, g = lane >> 4, i = lane & 15, wm = w >> 1, wn = w & 1;
+  const int m0 = blockIdx.x * T, n0 = blockIdx.y * T;
+  const unsigned char *as[NL], *bs[NL];
+  int off[NL];
+#pragma unroll
+  for (int n = 0; n < NL; ++n) {
+    const int r = (t + n * 256) >> 3, c = t & 7;
+    as[n] = p.A + (size_t)min(m0 + r, p.M - 1) * p.lda + c * 16;
+    bs[n] = p.B + (size_t)min(n0 + r, p.N - 1) * p.ldb + c * 16;
+    off[n] = r * 128 + ((c ^ (r & 7)) << 4);
+  }
+  int row[WB];
+#pragma unroll
+  for (int j = 0; j < WB; ++j) row[j] = min(m0 + wm * 16 * WB + 16 * j + i, p.M - 1);
+  const unsigned char* sb = p.sb + (size_t)(n0 >> 7) * p.Kb;
+  f32x4 acc[WB][WB];
+#pragma unroll
+  for (int x = 0; x < WB; ++x)
+#pragma unroll
+    for (int y = 0; y < WB; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+  blk_i32x4 ra[NL], rb[NL];
+  auto fetch = [&](int kt) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) { ra[n] = *reinterpret_cast<const blk_i32x4*>(as[n] + (size_t)kt * 128); rb[n] = *reinterpret_cast<const blk_i32x4*>(bs[n] + (size_t)kt * 128); }
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < NL; ++n) { *reinterpret_cast<blk_i32x4*>(la[buf] + off[n]) = ra[n]; *reinterpret_cast<blk_i32x4*>(lb[buf] + off[n]) = rb[n]; }
+  };
+  unsigned sw[WB];
+  fetch(0); put(0);
+  __syncthreads();
+  const int sz = i & 7;
+  for (int kt = 0; kt < p.Kb; ++kt) {
+    const int buf = kt & 1;
+    if (kt + 1 < p.Kb) fetch(kt + 1);
+    if ((kt & 3) == 0) {
+#pragma unroll
+      for (int j = 0; j < WB; ++j) sw[j] = p.sa[(size_t)(kt >> 2) * p.lds_a + row[j]];
+    }
+    const int es = sb[kt];
+    blk_i32x8 bv[WB];
+#pragma unroll
+    for (int y = 0; y < WB; ++y) {
+      const unsigned char* q = lb[buf] + (wn * 16 * WB + 16 * y + i) * 128;
+      bv[y] = blk_cat(*reinterpret_cast<const blk_i32x4*>(q + (((2 * g) ^ sz) << 4)), *reinterpret_cast<const blk_i32x4*>(q + (((2 * g + 1) ^ sz) << 4)));
+    }
+#pragma unroll
+    for (int x = 0; x < WB; ++x) {
+      const unsigned char* q = la[buf] + (wm * 16 * WB + 16 * x + i) * 128;
+      const blk_i32x8 av = blk_cat(*reinterpret_cast<const blk_i32x4*>(q + (((2 * g) ^ sz) << 4)), *reinterpret_cast<const blk_i32x4*>(q + (((2 * g + 1) ^ sz) << 4)));
+#pragma unroll
+      for (int y = 0; y < WB; ++y) acc[x][y] = blk_mfma(bv[y], av, acc[x][y], es, (int)sw[x]);
+      sw[x] >>= 8;
+    }
+    if (kt + 1 < p.Kb) put(buf ^ 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int x = 0; x < WB; ++x)
+#pragma unroll
+    for (int y = 0; y < WB; ++y) blk_put(p, m0 + wm * 16 * WB + 16 * x + i, n0 + wn * 16 * WB + 16 * y + 4 * g, acc[x][y]);
+}
+
+extern "C" int uc2_gemm_fp8_block(int M, int N, int K, const void* A8, int lda, const void* scale_a, int rows_a, const void* B8, int ldb,
+                                  const void* scale_b, const float* bias, void* C, int ldc, void* stream) {
+  UC2_CHECK_ARG(M >= 0 && N >= 0 && K >= 1 && K <= (1 << 30));
+  if (M == 0 || N == 0) return 0;
+  const int Kp = (K + 127) / 128 * 128;
+  UC2_CHECK_ARG(A8 && scale_a && B8 && scale_b && C);
+  UC2_CHECK_ARG(lda >= Kp && ldb >= Kp && ldc >= N && rows_a >= M && (lda % 16) == 0 && (ldb % 16) == 0);
+  UC2_CHECK_ARG((((uintptr_t)A8 | (uintptr_t)B8) & 15) == 0 && ((uintptr_t)scale_a & 3) == 0 && ((uintptr_t)C & 1) == 0 && ((uintptr_t)bias & 3) == 0);
+  BlkGemm p{};
+  p.M = M; p.N = N; p.Kb = Kp / 128; p.lda = lda; p.ldb = ldb; p.ldc = ldc; p.lds_a = rows_a;
+  p.vec = (ldc % 4) == 0 && ((uintptr_t)C & 7) == 0;
+  p.A = (const unsigned char*)A8; p.B = (const unsigned char*)B8; p.sa = (const unsigned*)scale_a; p.sb = (const unsigned char*)scale_b;
+  p.bias = bias; p.C = (bf16*)C;
+  hipStream_t st = (hipStream_t)stream;
+  if (M <= 64) {
+    const int mb = (M + 15) / 16;
+    const dim3 grid((N + 15) / 16, 1);
+    if (mb == 1) hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<1>, grid, dim3(512), 0, st, p);
+    else if (mb == 2) hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<2>, grid, dim3(512), 0, st, p);
+    else hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<4>, grid, dim3(512), 0, st, p);
+  } else {
+    // 128 x 128 tiles once they fill the chip, 64 x 64 ones below
+    const long long t128 = (long long)((M + 127) / 128) * ((N + 127) / 128);
+    const int T = t128 >= 256 ? 128 : 64;
+    const dim3 grid((M + T - 1) / T, (N + T - 1) / T);
+    UC2_CHECK_ARG(grid.y < 65536);
+    if (T == 128) hipLaunchKernelGGL(gemm_fp8_block_tile_kernel<4>, grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL(gemm_fp8_block_tile_kernel<2>, grid, dim3(256), 0, st, p);
+  }
+  UC2_LAUNCH_CHECK();
+  return 0;
+}

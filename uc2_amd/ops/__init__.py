@@ -9,6 +9,8 @@ torch.autograd.Function nodes the model modules are built from.  Split by concer
     kernels    LayerNorm, attention, cast wrappers
     layer      BertLayerFn (one autograd node per encoder layer)
     functions  the other autograd Functions (embeddings, heads, losses)
+    block      e4m3 under block scales: quantisation, product, linear layer; the root-mean-square norm that feeds them
+    cross      attention to the states of another sequence
 
 Knobs live in uc2_amd.config.cfg (read from UC2_* once), run-time hooks in uc2_amd.config.state; everything else is re-exported
 here, so `from uc2_amd import ops; ops.gemm(...)` keeps working."""
@@ -51,6 +53,11 @@ from .functions import (  # noqa: F401
     GatherRowsFn, GeluFn, KLDivFn, LayerNormFn, LinearFn, MSEFn, MaskEmbedFn, OTDistFn, PadRowsFn, UnpadRowsFn, padded_rows, SelectRowsFn, TiedSubsetDecoderFn,
     TripletFn, _DEC_ROWS, _dec_chunks, _dgelu, add_rowvec, attn_general_probs_mean, attn_probs_mean,
 )
+from .block import (  # noqa: F401
+    BlockRows, BlockWeight, LinearBlockFp8Fn, RMSNormFn, fp8_quantize_block, fp8_quantize_weight_block, gemm_fp8_block, linear_fp8_block,
+    rms_norm, rms_norm_fp8,
+)
+from .cross import CrossAttentionFn, cross_attention  # noqa: F401
 
 if knobs.gemm_plans:
     load_plans(knobs.gemm_plans_file)

@@ -124,6 +124,22 @@ def _require_cuda(t):
         raise _lib.Uc2Error("uc2_amd kernels run on the GPU only (tensor on %s); there is no CPU fallback" % t.device)
 
 
+class _NoGuard:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+def device_guard(t):
+    """with device_guard(x): launches go to x's device and to the stream that is current there (nothing to do on the current device)"""
+    return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
 # --------------------------------------------------------------------------------------
 # dropout seed state (device side, so a captured hipGraph draws fresh masks on every replay)
 # --------------------------------------------------------------------------------------
