@@ -82,7 +82,8 @@ def test_quantize_strided_rows():
 
 # ---- product --------------------------------------------------------------------------------------------------------------------
 GEMM_SIZES = [(1, 1, 1), (1, 1024, 4096), (8, 4096, 1024), (16, 17, 128), (17, 130, 256), (33, 1000, 300), (64, 255, 1024), (65, 129, 640),
-              (128, 128, 128), (200, 777, 1000), (256, 256, 512), (512, 768, 768), (1030, 516, 384), (2048, 2304, 768), (1024, 1024, 1152)]
+              (128, 128, 128), (200, 777, 1000), (256, 256, 512), (512, 768, 768), (1030, 516, 384), (2048, 2304, 768), (1024, 1024, 1152),
+              (4096, 2304, 768), (8300, 1100, 512), (33000, 256, 256), (4200, 2304, 1000), (4096, 2304, 1152)]
 
 
 @pytest.mark.parametrize("M,N,K", GEMM_SIZES)

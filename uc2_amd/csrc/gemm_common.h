@@ -48,6 +48,8 @@ struct GemmArgs {
   unsigned drop_thresh; float drop_scale; const uint64_t* drop_seed_ptr; uint64_t drop_seed_imm;
   void* q_out; int ldq;
   const unsigned* q_amax_prev; unsigned* q_amax_next; unsigned* q_amax_clear; float* q_scale_out;
+  // ... with a power-of-two scale for each block of 128 (fp8_block.h): A's words [ceil(blocks / 4)][blk_sa_ld], B's bytes [ceil(N / 128)][blk_sb_ld]
+  const unsigned* blk_sa; const unsigned char* blk_sb; int blk_sa_ld, blk_sb_ld;
 };
 
 // ------------------------------------------------------------------------------------------

@@ -6,6 +6,10 @@
 #include "../../include/uc2_hip.h"
 #include "common.h"
 #include "fp8_block.h"
+#include "gemm_tile.h"
+#include "gemm_pp8_kernel.h"
+
+bool uc2_gemm_pp8_supported(const GemmArgs& p);                   // gemm_pp8.hip: whole 256 x 256 tiles, an even number of blocks
 
 typedef __attribute__((ext_vector_type(8))) int blk_i32x8;
 typedef __attribute__((ext_vector_type(4))) int blk_i32x4;
@@ -147,11 +151,58 @@ __global__ __launch_bounds__(256) void gemm_fp8_block_tile_kernel(BlkGemm p) {
     for (int y = 0; y < WB; ++y) blk_put(p, m0 + wm * 16 * WB + 16 * x + i, n0 + wn * 16 * WB + 16 * y + 4 * g, acc[x][y]);
 }
 
+static void blk_launch_tiles(const BlkGemm& p, hipStream_t st) {
+  if (p.M <= 64) {
+    const dim3 grid((p.N + 15) / 16);
+    if (p.M <= 16) hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<1>, grid, dim3(512), 0, st, p);
+    else if (p.M <= 32) hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<2>, grid, dim3(512), 0, st, p);
+    else hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<4>, grid, dim3(512), 0, st, p);
+    return;
+  }
+  // 128 x 128 tiles once they fill the chip, 64 x 64 ones below
+  const long long t128 = (long long)((p.M + 127) / 128) * ((p.N + 127) / 128);
+  const int T = t128 >= 256 ? 128 : 64;
+  const dim3 grid((p.M + T - 1) / T, (p.N + T - 1) / T);
+  if (T == 128) hipLaunchKernelGGL(gemm_fp8_block_tile_kernel<4>, grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL(gemm_fp8_block_tile_kernel<2>, grid, dim3(256), 0, st, p);
+}
+#ifndef BLK_PP_MIN
+#define BLK_PP_MIN 128
+#endif
+static void blk_launch(BlkGemm p, hipStream_t st) {
+  // whole 256 x 256 tiles go to the persistent kernel once there are enough of them; what is left of the rows and of the columns to the tiles here
+  const int M0 = p.M / 256 * 256, N0 = p.N / 256 * 256;
+  if ((long long)(M0 / 256) * (N0 / 256) >= BLK_PP_MIN && ((uintptr_t)p.sb & 1) == 0) {
+    GemmArgs g{};                                                  // (the "bf16 view" of bytes: K and leading dimensions halved)
+    g.A = p.A; g.B = p.B; g.C = p.C; g.bias = p.bias; g.M = M0; g.N = N0; g.K = p.Kb * 64; g.lda = p.lda / 2; g.ldb = p.ldb / 2; g.ldc = g.ldaux = p.ldc;
+    g.epi = EPI_NONE; g.split_k = 1; g.a_vec = g.b_vec = 1; g.alpha = 1.0f;
+    g.blk_sa = p.sa; g.blk_sa_ld = p.lds_a; g.blk_sb = p.sb; g.blk_sb_ld = p.Kb;
+    if (uc2_gemm_pp8_supported(g)) {
+      g.col_group = pp8_col_group(N0);
+      pp8_launch0<EPI_NONE, false, true>(g, st);
+      if (N0 < p.N) {
+        BlkGemm c = p;
+        c.M = M0; c.N = p.N - N0; c.B += (size_t)N0 * p.ldb; c.sb += (size_t)(N0 / 128) * p.Kb; c.C += N0;
+        if (c.bias) c.bias += N0;
+        blk_launch_tiles(c, st);
+      }
+      if (M0 < p.M) {
+        BlkGemm r = p;
+        r.M = p.M - M0; r.A += (size_t)M0 * p.lda; r.sa += M0; r.C += (size_t)M0 * p.ldc;
+        blk_launch_tiles(r, st);
+      }
+      return;
+    }
+  }
+  blk_launch_tiles(p, st);
+}
+
 extern "C" int uc2_gemm_fp8_block(int M, int N, int K, const void* A8, int lda, const void* scale_a, int rows_a, const void* B8, int ldb,
                                   const void* scale_b, const float* bias, void* C, int ldc, void* stream) {
   UC2_CHECK_ARG(M >= 0 && N >= 0 && K >= 1 && K <= (1 << 30));
   if (M == 0 || N == 0) return 0;
   const int Kp = (K + 127) / 128 * 128;
+  UC2_CHECK_ARG((N + 63) / 64 < 65536);                            // (a launch's second grid dimension)
   UC2_CHECK_ARG(A8 && scale_a && B8 && scale_b && C);
   UC2_CHECK_ARG(lda >= Kp && ldb >= Kp && ldc >= N && rows_a >= M && (lda % 16) == 0 && (ldb % 16) == 0);
   UC2_CHECK_ARG((((uintptr_t)A8 | (uintptr_t)B8) & 15) == 0 && ((uintptr_t)scale_a & 3) == 0 && ((uintptr_t)C & 1) == 0 && ((uintptr_t)bias & 3) == 0);
@@ -160,22 +211,7 @@ extern "C" int uc2_gemm_fp8_block(int M, int N, int K, const void* A8, int lda, 
   p.vec = (ldc % 4) == 0 && ((uintptr_t)C & 7) == 0;
   p.A = (const unsigned char*)A8; p.B = (const unsigned char*)B8; p.sa = (const unsigned*)scale_a; p.sb = (const unsigned char*)scale_b;
   p.bias = bias; p.C = (bf16*)C;
-  hipStream_t st = (hipStream_t)stream;
-  if (M <= 64) {
-    const int mb = (M + 15) / 16;
-    const dim3 grid((N + 15) / 16, 1);
-    if (mb == 1) hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<1>, grid, dim3(512), 0, st, p);
-    else if (mb == 2) hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<2>, grid, dim3(512), 0, st, p);
-    else hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<4>, grid, dim3(512), 0, st, p);
-  } else {
-    // 128 x 128 tiles once they fill the chip, 64 x 64 ones below
-    const long long t128 = (long long)((M + 127) / 128) * ((N + 127) / 128);
-    const int T = t128 >= 256 ? 128 : 64;
-    const dim3 grid((M + T - 1) / T, (N + T - 1) / T);
-    UC2_CHECK_ARG(grid.y < 65536);
-    if (T == 128) hipLaunchKernelGGL(gemm_fp8_block_tile_kernel<4>, grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL(gemm_fp8_block_tile_kernel<2>, grid, dim3(256), 0, st, p);
-  }
+  blk_launch(p, (hipStream_t)stream);
   UC2_LAUNCH_CHECK();
   return 0;
 }
