@@ -9,9 +9,11 @@
 #ifndef PP16_AUX_TOUCH
 #define PP16_AUX_TOUCH 1     // touch the lines of the epilogue's aux_in tile two k-tiles ahead (residual-add / gelu'-multiply / dGELU kinds)
 #endif
-// BLK: block scales (fp8_block.h) instead of the tensors' two: a k-tile of 128 bytes is one block, the matrix instruction takes the row's and the
-// weight block's exponent bytes.  They wait in registers for a pair of k-tiles (16 bits each: op_sel picks the byte); a half's four words are loaded
-// again in the first section behind their last use, two sections (~1000 cycles) before the next: no registers for a second set.
+// BLK: block scales (fp8_block.h) instead of the tensors' two: a k-tile of 128 bytes is one block, the matrix instruction takes the exponent bytes of
+// the lane's row and of the wave's 64 columns (one weight block).  The scales of 28 k-tiles wait in the wave's own transposition buffer, which only the epilogue uses: fetched by LDS-DMA between the epilogue's last read of it and its stores, so that the wait for
+// them leaves the stores in flight; a lane reads the four bytes of a half per k-tile (beside 16 times as many operand bytes).  As plain loads into
+// registers, with the waits that hipcc puts in front of their uses, they cost half of the main loop: 8192^3 at 1858 instead of 2600 TFLOP/s.
+// More k-tiles: the buffer is filled again every 28, in the open (~1 us of ~28).
 template <bool TA, bool TB, bool TACC, int EPI, int HI, bool QOUT = false, bool BLK = false>
 __global__ __launch_bounds__(512, 2) void gemm_fp8_pp8_kernel(GemmArgs p) {
   static_assert(HI == 2 && TACC && !TA && !TB, "256-row tiles, transposed accumulators, k-contiguous e4m3 operands");
@@ -184,28 +186,44 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_pp8_kernel(GemmArgs p) {
   // bf16 kernel's).  What the compiler can no longer see -- vector writes before and reads after an MFMA -- gets s_nops (init_acc, epilogue).
   int usc = 0x7F7F7F7F;                                // unit block scales (E8M0 127) for both operands
   asm volatile("" : "+v"(usc));
-  int bsa[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, bsb = 0, bsbn = 0;     // (BLK) exponent bytes of a pair of k-tiles: A halves x row blocks, B; B of the next pair
-  const unsigned blk_lane = (unsigned)(wr * RW + (lane & 15)) * 4u;
-  auto blk_load_a = [&](int h, int kt) __attribute__((always_inline)) {
-    const char* s = reinterpret_cast<const char*>(p.blk_sa) + ((size_t)(kt >> 2) * p.blk_sa_ld + m0) * 4 + (kt & 2);
-#pragma unroll
-    for (int mb = 0; mb < 4; ++mb) bsa[h][mb] = *reinterpret_cast<const volatile unsigned short*>(s + blk_lane + h * 256 + mb * 64);
+  constexpr int BW = 28;                               // (BLK) k-tiles whose scales the buffer holds: 7 words of 128 rows, 3584 bytes, and B's bytes behind them
+  int bsa[4] = {0, 0, 0, 0}, bsb = 0, bkt = 0;         // exponent bytes of the half's four row blocks and of the weight block; first k-tile in the buffer
+  const unsigned blk_rb = lds0 + 131072u + (unsigned)w * 4096u + 3584u, blk_rd = blk_rb - 3584u + (unsigned)(lane & 15) * 4u;
+  auto blk_fetch = [&](int kt) __attribute__((always_inline)) {      // k-tiles kt .. kt + BW - 1 of the item at (m0, n0)
+    const int n = min(BW, ktiles - kt), words = (n + 3) >> 2;
+    bkt = kt;
+    int ln = lane;
+    asm volatile("" : "+v"(ln));                       // (addresses made here, not kept across the main loop)
+    const unsigned* s = p.blk_sa + (size_t)(kt >> 2) * p.blk_sa_ld + m0 + wr * RW;
+    for (int i = 0; i < words; ++i) {
+      __builtin_amdgcn_global_load_lds((glb_void_p)(s + ln), (lds_void_p)(smem + 131072 + w * 4096 + i * 512), 4, 0, 0);
+      __builtin_amdgcn_global_load_lds((glb_void_p)(s + 64 + ln), (lds_void_p)(smem + 131072 + w * 4096 + i * 512 + 256), 4, 0, 0);
+      s += p.blk_sa_ld;
+    }
+    // one byte per lane, at dword lane
+    __builtin_amdgcn_global_load_lds((glb_void_p)(p.blk_sb + (size_t)((n0 + wc * 64) >> 7) * p.blk_sb_ld + kt + min(ln, n - 1)),
+                                     (lds_void_p)(smem + 131072 + w * 4096 + 3584), 1, 0, 0);
   };
-  auto blk_load_b = [&](int kt) __attribute__((always_inline)) {
-    return (int)*reinterpret_cast<const volatile unsigned short*>(p.blk_sb + (size_t)((n0 + wc * 64) >> 7) * p.blk_sb_ld + kt);
-  };
+#define BLK_READ(H, KT)                                                                                        \
+  do {                                                                                                         \
+    if (BLK) {                                                                                                 \
+      const int kw_ = (KT) - bkt;                                                                              \
+      const unsigned ra_ = blk_rd + (unsigned)((kw_ >> 2) * 512 + (kw_ & 3));                                  \
+      if ((H) == 0) asm volatile("ds_read_u8 %0, %1" : "=v"(bsb) : "v"(blk_rb + (unsigned)(kw_ * 4)));         \
+      asm volatile("ds_read_u8 %0, %1 offset:%2" : "=v"(bsa[0]) : "v"(ra_), "n"((H) * 256));                   \
+      asm volatile("ds_read_u8 %0, %1 offset:%2" : "=v"(bsa[1]) : "v"(ra_), "n"((H) * 256 + 64));              \
+      asm volatile("ds_read_u8 %0, %1 offset:%2" : "=v"(bsa[2]) : "v"(ra_), "n"((H) * 256 + 128));             \
+      asm volatile("ds_read_u8 %0, %1 offset:%2" : "=v"(bsa[3]) : "v"(ra_), "n"((H) * 256 + 192));             \
+    }                                                                                                          \
+  } while (0)
 #define PP_MFMA(H, JB, BREG)                                                                                   \
   do {                                                                                                         \
     _Pragma("unroll") for (int mb = 0; mb < 4; ++mb)                                                           \
       _Pragma("unroll") for (int nbl = 0; nbl < 2; ++nbl)                                                      \
-        if constexpr (BLK && !SW)                                                                              \
-          asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[0,0,0] op_sel_hi:[0,0,0]" \
+        if constexpr (BLK)                                                                                     \
+          asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"            \
                      : "+v"(acc[H][mb][2 * (JB) + nbl])                                                        \
-                     : "v"(pp8_cat(BREG[2 * nbl], BREG[2 * nbl + 1])), "v"(pp8_cat(a[mb][0], a[mb][1])), "v"(bsb), "v"(bsa[H][mb])); \
-        else if constexpr (BLK)                                                                                \
-          asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0]" \
-                     : "+v"(acc[H][mb][2 * (JB) + nbl])                                                        \
-                     : "v"(pp8_cat(BREG[2 * nbl], BREG[2 * nbl + 1])), "v"(pp8_cat(a[mb][0], a[mb][1])), "v"(bsb), "v"(bsa[H][mb])); \
+                     : "v"(pp8_cat(BREG[2 * nbl], BREG[2 * nbl + 1])), "v"(pp8_cat(a[mb][0], a[mb][1])), "v"(bsb), "v"(bsa[mb])); \
         else asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %3 op_sel_hi:[0,0,0]"              \
                      : "+v"(acc[H][mb][2 * (JB) + nbl])                                                        \
                      : "v"(pp8_cat(BREG[2 * nbl], BREG[2 * nbl + 1])), "v"(pp8_cat(a[mb][0], a[mb][1])), "v"(usc)); \
@@ -264,8 +282,9 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_pp8_kernel(GemmArgs p) {
     // the registers of B1 (dead after phase 2; the current B0 is still needed by this phase's MFMAs) -- the two B
     // register sets swap roles every k-tile.  The unit order of the stream is therefore B0, A0, B1, A1: every phase
     // consumes exactly the unit the previous phase's wait retired.
-    if (BLK && !SW && kt > 0) { bsb = bsbn; blk_load_a(1, kt); }
+    if (BLK && !SW && kt - bkt == BW) { blk_fetch(kt); wait_vmcnt<0>(); }
     // ---- phase 0
+    BLK_READ(0, kt);
     if (!dg_nord || kt == 0) PP_READ_A(CB, 0);
     if (PP16_AUX_TOUCH && AUXK && TAIL && !SW && aux_touch) {
       // Two k-tiles before the epilogue needs them: one 4-byte load per 128-byte line of this wave's aux_in tile (128 rows x 64
@@ -296,7 +315,7 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_pp8_kernel(GemmArgs p) {
     // into the ring positions a prologue would use (nt is even).  The next item then starts with its operands in LDS
     // instead of issuing 96 KiB of LDS-DMA and waiting for it with the matrix pipe idle.
     if (TAIL && !SW && more) setup(nxt);
-    if (BLK && SW && !TAIL) { blk_load_a(0, kt + 1); bsbn = blk_load_b(kt + 1); }
+    BLK_READ(1, kt);
     if (!dg_nord || kt == 0) PP_READ_A(CB, 3);
     if ((!TAIL || f0 + 8 < nunits || more) && !dg_nodma) PP_ISSUE(1, nb ^ 1);
     PP_SYNC_L((TAIL && !more) ? nunits - 5 - f0 : 4, 2);
@@ -326,6 +345,7 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_pp8_kernel(GemmArgs p) {
   m0 = m0x; n0 = n0x; nt = ntx; zsplit = zx;
   if (GRP) { pdst = pdstx; pld = pldx; }
   PP_PROLOGUE();
+  if (BLK) blk_fetch(0);
   int younger = GKT;                                   // VMEM operations issued after the first two units of the current item
   for (;;) {
     // Accumulators start at the bias (scalar loads: uniform address in constant space, lgkmcnt, no vector registers).
@@ -365,7 +385,8 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_pp8_kernel(GemmArgs p) {
     };
     // units 0 and 1 of this item: this wave's part has landed, then publish
     auto item_barrier = [&]() __attribute__((always_inline)) {
-      if (younger == GKT) { if (HI == 2) wait_vmcnt<8>(); else wait_vmcnt<7>(); }
+      if (BLK) { if (younger == GKT) wait_vmcnt<0>(); else wait_vmcnt<NST>(); }      // (the scales: behind the units, in front of the stores)
+      else if (younger == GKT) { if (HI == 2) wait_vmcnt<8>(); else wait_vmcnt<7>(); }
       else if (younger == GKT + NST) { if (HI == 2) wait_vmcnt<24>(); else wait_vmcnt<19>(); }
       else if (younger == GKT + 2 * NST) { if (HI == 2) wait_vmcnt<40>(); else wait_vmcnt<31>(); }
       else if (QOUT && younger == GKT + NST + 8) wait_vmcnt<32>();
@@ -394,7 +415,6 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_pp8_kernel(GemmArgs p) {
     more = nxt < item_end;
     if (!(p.atomic & 0x4000)) {                        // (diagnostic 0x4000: epilogue only)
       using F = std::false_type; using T = std::true_type;
-      if (BLK) { blk_load_a(0, 0); blk_load_a(1, 0); bsb = blk_load_b(0); }
       PP_READ_B(bx, 0, 1);                             // B0 of k-tile 0 (later k-tiles get theirs one phase ahead)
       int kt = 0;
       for (; kt + 2 < nt; kt += 2) { body(F{}, F{}, kt); body(F{}, T{}, kt + 1); }     // nt is even (host-checked)
@@ -465,6 +485,7 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_pp8_kernel(GemmArgs p) {
       ticket_ready(); ticket_publish();
       PP_STAMP(3);
       asm volatile("" : "+v"(ln));
+      if (BLK && more) { blk_fetch(0); __builtin_amdgcn_sched_barrier(0); }
       if (QOUT) pp_epi_store<EPI_NONE, HI>(p, out, em0, en0, ln);       // (the second stream and the e4m3 stream left block by block)
       else pp_epi_store<EPI, HI>(p, out, em0, en0, ln);
       PP_STAMP(4);
@@ -496,6 +517,7 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_pp8_kernel(GemmArgs p) {
     }
   }
 #undef PP_STAMP
+#undef BLK_READ
 #undef PP_ISSUE
 #undef PP_PROLOGUE
 #undef PP_MFMA
