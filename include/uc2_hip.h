@@ -186,6 +186,12 @@ int uc2_fp8_quant_square(int dtype, int N, int K, const void* w, long long ldw, 
  * of a longer operand may be multiplied); C of any alignment.  Any M, N, K; any number of rows including single ones. */
 int uc2_gemm_fp8_block(int M, int N, int K, const void* A8, int lda, const void* scale_a, int rows_a, const void* B8, int ldb,
                        const void* scale_b, const float* bias, void* C, int ldc, void* stream);
+/* dw[N,K] = dy[M,N]^T x[M,K] and (dbias not NULL) dbias[N] = column sums of dy: the weight gradient of such a layer, on the unquantised bf16
+ * rows (as uc2_gemm's in the per-tensor mode, which wants whole tiles and aligned rows to be fast).  Written, not accumulated; rows of any stride
+ * and alignment, M >= 1; fp32 sums in a fixed order through ws (uc2_linear_wgrad_workspace bytes; 0: may be NULL). */
+size_t uc2_linear_wgrad_workspace(int M, int N, int K);
+int uc2_linear_wgrad(int M, int N, int K, const void* dy, long long lddy, const void* x, long long ldx, float* dw, long long lddw, float* dbias,
+                     void* ws, size_t ws_bytes, void* stream);
 
 /* ---- root-mean-square norm of a residual stream (beside LayerNorm below) ------------------------------------------------------------------
  *   sum = x + residual rounded to the tensors' type (both NULL: the norm reads x);  y = sum rstd gamma,  rstd = 1 / sqrt(mean(sum^2) + eps)

@@ -67,6 +67,8 @@ SIGNATURES = {
     "uc2_fp8_quant_rows": (I, [I, I, I, P, I64, P, P, P]),
     "uc2_fp8_quant_square": (I, [I, I, I, P, I64, P, P, P, P, P]),
     "uc2_gemm_fp8_block": (I, [I, I, I, P, I, P, I, P, I, P, P, P, I, P]),
+    "uc2_linear_wgrad_workspace": (SZ, [I, I, I]),
+    "uc2_linear_wgrad": (I, [I, I, I, P, I64, P, I64, P, I64, P, P, SZ, P]),
     "uc2_rms_fwd": (I, [I, I, I, P, P, P, F, P, P, P, P, P, P]),
     "uc2_rms_bwd_workspace": (SZ, [I, I]),
     "uc2_rms_bwd": (I, [I, I, I, P, P, P, P, P, P, P, P, SZ, P]),

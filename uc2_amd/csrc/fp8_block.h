@@ -11,26 +11,60 @@
 typedef bf16 blk_bf16x8_u __attribute__((ext_vector_type(8), aligned(2)));
 typedef float blk_f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 
-// elements c .. c + 7 of a row of n, zeros behind its end; no alignment needed
-__device__ __forceinline__ void blk_load8(const bf16* row, int c, int n, float (&v)[8]) {
-  if (c + 8 <= n) {
-    const blk_bf16x8_u x = *reinterpret_cast<const blk_bf16x8_u*>(row + c);
+// elements c .. c + 7 (c < n) of a row of n that ends inside them, zeros behind its end: the row's last eight, shifted down (eight guarded loads
+// in their place made the workgroups of a matrix's last columns several times slower than the others)
+__device__ __forceinline__ bf16x8 blk_tail8(const bf16* row, int c, int n) {
+  if (n < 8) {
+    bf16x8 v = {};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)x[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < n ? (float)row[c + e] : 0.f;
+    for (int e = 0; e < 8; ++e) if (c + e < n) v[e] = row[c + e];
+    return v;
   }
+  typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+  u64x2 u = __builtin_bit_cast(u64x2, (bf16x8)*reinterpret_cast<const blk_bf16x8_u*>(row + n - 8));
+  const int sh = (c + 8 - n) * 16;                     // 16 .. 112 bits
+  const unsigned long long lo = sh < 64 ? (u[0] >> sh) | (u[1] << (64 - sh)) : u[1] >> (sh - 64), hi = sh < 64 ? u[1] >> sh : 0ull;
+  return __builtin_bit_cast(bf16x8, u64x2{lo, hi});
 }
-__device__ __forceinline__ void blk_load8(const float* row, int c, int n, float (&v)[8]) {
-  if (c + 8 <= n) {
-    const blk_f32x4_u x = *reinterpret_cast<const blk_f32x4_u*>(row + c), y = *reinterpret_cast<const blk_f32x4_u*>(row + c + 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { v[e] = x[e]; v[4 + e] = y[e]; }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < n ? row[c + e] : 0.f;
+// Eight neighbouring elements of a row, loaded (no alignment needed) and converted in two steps: every load of a row is issued before the first is used.
+// WHOLE (rows of a multiple of 8): no branch -- hipcc waits for a load at the end of the branch that uses it, and a chunk behind the row's end loads
+// the row's last one and counts as zeros.  Otherwise the last chunk goes element by element.
+template <typename T> struct Blk8;
+template <> struct Blk8<bf16> {
+  bf16x8 v;
+  template <bool WHOLE> __device__ __forceinline__ void load(const bf16* row, int c, int n) {
+    if (WHOLE) v = *reinterpret_cast<const blk_bf16x8_u*>(row + min(c, n - 8));
+    else if (c + 8 <= n) v = *reinterpret_cast<const blk_bf16x8_u*>(row + c);
+    else if (c < n) v = blk_tail8(row, c, n);
+    else v = bf16x8{};
   }
+  template <bool WHOLE> __device__ __forceinline__ void get(float (&o)[8], int c, int n) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (WHOLE && c >= n) ? 0.f : (float)v[e];
+  }
+};
+template <> struct Blk8<float> {
+  f32x4 v[2];
+  template <bool WHOLE> __device__ __forceinline__ void load(const float* row, int c, int n) {
+    if (WHOLE) {
+      const float* p = row + min(c, n - 8);
+      v[0] = *reinterpret_cast<const blk_f32x4_u*>(p); v[1] = *reinterpret_cast<const blk_f32x4_u*>(p + 4);
+    } else if (c + 8 <= n) {
+      v[0] = *reinterpret_cast<const blk_f32x4_u*>(row + c); v[1] = *reinterpret_cast<const blk_f32x4_u*>(row + c + 4);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e >> 2][e & 3] = c + e < n ? row[c + e] : 0.f;
+    }
+  }
+  template <bool WHOLE> __device__ __forceinline__ void get(float (&o)[8], int c, int n) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (WHOLE && c >= n) ? 0.f : v[e >> 2][e & 3];
+  }
+};
+template <bool WHOLE, typename T> __device__ __forceinline__ void blk_load8(const T* row, int c, int n, float (&v)[8]) {
+  Blk8<T> r;
+  r.template load<WHOLE>(row, c, n);
+  r.template get<WHOLE>(v, c, n);
 }
 __device__ __forceinline__ void blk_store8(bf16* row, int c, int n, const float (&v)[8]) {
   if (c + 8 <= n) {

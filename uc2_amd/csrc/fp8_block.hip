@@ -6,20 +6,22 @@
 #include "fp8_block.h"
 
 // a wave takes 512 columns of R rows: R loads in flight, then R reductions over 16 lanes
-template <typename T, int R>
+template <typename T, int R, bool WHOLE>
 __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(int M, int K, int Kp, const T* __restrict__ x, long long ldx, unsigned char* __restrict__ q,
                                                              unsigned* __restrict__ scale, int groups, long long items) {
   const int lane = threadIdx.x & 63;
   const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (item >= items) return;
   const int rb = (int)(item / groups), g = (int)(item - (long long)rb * groups), c = g * 512 + lane * 8;
-  float v[R][8];
+  Blk8<T> x8[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) if (rb * R + r < M) blk_load8(x + (size_t)(rb * R + r) * ldx, c, K, v[r]);
+  for (int r = 0; r < R; ++r) x8[r].template load<WHOLE>(x + (size_t)min(rb * R + r, M - 1) * ldx, c, K);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int row = rb * R + r;
-    if (row < M) blk_quant_row(v[r], c, Kp, q + (size_t)row * Kp, scale + (size_t)g * M + row, lane);
+    float v[8];
+    x8[r].template get<WHOLE>(v, c, K);
+    if (row < M) blk_quant_row(v, c, Kp, q + (size_t)row * Kp, scale + (size_t)g * M + row, lane);
   }
 }
 extern "C" int uc2_fp8_quant_rows(int dtype, int M, int K, const void* x, long long ldx, void* out, void* scale, void* stream) {
@@ -33,23 +35,29 @@ extern "C" int uc2_fp8_quant_rows(int dtype, int M, int K, const void* x, long l
   const long long items = (long long)((M + R - 1) / R) * groups, blocks = (items + 3) / 4;
   UC2_CHECK_ARG(blocks < (1ll << 31));
   hipStream_t st = (hipStream_t)stream;
-#define QROWS(T_, R_) hipLaunchKernelGGL((fp8_quant_rows_kernel<T_, R_>), dim3((unsigned)blocks), dim3(256), 0, st, M, K, Kp, (const T_*)x, ldx, (unsigned char*)out, (unsigned*)scale, groups, items)
+#define QROWS_(T_, R_, W_) hipLaunchKernelGGL((fp8_quant_rows_kernel<T_, R_, W_>), dim3((unsigned)blocks), dim3(256), 0, st, M, K, Kp, (const T_*)x, ldx, (unsigned char*)out, (unsigned*)scale, groups, items)
+#define QROWS(T_, R_) do { if (K % 8 == 0) QROWS_(T_, R_, true); else QROWS_(T_, R_, false); } while (0)
   if (dtype == 1) { if (R == 4) QROWS(bf16, 4); else QROWS(bf16, 1); } else { if (R == 4) QROWS(float, 4); else QROWS(float, 1); }
   UC2_LAUNCH_CHECK();
   return 0;
 }
 
 // one workgroup per 128 x 128 block; a thread holds 8 x 8 elements, so its 8-byte pieces of W^T are made in registers
-template <typename T>
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void fp8_quant_square_kernel(int N, int K, int Np, int Kp, const T* __restrict__ w, long long ldw, unsigned char* __restrict__ q,
                                                                unsigned char* __restrict__ scale, unsigned char* __restrict__ qt, unsigned char* __restrict__ scale_t) {
   __shared__ float wm[4];
   const int kb = blockIdx.x, nb = blockIdx.y, t = threadIdx.x, r0 = nb * 128 + (t >> 4) * 8, c0 = kb * 128 + (t & 15) * 8;
   float v[8][8], m = 0.f;
+  Blk8<T> w8[8];
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
-    if (r0 + r < N) blk_load8(w + (size_t)(r0 + r) * ldw, c0, K, v[r]);
-    else {
+    w8[r].template load<WHOLE>(w + (size_t)min(r0 + r, N - 1) * ldw, c0, K);
+  }
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    w8[r].template get<WHOLE>(v[r], c0, K);
+    if (r0 + r >= N) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[r][e] = 0.f;
     }
@@ -91,8 +99,8 @@ extern "C" int uc2_fp8_quant_square(int dtype, int N, int K, const void* w, long
   UC2_CHECK_ARG(w && out && scale && (out_t == nullptr) == (scale_t == nullptr) && (((uintptr_t)out | (uintptr_t)out_t) & 7) == 0);
   const int Kp = (K + 127) / 128 * 128, Np = (N + 127) / 128 * 128;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == 1) hipLaunchKernelGGL(fp8_quant_square_kernel<bf16>, dim3(Kp / 128, Np / 128), dim3(256), 0, st, N, K, Np, Kp, (const bf16*)w, ldw, (unsigned char*)out, (unsigned char*)scale, (unsigned char*)out_t, (unsigned char*)scale_t);
-  else hipLaunchKernelGGL(fp8_quant_square_kernel<float>, dim3(Kp / 128, Np / 128), dim3(256), 0, st, N, K, Np, Kp, (const float*)w, ldw, (unsigned char*)out, (unsigned char*)scale, (unsigned char*)out_t, (unsigned char*)scale_t);
+#define QSQ(T_, W_) hipLaunchKernelGGL((fp8_quant_square_kernel<T_, W_>), dim3(Kp / 128, Np / 128), dim3(256), 0, st, N, K, Np, Kp, (const T_*)w, ldw, (unsigned char*)out, (unsigned char*)scale, (unsigned char*)out_t, (unsigned char*)scale_t)
+  if (dtype == 1) { if (K % 8 == 0) QSQ(bf16, true); else QSQ(bf16, false); } else { if (K % 8 == 0) QSQ(float, true); else QSQ(float, false); }
   UC2_LAUNCH_CHECK();
   return 0;
 }

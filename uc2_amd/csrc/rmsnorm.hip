@@ -30,7 +30,7 @@ template <int NW> __device__ __forceinline__ float row_sum(float v, float* red, 
   return t;
 }
 
-template <typename T, int NW, int NV, bool Q>
+template <typename T, int NW, int NV, bool Q, bool WHOLE>
 __global__ __launch_bounds__(NW == 16 ? 1024 : 256) void rms_fwd_kernel(RmsArgs a) {
   constexpr int RPB = NW == 1 ? 4 : 1;                // rows per workgroup
   __shared__ float red[NW > 1 ? NW : 1];
@@ -41,17 +41,24 @@ __global__ __launch_bounds__(NW == 16 ? 1024 : 256) void rms_fwd_kernel(RmsArgs 
   const T* res = a.res ? (const T*)a.res + (size_t)row * a.H : nullptr;
   float v[NV][8];
   float ss = 0.f;
+  Blk8<T> x8[NV], r8[NV];
+  Blk8<float> w8[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = ((i * NW + w) * 64 + lane) * 8;
-    blk_load8(x, c, a.H, v[i]);
+  for (int i = 0; i < NV; ++i) x8[i].template load<WHOLE>(x, ((i * NW + w) * 64 + lane) * 8, a.H);
+  if (res) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) r8[i].template load<WHOLE>(res, ((i * NW + w) * 64 + lane) * 8, a.H);
   }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) w8[i].template load<WHOLE>(a.w, ((i * NW + w) * 64 + lane) * 8, a.H);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) x8[i].template get<WHOLE>(v[i], ((i * NW + w) * 64 + lane) * 8, a.H);
   if (res) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = ((i * NW + w) * 64 + lane) * 8;
       float r[8];
-      blk_load8(res, c, a.H, r);
+      r8[i].template get<WHOLE>(r, c, a.H);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = to_f<T>(from_f<T>(v[i][e] + r[e]));
       blk_store8((T*)a.s_out + (size_t)row * a.H, c, a.H, v[i]);
@@ -68,7 +75,7 @@ __global__ __launch_bounds__(NW == 16 ? 1024 : 256) void rms_fwd_kernel(RmsArgs 
   for (int i = 0; i < NV; ++i) {
     const int c = ((i * NW + w) * 64 + lane) * 8;
     float g[8];
-    blk_load8(a.w, c, a.H, g);
+    w8[i].template get<WHOLE>(g, c, a.H);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * r * g[e];
     if (a.y) blk_store8((T*)a.y + (size_t)row * a.H, c, a.H, v[i]);
@@ -77,7 +84,7 @@ __global__ __launch_bounds__(NW == 16 ? 1024 : 256) void rms_fwd_kernel(RmsArgs 
 }
 
 // dx and the workgroup's share of dw: rows are dealt to the waves (NW = 1) or workgroups in turn, each lane keeps the sums of its own columns
-template <typename T, int NW, int NV>
+template <typename T, int NW, int NV, bool WHOLE>
 __global__ __launch_bounds__(NW == 16 ? 1024 : 256) void rms_bwd_kernel(RmsArgs a) {
   constexpr int RPB = NW == 1 ? 4 : 1;
   __shared__ float red[NW > 1 ? NW : 1];
@@ -86,18 +93,28 @@ __global__ __launch_bounds__(NW == 16 ? 1024 : 256) void rms_bwd_kernel(RmsArgs 
   float dw[NV][8], g[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    blk_load8(a.w, ((i * NW + w) * 64 + lane) * 8, a.H, g[i]);
+    blk_load8<WHOLE>(a.w, ((i * NW + w) * 64 + lane) * 8, a.H, g[i]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[i][e] = 0.f;
   }
   for (int row = blockIdx.x * RPB + (NW == 1 ? wv : 0); row < a.M; row += gridDim.x * RPB) {
     const size_t at = (size_t)row * a.H;
     float h[NV][8], d[NV][8];
+    Blk8<T> s8[NV], y8[NV], z8[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) blk_load8((const T*)a.s + at, ((i * NW + w) * 64 + lane) * 8, a.H, h[i]);
+    for (int i = 0; i < NV; ++i) s8[i].template load<WHOLE>((const T*)a.s + at, ((i * NW + w) * 64 + lane) * 8, a.H);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) blk_load8((const T*)a.dy + at, ((i * NW + w) * 64 + lane) * 8, a.H, d[i]);
+    for (int i = 0; i < NV; ++i) y8[i].template load<WHOLE>((const T*)a.dy + at, ((i * NW + w) * 64 + lane) * 8, a.H);
+    if (a.ds) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) z8[i].template load<WHOLE>((const T*)a.ds + at, ((i * NW + w) * 64 + lane) * 8, a.H);
+    }
     const float r = a.rstd_in[row];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      s8[i].template get<WHOLE>(h[i], ((i * NW + w) * 64 + lane) * 8, a.H);
+      y8[i].template get<WHOLE>(d[i], ((i * NW + w) * 64 + lane) * 8, a.H);
+    }
     float c = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -113,7 +130,7 @@ __global__ __launch_bounds__(NW == 16 ? 1024 : 256) void rms_bwd_kernel(RmsArgs 
     for (int i = 0; i < NV; ++i) {
       const int col = ((i * NW + w) * 64 + lane) * 8;
       float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (a.ds) blk_load8((const T*)a.ds + at, col, a.H, z);
+      if (a.ds) z8[i].template get<WHOLE>(z, col, a.H);
 #pragma unroll
       for (int e = 0; e < 8; ++e) z[e] = fmaf(r, fmaf(-h[i][e], c, d[i][e]), z[e]);
       blk_store8((T*)a.dx + at, col, a.H, z);
@@ -142,18 +159,21 @@ __global__ __launch_bounds__(NW == 16 ? 1024 : 256) void rms_bwd_kernel(RmsArgs 
     for (int i = 0; i < NV; ++i) blk_store8(out, ((i * NW + w) * 64 + lane) * 8, a.H, dw[i]);
   }
 }
-// dw[c] = sum of the n workgroups' shares, in a fixed order: 64 columns per workgroup, 16 waves over the rows
+// dw[c] = sum of the n workgroups' shares, in a fixed order: 16 columns per workgroup, 64 rows at a time
 __global__ __launch_bounds__(1024) void rms_dw_kernel(int n, int H, const float* __restrict__ part, float* __restrict__ dw) {
-  __shared__ float red[16][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  __shared__ float red[64][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
   float s = 0.f;
-  if (c < H) for (int i = w; i < n; i += 16) s += part[(size_t)i * H + c];
-  red[w][lane] = s;
+  if (c < H) {
+#pragma unroll 8
+    for (int i = y; i < n; i += 64) s += part[(size_t)i * H + c];
+  }
+  red[y][x] = s;
   __syncthreads();
-  if (w == 0 && c < H) {
+  if (threadIdx.x < 16 && c < H) {
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += red[i][lane];
+    for (int i = 0; i < 64; ++i) t += red[i][x];
     dw[c] = t;
   }
 }
@@ -168,7 +188,7 @@ static int rms_bwd_blocks(int M, int H) {
   int nw, nv;
   rms_shape(H, nw, nv);
   const int rows = nw == 1 ? (M + 3) / 4 : M;
-  return rows < 1024 ? rows : 1024;                   // about four workgroups of 256 per CU
+  return rows < 512 ? rows : 512;                     // two workgroups per CU: 66560 x 1024 in 104 us, 110 with twice or four times as many
 }
 #define RMS_GO(KERN, T_, ...)                                                                                                       \
   do {                                                                                                                              \
@@ -191,7 +211,12 @@ extern "C" int uc2_rms_fwd(int dtype, int M, int H, const void* x, const void* r
   rms_shape(H, nw, nv);
   const int blocks = nw == 1 ? (M + 3) / 4 : M, threads = nw == 16 ? 1024 : 256;
   hipStream_t st = (hipStream_t)stream;
-#define RMS_F(T_, NW_, NV_, Q_) hipLaunchKernelGGL((rms_fwd_kernel<T_, NW_, NV_, Q_>), dim3(blocks), dim3(threads), 0, st, a)
+  const bool whole = H % 8 == 0;
+#define RMS_F(T_, NW_, NV_, Q_)                                                                                                     \
+  do {                                                                                                                              \
+    if (whole) hipLaunchKernelGGL((rms_fwd_kernel<T_, NW_, NV_, Q_, true>), dim3(blocks), dim3(threads), 0, st, a);                  \
+    else hipLaunchKernelGGL((rms_fwd_kernel<T_, NW_, NV_, Q_, false>), dim3(blocks), dim3(threads), 0, st, a);                       \
+  } while (0)
   if (dtype == 1) { if (q_out) RMS_GO(RMS_F, bf16, true); else RMS_GO(RMS_F, bf16, false); }
   else { if (q_out) RMS_GO(RMS_F, float, true); else RMS_GO(RMS_F, float, false); }
   UC2_LAUNCH_CHECK();
@@ -204,7 +229,7 @@ extern "C" int uc2_rms_bwd(int dtype, int M, int H, const void* dy, const void* 
   UC2_CHECK_ARG(M >= 0 && M <= (1 << 30) && H >= 1 && H <= 16384);
   hipStream_t st = (hipStream_t)stream;
   if (M == 0) {
-    if (dgamma) hipLaunchKernelGGL(rms_dw_kernel, dim3((H + 63) / 64), dim3(1024), 0, st, 0, H, (const float*)nullptr, dgamma);
+    if (dgamma) hipLaunchKernelGGL(rms_dw_kernel, dim3((H + 15) / 16), dim3(1024), 0, st, 0, H, (const float*)nullptr, dgamma);
     UC2_LAUNCH_CHECK();
     return 0;
   }
@@ -215,9 +240,14 @@ extern "C" int uc2_rms_bwd(int dtype, int M, int H, const void* dy, const void* 
   int nw, nv;
   rms_shape(H, nw, nv);
   const int blocks = rms_bwd_blocks(M, H), threads = nw == 16 ? 1024 : 256;
-#define RMS_B(T_, NW_, NV_, ...) hipLaunchKernelGGL((rms_bwd_kernel<T_, NW_, NV_>), dim3(blocks), dim3(threads), 0, st, a)
+  const bool whole = H % 8 == 0;
+#define RMS_B(T_, NW_, NV_, ...)                                                                                                    \
+  do {                                                                                                                              \
+    if (whole) hipLaunchKernelGGL((rms_bwd_kernel<T_, NW_, NV_, true>), dim3(blocks), dim3(threads), 0, st, a);                      \
+    else hipLaunchKernelGGL((rms_bwd_kernel<T_, NW_, NV_, false>), dim3(blocks), dim3(threads), 0, st, a);                           \
+  } while (0)
   if (dtype == 1) RMS_GO(RMS_B, bf16, 0); else RMS_GO(RMS_B, float, 0);
-  if (dgamma) hipLaunchKernelGGL(rms_dw_kernel, dim3((H + 63) / 64), dim3(1024), 0, st, blocks, H, (const float*)ws, dgamma);
+  if (dgamma) hipLaunchKernelGGL(rms_dw_kernel, dim3((H + 15) / 16), dim3(1024), 0, st, blocks, H, (const float*)ws, dgamma);
   UC2_LAUNCH_CHECK();
   return 0;
 }

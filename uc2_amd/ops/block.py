@@ -10,7 +10,8 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import call, dt, ptr, stream
-from .base import GEMM_AUTO, _Timed, _require_cuda, device_guard
+from .base import _Timed, _require_cuda, device_guard
+from .linear import colsum_accum
 
 BLOCK = 128
 
@@ -136,15 +137,22 @@ class LinearBlockFp8Fn(torch.autograd.Function):
         with device_guard(dy2):
             if ctx.needs_input_grad[0]:
                 dx = gemm_fp8_block(fp8_quantize_block(dy2), BlockWeight(wt, st)).view(shp)
-            if ctx.needs_input_grad[1]:
-                dw = torch.zeros((N, K), dtype=torch.float32, device=dy2.device)
-                if M:
-                    call("uc2_gemm", dt(dy2.dtype), 1, 1, N, K, M, ptr(dy2), dy2.stride(0), ptr(x2), x2.stride(0), ptr(dw), K, 1, None, 0, None, None, 0, 0, 1,
-                         GEMM_AUTO, None, 0, 0, stream())
-                dw = dw if wtype == torch.float32 else dw.to(wtype)
-            if ctx.needs_input_grad[2]:
-                db = torch.zeros(N, dtype=torch.float32, device=dy2.device)
-                call("uc2_colsum_accum", dt(dy2.dtype), M, N, ptr(dy2), dy2.stride(0), None, ptr(db), stream())
+            need_db = ctx.needs_input_grad[2]
+            if ctx.needs_input_grad[1] and M:
+                dw = torch.empty((N, K), dtype=torch.float32, device=dy2.device)
+                db = torch.empty(N, dtype=torch.float32, device=dy2.device) if need_db else None
+                n = _lib.load().uc2_linear_wgrad_workspace(M, N, K)
+                ws = torch.empty(n, dtype=torch.uint8, device=dy2.device) if n else None
+                call("uc2_linear_wgrad", M, N, K, ptr(dy2), dy2.stride(0), ptr(x2), x2.stride(0), ptr(dw), K, ptr(db), ptr(ws), n, stream())
+            else:
+                if ctx.needs_input_grad[1]:
+                    dw = torch.zeros((N, K), dtype=torch.float32, device=dy2.device)
+                if need_db:
+                    db = torch.zeros(N, dtype=torch.float32, device=dy2.device)
+                    if M:
+                        colsum_accum(dy2, db)
+            if dw is not None and wtype != torch.float32:
+                dw = dw.to(wtype)
         return dx, dw, db
 
 
