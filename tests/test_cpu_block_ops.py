@@ -7,9 +7,21 @@ import torch
 
 import block_ref as R
 from uc2_amd import _lib, ops
-from uc2_amd.ops.cross import _CrossAttn, _CrossAttnGrad
+from uc2_amd.ops.cross import _ATTN, _GRAD
 
 P = 4096                        # an aligned address; no check dereferences it
+I, F, A, L = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong
+
+
+class _CrossAttn(ctypes.Structure):             # Uc2CrossAttn
+    _fields_ = ([(n, I) for n in "dtype B Lq Lk nh nkv D".split()] + [("scale", F), ("drop_p", F)] + [(n, A) for n in "qkv"]
+                + [(n, L) for n in "q_sb q_sl q_sh k_sb k_sl k_sh v_sb v_sl v_sh".split()]
+                + [("key_mask", A), ("key_mask_sb", L), ("k_lens", A), ("out", A), ("o_sb", L), ("o_sl", L), ("o_sh", L), ("lse", A), ("seed", A), ("site", ctypes.c_uint64)])
+
+
+class _CrossAttnGrad(ctypes.Structure):         # Uc2CrossAttnGrad
+    _fields_ = ([("dout", A), ("dout_sb", L), ("dout_sl", L), ("dout_sh", L), ("dq", A), ("dk", A), ("dv", A)]
+                + [(n, L) for n in "dq_sb dq_sl dq_sh dk_sb dk_sl dk_sh dv_sb dv_sl dv_sh".split()])
 
 
 def attn(**kw):
@@ -20,7 +32,7 @@ def attn(**kw):
 
 
 @pytest.mark.parametrize("bad", [dict(dtype=2), dict(D=48), dict(D=0), dict(nkv=3), dict(nkv=0), dict(B=-1), dict(Lq=-1), dict(Lk=-2), dict(drop_p=1.0), dict(drop_p=-0.5), dict(q=0),
-                                 dict(k=0), dict(out=0), dict(q=P + 2), dict(v=P + 8), dict(q_sl=257), dict(k_sh=4), dict(o_sb=-8), dict(Lq=1 << 30)])
+                                 dict(k=0), dict(out=0), dict(q=P + 2), dict(v=P + 8), dict(q_sl=257), dict(k_sh=4), dict(o_sb=-8), dict(k_sl=1 << 22), dict(Lq=1 << 30)])
 def test_cross_attention_argument_errors(bad):
     lib = _lib.load()
     assert lib.uc2_xattn_fwd(ctypes.byref(attn(**bad)), None, 0, None) == -1
@@ -98,9 +110,24 @@ def test_cpu_tensors_are_refused():
             f()
 
 
-def test_structures_match_the_header():
-    """sizes as a C compiler lays the header's structures out (pointers of 8 bytes)"""
-    assert ctypes.sizeof(_CrossAttn) == 216 and ctypes.sizeof(_CrossAttnGrad) == 128
+def test_structures_match_the_header(tmp_path):
+    """the binding's packed structures, these here and a C compiler's: the same sizes, and each field at the same place"""
+    import os
+    import subprocess
+    fields = [(t, n) for t, c in (("Uc2CrossAttn", _CrossAttn), ("Uc2CrossAttnGrad", _CrossAttnGrad)) for n, _ in c._fields_]
+    src = tmp_path / "s.c"
+    src.write_text('#include "uc2_hip.h"\n#include <stdio.h>\nint main(void) {\n' + "".join('printf("%%zu ", offsetof(%s, %s));\n' % f for f in fields)
+                   + 'printf("%zu %zu", sizeof(Uc2CrossAttn), sizeof(Uc2CrossAttnGrad)); return 0; }\n')
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.check_call(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "s")])
+    want = [int(x) for x in subprocess.check_output([str(tmp_path / "s")]).split()]
+    here = [getattr(c, n).offset for c in (_CrossAttn, _CrossAttnGrad) for n, _ in c._fields_] + [ctypes.sizeof(_CrossAttn), ctypes.sizeof(_CrossAttnGrad)]
+    assert want == here and [_ATTN.size, _GRAD.size] == here[-2:]
+    packed = _CrossAttn.from_buffer_copy(_ATTN.pack(*range(1, 8), 0.5, 0.25, *range(10, 32)))
+    got = [getattr(packed, n) for n, _ in _CrossAttn._fields_]
+    assert got == [*range(1, 8), 0.5, 0.25, *range(10, 32)]
+    packed = _CrossAttnGrad.from_buffer_copy(_GRAD.pack(*range(1, 17)))
+    assert [getattr(packed, n) for n, _ in _CrossAttnGrad._fields_] == list(range(1, 17))
 
 
 def test_oracle_rounds_as_torch_does():

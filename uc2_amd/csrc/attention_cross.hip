@@ -138,32 +138,71 @@ __device__ __forceinline__ float xa_key_bias(const XaArgs& a, int b, int key, in
   return m <= XA_REMOVED ? -INFINITY : m * XA_LOG2E;
 }
 
-// staging of TT rows x D of two tensors by NT threads, through registers
+// Staging of TT rows x D of two tensors by NT threads, through registers.  A thread's chunks lie at the same 32-bit offsets from the tile's first row in every
+// tile (packed rows: where G divides TT), so a tile's loads cost no vector arithmetic; no branch around them: rows behind the last one load that
+// one's, and keep() clears what takes no part on the way into LDS.
 template <typename T, int D, int NT, bool PACKED> struct XaStage {
   typedef XaCfg<T, D> C;
   static constexpr int N = C::TT * C::CPR / NT;                  // chunks per thread and tensor
   static_assert(N >= 1 && C::TT * C::CPR % NT == 0, "");
-  uint4 x[N], y[N];
-  __device__ __forceinline__ void load(const XaArgs& a, const XaView& X, const XaView& Y, int b, int kvh, int row0, int limit, int t) {
+  typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+  u32x4 x[N], y[N];
+  const char *px, *py;                                            // row 0 of the two tensors (wave-uniform)
+  unsigned ox[N], oy[N];
+  int limit, t;
+  __device__ __forceinline__ unsigned off(const XaArgs& a, const XaView& X, int r, int c) const {
+    if (!PACKED || a.G == 1) return (unsigned)(r * (int)X.sl) + c * 16;
+    const int i = (int)((unsigned)r / (unsigned)a.G);
+    return (unsigned)(i * (int)X.sl + (r - i * a.G) * (int)X.sh) + c * 16;
+  }
+  __device__ __forceinline__ void init(const XaArgs& a, const XaView& X, const XaView& Y, int b, int kvh, int limit_, int t_) {
+    limit = limit_; t = t_;
+    px = X.p + b * X.sb + (PACKED ? kvh * a.G : kvh) * X.sh;
+    py = Y.p + b * Y.sb + (PACKED ? kvh * a.G : kvh) * Y.sh;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int idx = t + n * NT, row = row0 + idx / C::CPR, c = idx % C::CPR;
-      bool take = row < limit;
-      if (!PACKED && take && a.kmask) take = !(a.kmask[b * a.kmask_sb + row] <= XA_REMOVED);
-      x[n] = uint4{0, 0, 0, 0}; y[n] = uint4{0, 0, 0, 0};
-      if (take) {
-        x[n] = *reinterpret_cast<const uint4*>(xa_row<PACKED>(a, X, b, kvh, row) + c * 16);
-        y[n] = *reinterpret_cast<const uint4*>(xa_row<PACKED>(a, Y, b, kvh, row) + c * 16);
+      const int idx = t + n * NT;
+      ox[n] = off(a, X, idx / C::CPR, idx % C::CPR);
+      oy[n] = off(a, Y, idx / C::CPR, idx % C::CPR);
+    }
+  }
+  // every chunk of tile tt (tt * TT < limit)
+  __device__ __forceinline__ void load(const XaArgs& a, const XaView& X, const XaView& Y, int tt) {
+    const int row0 = tt * C::TT;
+    const bool even = !PACKED || a.G == 1 || C::TT % a.G == 0;    // (uniform)
+    if (even && row0 + C::TT <= limit) {
+      const int i0 = PACKED ? row0 / a.G : row0;
+      const char *qx = px + (long long)i0 * X.sl, *qy = py + (long long)i0 * Y.sl;
+#pragma unroll
+      for (int n = 0; n < N; ++n) { x[n] = *reinterpret_cast<const u32x4*>(qx + ox[n]); y[n] = *reinterpret_cast<const u32x4*>(qy + oy[n]); }
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int idx = t + n * NT, r = min(row0 + idx / C::CPR, limit - 1), c = idx % C::CPR;
+        int i = r, g = 0;
+        if (PACKED) xa_split(a, r, i, g);
+        x[n] = *reinterpret_cast<const u32x4*>(px + (long long)i * X.sl + (long long)g * X.sh + c * 16);
+        y[n] = *reinterpret_cast<const u32x4*>(py + (long long)i * Y.sl + (long long)g * Y.sh + c * 16);
       }
     }
   }
-  __device__ __forceinline__ void store(char* lx, char* ly, int t) {
+  // mask: the key mask's row, or null
+  __device__ __forceinline__ void store(char* lx, char* ly, int tt, const float* mask) {
+    const int row0 = tt * C::TT;
+    if (mask || row0 + C::TT > limit) {                           // (uniform)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int r = row0 + (t + n * NT) / C::CPR;
+        const bool keep = r < limit && !(mask && mask[min(r, limit - 1)] <= XA_REMOVED);
+        if (!keep) { x[n] = u32x4{0, 0, 0, 0}; y[n] = u32x4{0, 0, 0, 0}; }
+      }
+    }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int idx = t + n * NT, row = idx / C::CPR, c = idx % C::CPR;
-      const int off = row * C::RB + ((c ^ xa_swz<C::CPR>(row)) << 4);
-      *reinterpret_cast<uint4*>(lx + off) = x[n];
-      *reinterpret_cast<uint4*>(ly + off) = y[n];
+      const int o = row * C::RB + ((c ^ xa_swz<C::CPR>(row)) << 4);
+      *reinterpret_cast<u32x4*>(lx + o) = x[n];
+      *reinterpret_cast<u32x4*>(ly + o) = y[n];
     }
   }
 };
@@ -241,19 +280,21 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
     for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
   float m = -INFINITY, l = 0.f;
   XaStage<T, D, NS * 64, false> st;
+  st.init(a, a.k, a.v, b, kvh, len, t);
+  const float* kmask = a.kmask ? a.kmask + b * a.kmask_sb : nullptr;
   float bias = 0.f; uint32_t hash = 0;
   auto fetch = [&](int tt) __attribute__((always_inline)) {
-    st.load(a, a.k, a.v, b, kvh, tt * C::TT, len, t);
+    st.load(a, a.k, a.v, tt);
     if (t < C::TT) {
       bias = xa_key_bias(a, b, tt * C::TT + t, len);
       if (DROP) hash = attn_line_hash(seed, bh, tt * C::TT + t, UC2_ATTN_SALT_K);
     }
   };
-  auto put = [&](int buf) __attribute__((always_inline)) {
-    st.store(lk[buf], lv[buf], t);
+  auto put = [&](int tt, int buf) __attribute__((always_inline)) {
+    st.store(lk[buf], lv[buf], tt, kmask);
     if (t < C::TT) { lb[buf][t] = bias; if (DROP) lh[buf][t] = hash; }
   };
-  if (t0 < t1) { fetch(t0); put(0); }
+  if (t0 < t1) { fetch(t0); put(t0, 0); }
   __syncthreads();
   int buf = 0;
   for (int tt = t0; tt < t1; ++tt) {
@@ -261,20 +302,29 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
     f32x16 s[C::NB];
 #pragma unroll
     for (int n = 0; n < C::NB; ++n) s[n] = M::rows(lk[buf], n, q, lane);
-    // x = score in base 2, masked; its maximum over the tile
+    // the tile's maximum of x = scale2 s (+ mask), in base 2
+    const bool masked = a.kmask != nullptr || (tt + 1) * C::TT > len || a.scale2 < 0.f;      // (uniform)
     float mx = -INFINITY;
-    const bool masked = a.kmask != nullptr || (tt + 1) * C::TT > len;
+    if (masked) {
 #pragma unroll
-    for (int n = 0; n < C::NB; ++n)
+      for (int n = 0; n < C::NB; ++n)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        f32x4 bv = {0.f, 0.f, 0.f, 0.f};
-        if (masked) bv = *reinterpret_cast<const f32x4*>(&lb[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+        for (int k = 0; k < 4; ++k) {
+          const f32x4 bv = *reinterpret_cast<const f32x4*>(&lb[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { s[n][4 * k + e] = fmaf(s[n][4 * k + e], a.scale2, bv[e]); mx = fmaxf(mx, s[n][4 * k + e]); }
-      }
+          for (int e = 0; e < 4; ++e) { s[n][4 * k + e] = fmaf(s[n][4 * k + e], a.scale2, bv[e]); mx = fmaxf(mx, s[n][4 * k + e]); }
+        }
+    } else {
+#pragma unroll
+      for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[n][e]);
+      mx *= a.scale2;
+    }
     mx = fmaxf(mx, __shfl_xor(mx, 32));
-    if (__any(mx > m)) {
+    // m is the maximum the weights are taken against: brought up only once a row's has grown by 2^8 (weights up to 256 lose nothing in fp32 or bf16,
+    // and the output and sum are rescaled in the first tiles only)
+    if (__any(mx > m + 8.f)) {
       const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       l *= al;
 #pragma unroll
@@ -283,7 +333,7 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
         for (int e = 0; e < 16; ++e) o[db][e] *= al;
       m = mn;
     }
-    const float mu = m == -INFINITY ? 0.f : m;
+    const float mu = m == -INFINITY ? 0.f : m, sc = masked ? 1.f : a.scale2;
 #pragma unroll
     for (int n = 0; n < C::NB; ++n) {
       float p[16];
@@ -294,14 +344,14 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
         const uint32_t hh[4] = {hk.x, hk.y, hk.z, hk.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float v = __builtin_amdgcn_exp2f(s[n][4 * k + e] - mu);
+          const float v = __builtin_amdgcn_exp2f(fmaf(s[n][4 * k + e], sc, -mu));
           l += v;
           p[4 * k + e] = DROP ? (attn_keep(hq, hh[e], a.thresh) ? v * a.keep_scale : 0.f) : v;
         }
       }
       M::cols(lv[buf], n, p, o, lane);
     }
-    if (tt + 1 < t1) put(buf ^ 1);
+    if (tt + 1 < t1) put(tt + 1, buf ^ 1);
     __syncthreads();
     buf ^= 1;
   }
@@ -320,31 +370,36 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
   }
 }
 
-// joins the splits of the forward: a wave per row, lane = element (two per lane at D = 128, half the lanes idle at 32)
+// joins the splits of the forward (64 at most): a wave per row; lane s first holds split s's factor, then every lane sums its elements over the splits
 template <typename T, int D>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a) {
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (long long)a.BH * a.R;
   if (row >= rows) return;
   const int lane = threadIdx.x & 63, bh = (int)(row / a.R), r = (int)(row - (long long)bh * a.R);
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.pml[2 * (s * rows + row)]);
-  const float mu = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[2] = {0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  if (lane < a.splits) { const float2 v = *reinterpret_cast<const float2*>(a.pml + 2 * (lane * rows + row)); m = v.x; l = v.y; }
+  const float top = wave_max(m), mu = top == -INFINITY ? 0.f : top;
+  const float f = __builtin_amdgcn_exp2f(m - mu);
+  l = wave_sum(f * l);
+  constexpr int E = D / 64 > 0 ? D / 64 : 1;
+  float o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  const float* p = a.part + row * D + (D >= 64 ? lane : lane % D);
+#pragma unroll 8
   for (int s = 0; s < a.splits; ++s) {
-    const size_t at = s * rows + row;
-    const float f = __builtin_amdgcn_exp2f(a.pml[2 * at] - mu);
-    l += f * a.pml[2 * at + 1];
-    if (D >= 64 || lane < D) o[0] += f * a.part[at * D + lane];
-    if (D == 128) o[1] += f * a.part[at * D + 64 + lane];
+    const float w = __shfl(f, s);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(w, p[s * rows * D + 64 * e], o[e]);
   }
   const float inv = l > 0.f ? 1.0f / l : (l == l ? 0.f : l);
   const int b = bh / a.nkv, kvh = bh - b * a.nkv;
   int i, g;
   xa_split(a, r, i, g);
   T* out = reinterpret_cast<T*>(a.out.p + b * a.out.sb + (long long)i * a.out.sl + (long long)(kvh * a.G + g) * a.out.sh);
-  if (D >= 64 || lane < D) out[lane] = from_f<T>(o[0] * inv);
-  if (D == 128) out[64 + lane] = from_f<T>(o[1] * inv);
-  if (a.lse && lane == 0) a.lse[row] = m + __log2f(l);
+#pragma unroll
+  for (int e = 0; e < E; ++e) if (D >= 64 || lane < D) out[lane + 64 * e] = from_f<T>(o[e] * inv);
+  if (a.lse && lane == 0) a.lse[row] = top + __log2f(l);
 }
 
 // dQ (owned query rows, streamed keys) and delta[r] = dout . out, which the dK / dV kernel reads
@@ -385,25 +440,28 @@ __global__ __launch_bounds__(NS * 64) void xattn_dq_kernel(XaArgs a) {
     if (lse == -INFINITY) lse = INFINITY;                          // a row without any key: p = 0
     if (split == 0 && lane < 32) a.delta[(size_t)bh * a.R + r] = delta;
   }
+  const float nlse = -lse;
   f32x16 dq[C::DB];
 #pragma unroll
   for (int db = 0; db < C::DB; ++db)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dq[db][e] = 0.f;
   XaStage<T, D, NS * 64, false> st;
+  st.init(a, a.k, a.v, b, kvh, len, t);
+  const float* kmask = a.kmask ? a.kmask + b * a.kmask_sb : nullptr;
   float bias = 0.f; uint32_t hash = 0;
   auto fetch = [&](int tt) __attribute__((always_inline)) {
-    st.load(a, a.k, a.v, b, kvh, tt * C::TT, len, t);
+    st.load(a, a.k, a.v, tt);
     if (t < C::TT) {
       bias = xa_key_bias(a, b, tt * C::TT + t, len);
       if (DROP) hash = attn_line_hash(seed, bh, tt * C::TT + t, UC2_ATTN_SALT_K);
     }
   };
-  auto put = [&](int buf) __attribute__((always_inline)) {
-    st.store(lk[buf], lv[buf], t);
+  auto put = [&](int tt, int buf) __attribute__((always_inline)) {
+    st.store(lk[buf], lv[buf], tt, kmask);
     if (t < C::TT) { lb[buf][t] = bias; if (DROP) lh[buf][t] = hash; }
   };
-  if (t0 < t1) { fetch(t0); put(0); }
+  if (t0 < t1) { fetch(t0); put(t0, 0); }
   __syncthreads();
   int buf = 0;
   for (int tt = t0; tt < t1; ++tt) {
@@ -416,21 +474,21 @@ __global__ __launch_bounds__(NS * 64) void xattn_dq_kernel(XaArgs a) {
       float ds[16];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        f32x4 bv = {0.f, 0.f, 0.f, 0.f};
+        f32x4 bv = {nlse, nlse, nlse, nlse};
         uint4 hk = {0, 0, 0, 0};
-        if (masked) bv = *reinterpret_cast<const f32x4*>(&lb[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+        if (masked) bv += *reinterpret_cast<const f32x4*>(&lb[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
         if (DROP) hk = *reinterpret_cast<const uint4*>(&lh[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
         const uint32_t hh[4] = {hk.x, hk.y, hk.z, hk.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * k + e], a.scale2, bv[e]) - lse);
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * k + e], a.scale2, bv[e]));
           const float d = DROP ? (attn_keep(hq, hh[e], a.thresh) ? dp[4 * k + e] * a.keep_scale : 0.f) : dp[4 * k + e];
           ds[4 * k + e] = p * (d - delta);
         }
       }
       M::cols(lk[buf], n, ds, dq, lane);
     }
-    if (tt + 1 < t1) put(buf ^ 1);
+    if (tt + 1 < t1) put(tt + 1, buf ^ 1);
     __syncthreads();
     buf ^= 1;
   }
@@ -474,9 +532,10 @@ __global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) { dk[db][e] = 0.f; dv[db][e] = 0.f; }
   XaStage<T, D, NS * 64, true> st;
+  st.init(a, a.q, a.dout, b, kvh, a.R, t);
   float lse = 0.f, delta = 0.f; uint32_t hash = 0;
   auto fetch = [&](int tt) __attribute__((always_inline)) {
-    st.load(a, a.q, a.dout, b, kvh, tt * C::TT, a.R, t);
+    st.load(a, a.q, a.dout, tt);
     if (t < C::TT) {
       const int r = tt * C::TT + t;
       lse = INFINITY; delta = 0.f;                                 // behind the last row, and rows without any key: p = 0
@@ -488,11 +547,11 @@ __global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
       }
     }
   };
-  auto put = [&](int buf) __attribute__((always_inline)) {
-    st.store(lq[buf], lg[buf], t);
-    if (t < C::TT) { ls[buf][t] = lse; ld[buf][t] = delta; if (DROP) lh[buf][t] = hash; }
+  auto put = [&](int tt, int buf) __attribute__((always_inline)) {
+    st.store(lq[buf], lg[buf], tt, nullptr);
+    if (t < C::TT) { ls[buf][t] = -lse; ld[buf][t] = delta; if (DROP) lh[buf][t] = hash; }
   };
-  if (t0 < t1) { fetch(t0); put(0); }
+  if (t0 < t1) { fetch(t0); put(t0, 0); }
   __syncthreads();
   int buf = 0;
   for (int tt = t0; tt < t1; ++tt) {
@@ -505,13 +564,15 @@ __global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int at = n * 32 + 8 * k + 4 * (lane >> 5);
-        const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[buf][at]), dl = *reinterpret_cast<const f32x4*>(&ld[buf][at]);
+        f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[buf][at]);
+        const f32x4 dl = *reinterpret_cast<const f32x4*>(&ld[buf][at]);
+        if (a.kmask) lv += f32x4{bias, bias, bias, bias};
         uint4 hv = {0, 0, 0, 0};
         if (DROP) hv = *reinterpret_cast<const uint4*>(&lh[buf][at]);
         const uint32_t hh[4] = {hv.x, hv.y, hv.z, hv.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[4 * k + e], a.scale2, bias) - lv[e]);
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[4 * k + e], a.scale2, lv[e]));
           float d = dp[4 * k + e], y = x;
           if (DROP) { const bool keep = attn_keep(hh[e], hk, a.thresh); d = keep ? d * a.keep_scale : 0.f; y = keep ? x * a.keep_scale : 0.f; }
           p[4 * k + e] = y;
@@ -521,11 +582,17 @@ __global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
       M::cols(lg[buf], n, p, dv, lane);
       M::cols(lq[buf], n, ds, dk, lane);
     }
-    if (tt + 1 < t1) put(buf ^ 1);
+    if (tt + 1 < t1) put(tt + 1, buf ^ 1);
     __syncthreads();
     buf ^= 1;
   }
   if (key >= a.Lk) return;
+  if (!part) {                                                     // (without a mask its column was computed: on zero vectors, into this lane alone)
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) { dk[db][e] = 0.f; dv[db][e] = 0.f; }
+  }
   if (a.splits == 1) {
     xa_put_row<T, C::DB>(a.dk.p + b * a.dk.sb + (long long)key * a.dk.sl + kvh * a.dk.sh, dk, a.scale, lane);
     xa_put_row<T, C::DB>(a.dv.p + b * a.dv.sb + (long long)key * a.dv.sl + kvh * a.dv.sh, dv, 1.0f, lane);
@@ -592,7 +659,16 @@ static XaPlan xa_plan(const Uc2CrossAttn* p) {
   return r;
 }
 static bool xa_str_ok(long long sb, long long sl, long long sh, int el) {      // 16-byte rows
-  return ((sb | sl | sh) & (16 / el - 1)) == 0 && sb >= 0 && sl >= 0 && sh >= 0;
+  return ((sb | sl | sh) & (16 / el - 1)) == 0 && sb >= 0 && sl >= 0 && sh >= 0 && sl < (1 << 22) && sh < (1 << 22);      // (64 rows within 2^31 bytes)
+}
+// a dimension of one element has no stride
+static void xa_one(int n, long long& a, long long& b) { if (n <= 1) a = b = 0; }
+static Uc2CrossAttn xa_norm(const Uc2CrossAttn* p) {
+  Uc2CrossAttn d = *p;
+  xa_one(d.B, d.q_sb, d.o_sb); xa_one(d.Lq, d.q_sl, d.o_sl); xa_one(d.nh, d.q_sh, d.o_sh);
+  xa_one(d.B, d.k_sb, d.v_sb); xa_one(d.Lk, d.k_sl, d.v_sl); xa_one(d.nkv, d.k_sh, d.v_sh);
+  if (d.B <= 1) d.key_mask_sb = 0;
+  return d;
 }
 static int xa_check(const Uc2CrossAttn* p) {
   UC2_CHECK_ARG(p != nullptr);
@@ -654,8 +730,9 @@ extern "C" size_t uc2_xattn_workspace(const Uc2CrossAttn* p, int backward) {
   return backward ? pl.bwd : pl.fwd;
 }
 
-extern "C" int uc2_xattn_fwd(const Uc2CrossAttn* p, void* ws, size_t ws_bytes, void* stream) {
-  if (int e = xa_check(p)) return e;
+extern "C" int uc2_xattn_fwd(const Uc2CrossAttn* attn, void* ws, size_t ws_bytes, void* stream) {
+  if (int e = xa_check(attn)) return e;
+  const Uc2CrossAttn norm = xa_norm(attn), *p = &norm;
   if (p->B == 0 || p->Lq == 0) return 0;
   if (int e = xa_ptrs(p)) return e;
   const XaPlan pl = xa_plan(p);
@@ -684,9 +761,13 @@ extern "C" int uc2_xattn_fwd(const Uc2CrossAttn* p, void* ws, size_t ws_bytes, v
   return 0;
 }
 
-extern "C" int uc2_xattn_bwd(const Uc2CrossAttn* p, const Uc2CrossAttnGrad* g, void* ws, size_t ws_bytes, void* stream) {
-  if (int e = xa_check(p)) return e;
-  UC2_CHECK_ARG(g != nullptr);
+extern "C" int uc2_xattn_bwd(const Uc2CrossAttn* attn, const Uc2CrossAttnGrad* grad, void* ws, size_t ws_bytes, void* stream) {
+  if (int e = xa_check(attn)) return e;
+  UC2_CHECK_ARG(grad != nullptr);
+  const Uc2CrossAttn norm = xa_norm(attn), *p = &norm;
+  Uc2CrossAttnGrad gnorm = *grad, *g = &gnorm;
+  xa_one(p->B, g->dout_sb, g->dq_sb); xa_one(p->Lq, g->dout_sl, g->dq_sl); xa_one(p->nh, g->dout_sh, g->dq_sh);
+  xa_one(p->B, g->dk_sb, g->dv_sb); xa_one(p->Lk, g->dk_sl, g->dv_sl); xa_one(p->nkv, g->dk_sh, g->dv_sh);
   if (p->B == 0) return 0;
   const int el = p->dtype ? 2 : 4;
   UC2_CHECK_ARG(p->Lq == 0 || (g->dout && g->dq && p->lse));

@@ -133,11 +133,12 @@ class _NoGuard:
 
 
 _NO_GUARD = _NoGuard()
+_cur_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def device_guard(t):
     """with device_guard(x): launches go to x's device and to the stream that is current there (nothing to do on the current device)"""
-    return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _NO_GUARD if t.get_device() == _cur_device() else torch.cuda.device(t.device)
 
 
 # --------------------------------------------------------------------------------------

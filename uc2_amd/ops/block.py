@@ -10,6 +10,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import call, dt, ptr, stream
+from ..config import state
 from .base import _Timed, _require_cuda, device_guard
 from .linear import colsum_accum
 
@@ -45,19 +46,33 @@ def _float_matrix(x, what):
     return x2 if x2.stride(1) == 1 and (x2.stride(0) >= x2.shape[1] or x2.shape[0] <= 1) else x2.contiguous()
 
 
-def _rows_out(M, K, device):
+def _rows_out(M, K, x):
     Kp = _up(K)
-    return (torch.empty((M, Kp), dtype=torch.uint8, device=device), torch.empty(((Kp + 511) // 512, M), dtype=torch.int32, device=device))
+    return x.new_empty((M, Kp), dtype=torch.uint8), x.new_empty(((Kp + 511) // 512, M), dtype=torch.int32)
+
+
+def _quant_rows(x2):
+    """fp8_quantize_block of a matrix as _float_matrix returns it, on its device"""
+    M, K = x2.shape
+    q, s = _rows_out(M, K, x2)
+    call("uc2_fp8_quant_rows", dt(x2.dtype), M, K, x2.data_ptr(), max(x2.stride(0), K), q.data_ptr(), s.data_ptr(), stream())
+    return BlockRows(q, s, K)
 
 
 def fp8_quantize_block(x):
     """[..., K] (fp32 or bf16, any row stride) -> BlockRows of its rows, one launch"""
     x2 = _float_matrix(x, "fp8_quantize_block")
-    M, K = x2.shape
     with device_guard(x2):
-        q, s = _rows_out(M, K, x2.device)
-        call("uc2_fp8_quant_rows", dt(x2.dtype), M, K, ptr(x2), max(x2.stride(0), K), ptr(q), ptr(s), stream())
-    return BlockRows(q, s, K)
+        return _quant_rows(x2)
+
+
+def _quant_weight(w, transpose):
+    N, K = w.shape
+    Np, Kp = _up(N), _up(K)
+    q, s = w.new_empty((N, Kp), dtype=torch.uint8), w.new_empty((Np // BLOCK, Kp // BLOCK), dtype=torch.uint8)
+    qt, st = (w.new_empty((K, Np), dtype=torch.uint8), w.new_empty((Kp // BLOCK, Np // BLOCK), dtype=torch.uint8)) if transpose else (None, None)
+    call("uc2_fp8_quant_square", dt(w.dtype), N, K, w.data_ptr(), max(w.stride(0), K), q.data_ptr(), s.data_ptr(), ptr(qt), ptr(st), stream())
+    return (BlockWeight(q, s), BlockWeight(qt, st)) if transpose else BlockWeight(q, s)
 
 
 def fp8_quantize_weight_block(w, transpose=False):
@@ -66,14 +81,8 @@ def fp8_quantize_weight_block(w, transpose=False):
     if not torch.is_tensor(w) or w.dim() != 2:
         raise _lib.Uc2Error("fp8_quantize_weight_block: a weight of two dimensions is needed")
     w = _float_matrix(w, "fp8_quantize_weight_block")
-    N, K = w.shape
-    Np, Kp = _up(N), _up(K)
     with device_guard(w):
-        new = lambda *s: torch.empty(s, dtype=torch.uint8, device=w.device)  # noqa: E731
-        q, s = new(N, Kp), new(Np // BLOCK, Kp // BLOCK)
-        qt, st = (new(K, Np), new(Kp // BLOCK, Np // BLOCK)) if transpose else (None, None)
-        call("uc2_fp8_quant_square", dt(w.dtype), N, K, ptr(w), max(w.stride(0), K), ptr(q), ptr(s), ptr(qt), ptr(st), stream())
-    return (BlockWeight(q, s), BlockWeight(qt, st)) if transpose else BlockWeight(q, s)
+        return _quant_weight(w, transpose)
 
 
 def _block_bias(bias, N, device):
@@ -84,28 +93,34 @@ def _block_bias(bias, N, device):
     return bias if bias.is_contiguous() else bias.contiguous()
 
 
+def _gemm(a8, sa, b8, sb, bias):
+    (M, Kp), N = a8.shape, b8.shape[0]
+    out = a8.new_empty((M, N), dtype=torch.bfloat16)
+    call("uc2_gemm_fp8_block", M, N, Kp, a8.data_ptr(), Kp, sa.data_ptr(), max(M, 1), b8.data_ptr(), Kp, sb.data_ptr(), ptr(bias), out.data_ptr(), max(N, 1), stream())
+    return out
+
+
 def gemm_fp8_block(a, b, bias=None):
     """bf16 [M, N] = a b^T + bias of a = BlockRows [M, K] (fp8_quantize_block, rms_norm_fp8) and b = BlockWeight [N, K]
     (fp8_quantize_weight_block; any (data, scale) pair of that layout); fp32 sums, one rounding"""
-    a8, sa = a[0], a[1]
-    b8, sb = b[0], b[1]
-    for t, kind, what in ((a8, torch.uint8, "a.data"), (sa, torch.int32, "a.scale"), (b8, torch.uint8, "b.data"), (sb, torch.uint8, "b.scale")):
-        if t.dtype != kind or t.dim() != 2:
-            raise _lib.Uc2Error("gemm_fp8_block: %s must be a two-dimensional %s tensor" % (what, kind))
-        _require_cuda(t)
-        if t.device != a8.device:
-            raise _lib.Uc2Error("gemm_fp8_block: operands on %s and %s" % (a8.device, t.device))
+    a8, sa, b8, sb = a[0], a[1], b[0], b[1]
+    device = a8.device
+    if not (a8.dtype == b8.dtype == sb.dtype == torch.uint8 and sa.dtype == torch.int32):
+        raise _lib.Uc2Error("gemm_fp8_block: a = (uint8, int32 scales), b = (uint8, uint8 scales) expected, got %s, %s, %s, %s" % (a8.dtype, sa.dtype, b8.dtype, sb.dtype))
+    _require_cuda(a8)
+    if not sa.device == b8.device == sb.device == device:
+        raise _lib.Uc2Error("gemm_fp8_block: operands on %s, %s, %s and %s" % (device, sa.device, b8.device, sb.device))
+    if not (a8.dim() == b8.dim() == sa.dim() == sb.dim() == 2):
+        raise _lib.Uc2Error("gemm_fp8_block: operands and scales of two dimensions expected")
     (M, Kp), N = a8.shape, b8.shape[0]
-    if Kp % BLOCK or Kp == 0 or b8.shape[1] != Kp or tuple(sa.shape) != ((Kp + 511) // 512, M) or tuple(sb.shape) != ((N + BLOCK - 1) // BLOCK, Kp // BLOCK):
+    if Kp % BLOCK or Kp == 0 or b8.shape[1] != Kp or sa.shape != ((Kp + 511) // 512, M) or sb.shape != ((N + BLOCK - 1) // BLOCK, Kp // BLOCK):
         raise _lib.Uc2Error("gemm_fp8_block: shapes do not match: %s with scales %s against %s with scales %s"
                             % (tuple(a8.shape), tuple(sa.shape), tuple(b8.shape), tuple(sb.shape)))
     if not (a8.is_contiguous() and sa.is_contiguous() and b8.is_contiguous() and sb.is_contiguous()):
         raise _lib.Uc2Error("gemm_fp8_block: operands must be contiguous")
-    bias = _block_bias(bias, N, a8.device)
+    bias = _block_bias(bias, N, device)
     with device_guard(a8):
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=a8.device)
-        call("uc2_gemm_fp8_block", M, N, Kp, ptr(a8), Kp, ptr(sa), max(M, 1), ptr(b8), Kp, ptr(sb), ptr(bias), ptr(out), max(N, 1), stream())
-    return out
+        return _gemm(a8, sa, b8, sb, bias)
 
 
 class LinearBlockFp8Fn(torch.autograd.Function):
@@ -115,37 +130,39 @@ class LinearBlockFp8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         shp = x.shape
-        x2 = _float_matrix(x, "linear_fp8_block")
-        need_dx = ctx.needs_input_grad[0]
-        w = fp8_quantize_weight_block(weight, transpose=need_dx)
-        wt = None
-        if need_dx:
-            w, wt = w
-        y = gemm_fp8_block(fp8_quantize_block(x2), w, bias)
-        ctx.save_for_backward(x2 if ctx.needs_input_grad[1] else None, *((wt.data, wt.scale) if wt is not None else (None, None)))
-        ctx.cfg = (shp, tuple(weight.shape), weight.dtype, bias is not None)
-        return y.view(*shp[:-1], weight.shape[0])
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        x2, weight = _float_matrix(x, "linear_fp8_block"), _float_matrix(weight, "linear_fp8_block")
+        with device_guard(x2):
+            w, wt = _quant_weight(weight, True) if need_dx else (_quant_weight(weight, False), (None, None))
+            a = _quant_rows(x2)
+            y = _gemm(a.data, a.scale, w.data, w.scale, bias)
+        ctx.save_for_backward(x2 if need_dw else None, wt[0], wt[1])
+        ctx.cfg = (shp, weight.shape, weight.dtype)
+        return y if len(shp) == 2 else y.view(*shp[:-1], weight.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x2, wt, st = ctx.saved_tensors
-        shp, (N, K), wtype, _ = ctx.cfg
+        shp, (N, K), wtype = ctx.cfg
+        need_dx, need_dw, need_db = ctx.needs_input_grad
         dy2 = _float_matrix(dy, "linear_fp8_block")
         M = dy2.shape[0]
         dx = dw = db = None
         with device_guard(dy2):
-            if ctx.needs_input_grad[0]:
-                dx = gemm_fp8_block(fp8_quantize_block(dy2), BlockWeight(wt, st)).view(shp)
-            need_db = ctx.needs_input_grad[2]
-            if ctx.needs_input_grad[1] and M:
-                dw = torch.empty((N, K), dtype=torch.float32, device=dy2.device)
-                db = torch.empty(N, dtype=torch.float32, device=dy2.device) if need_db else None
+            if need_dx:
+                a = _quant_rows(dy2)
+                dx = _gemm(a.data, a.scale, wt, st, None)
+                if len(shp) != 2:
+                    dx = dx.view(shp)
+            if need_dw and M:
+                dw = dy2.new_empty((N, K), dtype=torch.float32)
+                db = dy2.new_empty(N, dtype=torch.float32) if need_db else None
                 n = _lib.load().uc2_linear_wgrad_workspace(M, N, K)
-                ws = torch.empty(n, dtype=torch.uint8, device=dy2.device) if n else None
-                call("uc2_linear_wgrad", M, N, K, ptr(dy2), dy2.stride(0), ptr(x2), x2.stride(0), ptr(dw), K, ptr(db), ptr(ws), n, stream())
+                ws = dy2.new_empty(n, dtype=torch.uint8) if n else None
+                call("uc2_linear_wgrad", M, N, K, dy2.data_ptr(), max(dy2.stride(0), N), x2.data_ptr(), max(x2.stride(0), K), dw.data_ptr(), K, ptr(db), ptr(ws), n, stream())
             else:
-                if ctx.needs_input_grad[1]:
+                if need_dw:
                     dw = torch.zeros((N, K), dtype=torch.float32, device=dy2.device)
                 if need_db:
                     db = torch.zeros(N, dtype=torch.float32, device=dy2.device)
@@ -168,8 +185,7 @@ def linear_fp8_block(x, weight, bias=None):
     if weight.device != x.device:
         raise _lib.Uc2Error("linear_fp8_block: x on %s, weight on %s" % (x.device, weight.device))
     dt(weight.dtype)
-    _block_bias(bias, weight.shape[0], x.device)
-    return LinearBlockFp8Fn.apply(x, weight, bias)
+    return LinearBlockFp8Fn.apply(x, weight, _block_bias(bias, weight.shape[0], x.device))
 
 
 # ---- root-mean-square norm ----------------------------------------------------------------------------------------------------------
@@ -177,30 +193,35 @@ def _rms_args(x, weight, residual, what):
     if not torch.is_tensor(x) or x.dim() < 1:
         raise _lib.Uc2Error("%s: a tensor of one dimension at least is needed" % what)
     _require_cuda(x)
-    H = x.shape[-1]
+    H, device = x.shape[-1], x.device
     dt(x.dtype)
-    if weight.dtype != torch.float32 or tuple(weight.shape) != (H,) or weight.device != x.device:
-        raise _lib.Uc2Error("%s: weight must be fp32 [%d] on %s" % (what, H, x.device))
+    if weight.dtype != torch.float32 or weight.shape != (H,) or weight.device != device:
+        raise _lib.Uc2Error("%s: weight must be fp32 [%d] on %s" % (what, H, device))
     if not 1 <= H <= 16384:
         raise _lib.Uc2Error("%s: rows of 1 to 16384 elements, got %d" % (what, H))
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != device):
         raise _lib.Uc2Error("%s: residual must have the shape, type and device of x" % what)
-    return H
+
+
+def _dense(x, H):
+    return x.contiguous() if x.dim() == 2 else x.reshape(-1, H).contiguous()
 
 
 def _rms_fwd(x, weight, eps, residual, want_y, want_rstd, want_q):
     H = x.shape[-1]
-    x2 = x.reshape(-1, H).contiguous()
-    r2 = None if residual is None else residual.reshape(-1, H).contiguous()
+    x2 = _dense(x, H)
+    r2 = None if residual is None else _dense(residual, H)
     w = weight.contiguous()
     M = x2.shape[0]
     s = torch.empty_like(x2) if r2 is not None else None
     y = torch.empty_like(x2) if want_y else None
-    rstd = torch.empty(M, dtype=torch.float32, device=x.device) if want_rstd else None
-    q, qs = _rows_out(M, H, x.device) if want_q else (None, None)
-    with _Timed("rms_fwd", x2.element_size() * M * H * (1 + (2 if r2 is not None else 0) + int(want_y)) + (M * H if want_q else 0)):
-        call("uc2_rms_fwd", dt(x2.dtype), M, H, ptr(x2), ptr(r2), ptr(w), float(eps), ptr(s), ptr(y), ptr(rstd), ptr(q), ptr(qs), stream())
-    return x2 if s is None else s, y, rstd, None if q is None else BlockRows(q, qs, H)
+    rstd = x2.new_empty(M, dtype=torch.float32) if want_rstd else None
+    q, qs = _rows_out(M, H, x2) if want_q else (None, None)
+    timed = _Timed("rms_fwd", x2.element_size() * M * H * (1 + 2 * (r2 is not None) + want_y) + M * H * want_q) if state.hbm_timer is not None else None
+    call("uc2_rms_fwd", dt(x2.dtype), M, H, x2.data_ptr(), ptr(r2), w.data_ptr(), eps, ptr(s), ptr(y), ptr(rstd), ptr(q), ptr(qs), stream())
+    if timed is not None:
+        timed.__exit__()
+    return x2 if s is None else s, y, rstd, BlockRows(q, qs, H) if want_q else None
 
 
 class RMSNormFn(torch.autograd.Function):
@@ -208,14 +229,16 @@ class RMSNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, eps, residual):
-        grad = any(ctx.needs_input_grad)
+        grad = True in ctx.needs_input_grad
         with device_guard(x):
             s, y, rstd, _ = _rms_fwd(x, weight, eps, residual, True, grad, False)
         if grad:
-            ctx.save_for_backward(s, weight, rstd)
+            ctx.save_for_backward(s, weight.contiguous(), rstd)
         ctx.set_materialize_grads(False)
-        ctx.shp, ctx.res = x.shape, residual is not None
-        return (y.view(x.shape), s.view(x.shape)) if residual is not None else y.view(x.shape)
+        ctx.shp = x.shape
+        if x.dim() != 2:
+            y, s = y.view(x.shape), s.view(x.shape)
+        return y if residual is None else (y, s)
 
     @staticmethod
     @once_differentiable
@@ -224,25 +247,31 @@ class RMSNormFn(torch.autograd.Function):
         M, H = s.shape
         if dy is None:                                   # only the stream is used
             return ds, torch.zeros_like(weight) if ctx.needs_input_grad[1] else None, None, ds
+        need_dx, need_dw, _, need_dr = ctx.needs_input_grad
         with device_guard(s):
-            dy2 = dy.reshape(-1, H).contiguous()
-            ds2 = None if ds is None else ds.reshape(-1, H).contiguous()
+            dy2 = _dense(dy, H)
+            ds2 = None if ds is None else _dense(ds, H)
             dx = torch.empty_like(s)
             dw = ws = None
-            if ctx.needs_input_grad[1]:
-                dw = torch.empty(H, dtype=torch.float32, device=s.device)
-                ws = torch.empty(max(_lib.load().uc2_rms_bwd_workspace(M, H), 4), dtype=torch.uint8, device=s.device)
-            with _Timed("rms_bwd", s.element_size() * M * H * (3 + (ds2 is not None))):
-                call("uc2_rms_bwd", dt(s.dtype), M, H, ptr(dy2), ptr(ds2), ptr(s), ptr(weight.contiguous()), ptr(rstd), ptr(dx), ptr(dw), ptr(ws),
-                     0 if ws is None else ws.numel(), stream())
-        dx = dx.view(ctx.shp)
-        return dx if ctx.needs_input_grad[0] else None, dw, None, dx if ctx.res and ctx.needs_input_grad[3] else None
+            n = 0
+            if need_dw:
+                dw = torch.empty_like(weight)
+                n = _lib.load().uc2_rms_bwd_workspace(M, H)
+                ws = s.new_empty(n, dtype=torch.uint8)
+            timed = _Timed("rms_bwd", s.element_size() * M * H * (3 + (ds2 is not None))) if state.hbm_timer is not None else None
+            call("uc2_rms_bwd", dt(s.dtype), M, H, dy2.data_ptr(), ptr(ds2), s.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), ptr(dw), ptr(ws), n,
+                 stream())
+            if timed is not None:
+                timed.__exit__()
+        if dx.shape != ctx.shp:
+            dx = dx.view(ctx.shp)
+        return dx if need_dx else None, dw, None, dx if need_dr else None
 
 
 def rms_norm(x, weight, eps=1e-6, residual=None):
     """root-mean-square norm over the last dimension (fp32 or bf16, weight fp32): y, or (y, s) with s = x + residual, the stream to carry on"""
     _rms_args(x, weight, residual, "rms_norm")
-    return RMSNormFn.apply(x, weight, eps, residual)
+    return RMSNormFn.apply(x, weight, float(eps), residual)
 
 
 def rms_norm_fp8(x, weight, eps=1e-6, residual=None):
@@ -252,5 +281,5 @@ def rms_norm_fp8(x, weight, eps=1e-6, residual=None):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise _lib.Uc2Error("rms_norm_fp8 has no gradient: call it under torch.no_grad(), or use rms_norm and linear_fp8_block")
     with device_guard(x):
-        s, _, _, q = _rms_fwd(x, weight, eps, residual, False, False, True)
+        s, _, _, q = _rms_fwd(x, weight, float(eps), residual, False, False, True)
     return q, x if residual is None else s.view(x.shape)

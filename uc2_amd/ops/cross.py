@@ -1,53 +1,51 @@
 """Attention from one sequence to the states of another (cross attention with per-sequence lengths and shared key heads).  Part of
 uc2_amd.ops.  Beside AttentionGeneralFn (fp32 math, one thread per row, the additive [Lq, Lk] mask of MultiheadAttention)."""
-import ctypes
-import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import check, dt, ptr, stream
+from ..config import state
 from .base import _Timed, _require_cuda, device_guard, rng
 
-_I, _F, _P, _L = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong
-
-
-class _CrossAttn(ctypes.Structure):              # Uc2CrossAttn
-    _fields_ = [("dtype", _I), ("B", _I), ("Lq", _I), ("Lk", _I), ("nh", _I), ("nkv", _I), ("D", _I), ("scale", _F), ("drop_p", _F),
-                ("q", _P), ("k", _P), ("v", _P), ("q_sb", _L), ("q_sl", _L), ("q_sh", _L), ("k_sb", _L), ("k_sl", _L), ("k_sh", _L),
-                ("v_sb", _L), ("v_sl", _L), ("v_sh", _L), ("key_mask", _P), ("key_mask_sb", _L), ("k_lens", _P),
-                ("out", _P), ("o_sb", _L), ("o_sl", _L), ("o_sh", _L), ("lse", _P), ("seed", _P), ("site", ctypes.c_uint64)]
-
-
-class _CrossAttnGrad(ctypes.Structure):          # Uc2CrossAttnGrad
-    _fields_ = [("dout", _P), ("dout_sb", _L), ("dout_sl", _L), ("dout_sh", _L), ("dq", _P), ("dk", _P), ("dv", _P),
-                ("dq_sb", _L), ("dq_sl", _L), ("dq_sh", _L), ("dk_sb", _L), ("dk_sl", _L), ("dk_sh", _L), ("dv_sb", _L), ("dv_sl", _L), ("dv_sh", _L)]
+# Uc2CrossAttn and Uc2CrossAttnGrad (include/uc2_hip.h), packed in native alignment: a ctypes.Structure of as many fields takes 5 us to fill
+_ATTN = struct.Struct("@7i2f3P9qPqPP3qPPQ")
+_GRAD = struct.Struct("@P3q3P9q")
 
 
 def _rows16(x):
-    """x itself where the kernels can read it in place (contiguous heads, rows of 16-byte alignment), else a contiguous copy"""
-    el = 16 // x.element_size()
-    if x.stride(3) == 1 and x.data_ptr() % 16 == 0 and all(x.shape[i] <= 1 or (x.stride(i) % el == 0) for i in range(3)):
+    """x itself where the kernels can read it in place (contiguous heads, rows of 16-byte alignment less than 2^22 elements apart), else a
+    contiguous copy"""
+    sb, sl, sh, sd = x.stride()
+    B, L, nh, _ = x.shape
+    es = x.element_size()
+    if (sd == 1 and x.data_ptr() % 16 == 0 and (B <= 1 or sb * es % 16 == 0) and (L <= 1 or sl * es % 16 == 0 and sl < 1 << 22)
+            and (nh <= 1 or sh * es % 16 == 0 and sh < 1 << 22)):
         return x
     return x.clone(memory_format=torch.contiguous_format)          # (contiguous() would hand an unaligned dense tensor back)
 
 
-def _strides(x):
-    """batch, row and head strides; those of dimensions of one element do not matter (and need not be aligned)"""
-    return tuple(x.stride(i) if x.shape[i] > 1 else 0 for i in range(3))
-
-
 def _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site):
     B, Lq, nh, D = q.shape
-    return _CrossAttn(dt(q.dtype), B, Lq, k.shape[1], nh, k.shape[2], D, scale, drop_p, ptr(q), ptr(k), ptr(v), *_strides(q), *_strides(k), *_strides(v),
-                      ptr(key_mask), 0 if key_mask is None or key_mask.shape[0] <= 1 else key_mask.stride(0), ptr(k_lens), ptr(out), *_strides(out),
-                      ptr(lse), ptr(seed), site)
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    return _ATTN.pack(dt(q.dtype), B, Lq, k.shape[1], nh, k.shape[2], D, scale, drop_p, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                      qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                      0 if key_mask is None else key_mask.data_ptr(), 0 if key_mask is None else key_mask.stride(0), 0 if k_lens is None else k_lens.data_ptr(),
+                      out.data_ptr(), os[0], os[1], os[2], 0 if lse is None else lse.data_ptr(), 0 if seed is None else seed.data_ptr(), site)
 
 
-def _xattn_ws(desc, backward, device):
-    n = _lib.load().uc2_xattn_workspace(ctypes.byref(desc), backward)
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+def _run(name, nbytes, device, desc, grad=None):
+    lib = _lib.load()
+    n = lib.uc2_xattn_workspace(desc, 0 if grad is None else 1)
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    timed = _Timed(name, nbytes) if state.hbm_timer is not None else None
+    rc = lib.uc2_xattn_fwd(desc, ptr(ws), n, stream()) if grad is None else lib.uc2_xattn_bwd(desc, grad, ptr(ws), n, stream())
+    if timed is not None:
+        timed.__exit__()
+    if rc:
+        check(rc)
 
 
 class CrossAttentionFn(torch.autograd.Function):
@@ -58,13 +56,12 @@ class CrossAttentionFn(torch.autograd.Function):
         with device_guard(q):
             q, k, v = _rows16(q), _rows16(k), _rows16(v)
             B, Lq, nh, D = q.shape
-            grad = any(ctx.needs_input_grad[:3])
-            out = torch.empty((B, Lq, nh, D), dtype=q.dtype, device=q.device)
-            lse = torch.empty((B, k.shape[2], Lq, nh // k.shape[2]), dtype=torch.float32, device=q.device) if grad else None
-            desc = _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site)
-            ws = _xattn_ws(desc, 0, q.device)
-            with _Timed("xattn_fwd", q.element_size() * (2 * q.numel() + k.numel() + v.numel())):
-                check(_lib.load().uc2_xattn_fwd(ctypes.byref(desc), ptr(ws), 0 if ws is None else ws.numel(), stream()))
+            need = ctx.needs_input_grad
+            grad = need[0] or need[1] or need[2]
+            out = q.new_empty((B, Lq, nh, D))
+            lse = q.new_empty((B, k.shape[2], Lq, nh // k.shape[2]), dtype=torch.float32) if grad else None
+            _run("xattn_fwd", q.element_size() * (2 * q.numel() + k.numel() + v.numel()), q.device,
+                 _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site))
         if grad:
             ctx.save_for_backward(q, k, v, key_mask, k_lens, out, lse, seed)
             ctx.cfg = (scale, drop_p, site)
@@ -77,13 +74,12 @@ class CrossAttentionFn(torch.autograd.Function):
         scale, drop_p, site = ctx.cfg
         with device_guard(q):
             dout = _rows16(dout)
-            new = lambda x: torch.empty(x.shape, dtype=x.dtype, device=x.device)  # noqa: E731
-            dq, dk, dv = new(q), new(k), new(v)
-            desc = _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site)
-            grad = _CrossAttnGrad(ptr(dout), *_strides(dout), ptr(dq), ptr(dk), ptr(dv), *_strides(dq), *_strides(dk), *_strides(dv))
-            ws = _xattn_ws(desc, 1, q.device)
-            with _Timed("xattn_bwd", q.element_size() * (4 * q.numel() + 2 * (k.numel() + v.numel()))):
-                check(_lib.load().uc2_xattn_bwd(ctypes.byref(desc), ctypes.byref(grad), ptr(ws), 0 if ws is None else ws.numel(), stream()))
+            dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+            gs, qs, ks = dout.stride(), dq.stride(), dk.stride()
+            grad = _GRAD.pack(dout.data_ptr(), gs[0], gs[1], gs[2], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
+                              ks[0], ks[1], ks[2])
+            _run("xattn_bwd", q.element_size() * (4 * q.numel() + 2 * (k.numel() + v.numel())), q.device,
+                 _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site), grad)
         return dq, dk, dv, None, None, None, None, None, None
 
 
@@ -95,39 +91,43 @@ def cross_attention(q, k, v, key_mask=None, k_lens=None, scale=None, drop_p=0.0,
       drop_p    dropout on the weights, drawn from ops.rng like the encoder's (site: tells two calls inside one ops.rng.scope() apart)
     Keys that take no part reach nothing, whatever they hold; a query that has none gets zeros and passes no gradient.  scale defaults to
     1 / sqrt(D).  Gradients for q, k and v; results repeat bit for bit."""
-    for t, what in ((q, "q"), (k, "k"), (v, "v")):
-        if not torch.is_tensor(t) or t.dim() != 4:
-            raise _lib.Uc2Error("cross_attention: %s must be a tensor [batch, length, heads, head dimension]" % what)
-        _require_cuda(t)
-        if t.dtype != q.dtype or t.device != q.device:
-            raise _lib.Uc2Error("cross_attention: q, k and v must have one type and device")
+    if not (torch.is_tensor(q) and torch.is_tensor(k) and torch.is_tensor(v) and q.dim() == k.dim() == v.dim() == 4):
+        raise _lib.Uc2Error("cross_attention: q, k and v must be tensors [batch, length, heads, head dimension]")
+    _require_cuda(q)
+    device = q.device
+    if k.device != device or v.device != device or not q.dtype == k.dtype == v.dtype:
+        raise _lib.Uc2Error("cross_attention: q, k and v must have one type and device")
     dt(q.dtype)
     B, Lq, nh, D = q.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+    kshape = k.shape
+    if kshape != v.shape or kshape[0] != B or kshape[3] != D:
         raise _lib.Uc2Error("cross_attention: k and v must be [%d, Lk, nkv, %d], got %s and %s" % (B, D, tuple(k.shape), tuple(v.shape)))
     if D not in (32, 64, 128):
         raise _lib.Uc2Error("cross_attention: head dimensions of 32, 64 and 128, got %d" % D)
-    Lk, nkv = k.shape[1], k.shape[2]
+    Lk, nkv = kshape[1], kshape[2]
     if nkv < 1 or nh < 1 or nh % nkv:
         raise _lib.Uc2Error("cross_attention: %d query heads over %d key heads" % (nh, nkv))
     if not 0.0 <= drop_p < 1.0:
         raise _lib.Uc2Error("cross_attention: drop_p in [0, 1), got %s" % drop_p)
     if k_lens is not None:
-        if not torch.is_tensor(k_lens) or k_lens.device != q.device or tuple(k_lens.shape) != (B,) or k_lens.dtype not in (torch.int32, torch.int64):
-            raise _lib.Uc2Error("cross_attention: k_lens must be an int32 or int64 tensor [%d] on %s" % (B, q.device))
-        k_lens = k_lens.clamp(0, Lk).to(torch.int32) if k_lens.dtype == torch.int64 else k_lens
+        if not torch.is_tensor(k_lens) or k_lens.device != device or k_lens.shape != (B,) or k_lens.dtype not in (torch.int32, torch.int64):
+            raise _lib.Uc2Error("cross_attention: k_lens must be an int32 or int64 tensor [%d] on %s" % (B, device))
+        if k_lens.dtype == torch.int64:
+            k_lens = k_lens.clamp(0, Lk).to(torch.int32)
         k_lens = k_lens.contiguous()
     if key_mask is not None:
-        if not torch.is_tensor(key_mask) or key_mask.device != q.device or not key_mask.is_floating_point():
-            raise _lib.Uc2Error("cross_attention: key_mask must be an additive float mask on %s" % q.device)
+        if not torch.is_tensor(key_mask) or key_mask.device != device or not key_mask.is_floating_point():
+            raise _lib.Uc2Error("cross_attention: key_mask must be an additive float mask on %s" % device)
         if key_mask.dim() == 4 and key_mask.shape[1] == 1 and key_mask.shape[2] == 1:
             key_mask = key_mask[:, 0, 0]
-        if tuple(key_mask.shape) != (B, Lk):
+        if key_mask.shape != (B, Lk):
             raise _lib.Uc2Error("cross_attention: key_mask must be [%d, %d], got %s" % (B, Lk, tuple(key_mask.shape)))
         if key_mask.requires_grad:
             raise _lib.Uc2Error("cross_attention: key_mask takes no gradient")
         key_mask = key_mask.float()
-        if key_mask.stride(1) != 1 and Lk > 1:
+        if Lk > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
-    seed = rng.snapshot(q.device) if drop_p > 0.0 else None
-    return CrossAttentionFn.apply(q, k, v, key_mask, k_lens, 1.0 / math.sqrt(D) if scale is None else float(scale), float(drop_p), seed, rng.site(site))
+    seed = None
+    if drop_p > 0.0:
+        seed, site = rng.snapshot(device), rng.site(site)
+    return CrossAttentionFn.apply(q, k, v, key_mask, k_lens, D ** -0.5 if scale is None else float(scale), float(drop_p), seed, site)
