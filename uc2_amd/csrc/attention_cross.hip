@@ -50,10 +50,13 @@ template <typename T, int D> struct XaCfg {
   static constexpr int DB = D / 32;                               // 32-wide blocks of the head dimension
 };
 
-// chunk swizzle of a row: 8 consecutive rows of one chunk column fall on 8 distinct 16-byte bank groups (row reads), and so do the 4 rows x 2
-// chunks of a transposing read
+// chunk swizzle of a row.  256 bytes (64 banks) hold 16 chunks: the 16 rows that a quarter wave reads one chunk column of fall on 16 of them, and so do
+// the 4 rows x 2 chunks x 2 halves of a transposing read twice over, which is its least (the first choice, by the row's low three bits, cost a third of
+// the LDS cycles in conflicts)
 template <int CPR> __device__ __forceinline__ int xa_swz(int row) {
-  return CPR == 4 ? ((row & 2) | ((row >> 2) & 1)) : (((row & 3) << 1) | ((row >> 2) & 1));
+  if (CPR == 4) return (row >> 2) & 3;
+  if (CPR == 8) return ((row & 2) << 1) | ((row & 4) >> 1) | ((row & 8) >> 3);
+  return ((row & 1) << 3) | ((row & 2) << 1) | ((row & 4) >> 1) | ((row & 8) >> 3);
 }
 
 template <typename T, int D> struct XaMma;
@@ -264,7 +267,7 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
   if (!xa_block(a, bh, tile, split)) return;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, b = bh / a.nkv, kvh = bh - b * a.nkv;
   const int r = (tile * NS + w) * 32 + (lane & 31);
-  const bool mine = r < a.R;
+  const bool mine = r < a.R, live = (tile * NS + w) * 32 < a.R;      // live: the wave has a row (the others only stage)
   const int len = xa_len(a, b), nt = (len + C::TT - 1) / C::TT, per = (nt + a.splits - 1) / a.splits;
   const int t0 = split * per, t1 = min(nt, t0 + per);
   const uint64_t seed = DROP ? a.seed_imm + (a.seed_ptr ? *a.seed_ptr : 0ull) : 0ull;
@@ -299,15 +302,18 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
   int buf = 0;
   for (int tt = t0; tt < t1; ++tt) {
     if (tt + 1 < t1) fetch(tt + 1);
+    if (live) {
     f32x16 s[C::NB];
+    const int left = len - tt * C::TT;                            // keys from this tile on: a block of 32 behind them is not computed
 #pragma unroll
-    for (int n = 0; n < C::NB; ++n) s[n] = M::rows(lk[buf], n, q, lane);
+    for (int n = 0; n < C::NB; ++n) if (n == 0 || n * 32 < left) s[n] = M::rows(lk[buf], n, q, lane);
     // the tile's maximum of x = scale2 s (+ mask), in base 2
     const bool masked = a.kmask != nullptr || (tt + 1) * C::TT > len || a.scale2 < 0.f;      // (uniform)
     float mx = -INFINITY;
     if (masked) {
 #pragma unroll
       for (int n = 0; n < C::NB; ++n)
+        if (n == 0 || n * 32 < left)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const f32x4 bv = *reinterpret_cast<const f32x4*>(&lb[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
@@ -336,6 +342,7 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
     const float mu = m == -INFINITY ? 0.f : m, sc = masked ? 1.f : a.scale2;
 #pragma unroll
     for (int n = 0; n < C::NB; ++n) {
+      if (n > 0 && n * 32 >= left) break;
       float p[16];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -350,6 +357,7 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
         }
       }
       M::cols(lv[buf], n, p, o, lane);
+    }
     }
     if (tt + 1 < t1) put(tt + 1, buf ^ 1);
     __syncthreads();
@@ -415,7 +423,7 @@ __global__ __launch_bounds__(NS * 64) void xattn_dq_kernel(XaArgs a) {
   if (!xa_block(a, bh, tile, split)) return;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, b = bh / a.nkv, kvh = bh - b * a.nkv;
   const int r = (tile * NS + w) * 32 + (lane & 31);
-  const bool mine = r < a.R;
+  const bool mine = r < a.R, live = (tile * NS + w) * 32 < a.R;      // live: the wave has a row (the others only stage)
   const int len = xa_len(a, b), nt = (len + C::TT - 1) / C::TT, per = (nt + a.splits - 1) / a.splits;
   const int t0 = split * per, t1 = min(nt, t0 + per);
   const uint64_t seed = DROP ? a.seed_imm + (a.seed_ptr ? *a.seed_ptr : 0ull) : 0ull;
@@ -469,6 +477,7 @@ __global__ __launch_bounds__(NS * 64) void xattn_dq_kernel(XaArgs a) {
     const bool masked = a.kmask != nullptr || (tt + 1) * C::TT > len;
 #pragma unroll
     for (int n = 0; n < C::NB; ++n) {
+      if (!live || tt * C::TT + n * 32 >= len) break;
       const f32x16 s = M::rows(lk[buf], n, q, lane);
       const f32x16 dp = M::rows(lv[buf], n, go, lane);
       float ds[16];
@@ -516,7 +525,7 @@ __global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
   const int key = (tile * NS + w) * 32 + (lane & 31);
   const int len = xa_len(a, b);
   const float bias = xa_key_bias(a, b, key, len);
-  const bool part = bias != -INFINITY;
+  const bool part = bias != -INFINITY, live = (tile * NS + w) * 32 < len;      // live: the wave has a key
   const int nt = tile * NS * 32 < len ? (a.R + C::TT - 1) / C::TT : 0;          // a tile behind the length: zeros
   const int per = (nt + a.splits - 1) / a.splits;
   const int t0 = split * per, t1 = min(nt, t0 + per);
@@ -558,6 +567,7 @@ __global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
     if (tt + 1 < t1) fetch(tt + 1);
 #pragma unroll
     for (int n = 0; n < C::NB; ++n) {
+      if (!live || tt * C::TT + n * 32 >= a.R) break;
       const f32x16 s = M::rows(lq[buf], n, kf, lane);
       const f32x16 dp = M::rows(lg[buf], n, vf, lane);
       float p[16], ds[16];

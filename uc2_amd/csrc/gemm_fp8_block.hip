@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void gemm_fp8_block_tile_kernel(BlkGemm p) {
     const int r = (t + n * 256) >> 3, c = t & 7;
     as[n] = p.A + (size_t)min(m0 + r, p.M - 1) * p.lda + c * 16;
     bs[n] = p.B + (size_t)min(n0 + r, p.N - 1) * p.ldb + c * 16;
-    off[n] = r * 128 + ((c ^ (r & 7)) << 4);
+    off[n] = r * 128 + ((c ^ ((r >> 1) & 7)) << 4);
   }
   int row[WB];
 #pragma unroll
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256) void gemm_fp8_block_tile_kernel(BlkGemm p) {
   unsigned sw[WB];
   fetch(0); put(0);
   __syncthreads();
-  const int sz = i & 7;
+  const int sz = (i >> 1) & 7;                                    // (16 rows of one chunk column: 16 places of the 256 bytes that the banks hold)
   for (int kt = 0; kt < p.Kb; ++kt) {
     const int buf = kt & 1;
     if (kt + 1 < p.Kb) fetch(kt + 1);

@@ -16,7 +16,8 @@ struct WgradArgs {
   float* part; float* pdb; int dsplits;                 // [splits][N][K], [dsplits][N]
 };
 
-__device__ __forceinline__ int wg_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+// chunk swizzle: the 8 rows x 4 chunks of a transposing read meet each of the 16 chunk columns twice, its least
+__device__ __forceinline__ int wg_swz(int row) { return ((row & 1) << 3) | ((row & 2) << 1) | ((row & 4) >> 1) | ((row & 8) >> 3); }
 // 8 columns of a row from the clamped column cc = min(c, n - 8) and row (no branch around the load: hipcc waits for a load at the end of a branch that
 // uses it); wg_fix moves them into place and clears what is behind the row or the matrix.  Rows of less than 8 columns (TINY): one by one.
 template <bool TINY> __device__ __forceinline__ bf16x8 wg_load(const bf16* x, long long ld, int m, int M, int cc, int n) {
