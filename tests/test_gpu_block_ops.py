@@ -576,6 +576,17 @@ def test_operators_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(o1, step())) and all(torch.equal(a, b) for a, b in zip(o2, train()))
 
 
+def test_second_derivatives_are_refused():
+    q, k, v, dout = attn_inputs(1, 3, 9, 2, 2, 64, F32)
+    x, g = normal((4, 96), 1).requires_grad_(), torch.ones(96, device=DEV, requires_grad=True)
+    qg = q.clone().requires_grad_()
+    xb, w = normal((4, 96), 1, BF16).requires_grad_(), normal((8, 96), 2).requires_grad_()
+    for out, leaf in ((ops.cross_attention(qg, k, v), qg), (ops.rms_norm(x, g), x), (ops.linear_fp8_block(xb, w).float(), xb)):
+        d, = torch.autograd.grad(out.square().sum(), [leaf], create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(d.float().sum(), [leaf])
+
+
 def test_refusals_on_the_device():
     q, k, v, _ = attn_inputs(2, 3, 9, 4, 2, 64, BF16)
     for bad in (dict(key_mask=torch.zeros(2, 8, device=DEV)), dict(key_mask=torch.zeros(2, 9, device=DEV, dtype=torch.bool)), dict(k_lens=torch.zeros(3, device=DEV, dtype=torch.int32)),

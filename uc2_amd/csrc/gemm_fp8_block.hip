@@ -152,27 +152,27 @@ __global__ __launch_bounds__(256) void gemm_fp8_block_tile_kernel(BlkGemm p) {
 }
 
 static void blk_launch_tiles(const BlkGemm& p, hipStream_t st) {
-  if (p.M <= 64) {
-    const dim3 grid((p.N + 15) / 16);
+  // the rows kernel while it is one workgroup per CU at most: its waves share the blocks of K, where a tile takes them one after the other (measured,
+  // us: 256 x 1024 x 4096 11.3 against 14.3 in 64 x 64 tiles, 64 x 4096 x 1024 4.7 / 5.3; beyond, 512 x 768 x 768 5.8 / 4.8, 128 x 4096 x 1024 7.0 / 5.5)
+  if ((long long)((p.N + 15) / 16) * ((p.M + 63) / 64) <= 256) {
+    const dim3 grid((p.N + 15) / 16, (p.M + 63) / 64);
     if (p.M <= 16) hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<1>, grid, dim3(512), 0, st, p);
     else if (p.M <= 32) hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<2>, grid, dim3(512), 0, st, p);
     else hipLaunchKernelGGL(gemm_fp8_block_rows_kernel<4>, grid, dim3(512), 0, st, p);
     return;
   }
-  // 128 x 128 tiles once they fill the chip, 64 x 64 ones below
+  // 128 x 128 tiles once there is one for each CU, 64 x 64 ones below (4096 x 1024 x 4096: 34 us against 37; 4096 x 768 x 768, 192 tiles: 10.0 / 8.3)
   const long long t128 = (long long)((p.M + 127) / 128) * ((p.N + 127) / 128);
   const int T = t128 >= 256 ? 128 : 64;
   const dim3 grid((p.M + T - 1) / T, (p.N + T - 1) / T);
   if (T == 128) hipLaunchKernelGGL(gemm_fp8_block_tile_kernel<4>, grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL(gemm_fp8_block_tile_kernel<2>, grid, dim3(256), 0, st, p);
 }
-#ifndef BLK_PP_MIN
-#define BLK_PP_MIN 128
-#endif
 static void blk_launch(BlkGemm p, hipStream_t st) {
-  // whole 256 x 256 tiles go to the persistent kernel once there are enough of them; what is left of the rows and of the columns to the tiles here
+  // whole 256 x 256 tiles go to the persistent kernel from 128 of them on, where the two meet (8192 x 1024 x 4096: 44 us both; 192 tiles of K = 768: 16.5
+  // against 21.7; 96: 13.9 / 13.0); what is left of the rows and of the columns to the kernels above
   const int M0 = p.M / 256 * 256, N0 = p.N / 256 * 256;
-  if ((long long)(M0 / 256) * (N0 / 256) >= BLK_PP_MIN && ((uintptr_t)p.sb & 1) == 0) {
+  if ((long long)(M0 / 256) * (N0 / 256) >= 128 && ((uintptr_t)p.sb & 1) == 0) {
     GemmArgs g{};                                                  // (the "bf16 view" of bytes: K and leading dimensions halved)
     g.A = p.A; g.B = p.B; g.C = p.C; g.bias = p.bias; g.M = M0; g.N = N0; g.K = p.Kb * 64; g.lda = p.lda / 2; g.ldb = p.ldb / 2; g.ldc = g.ldaux = p.ldc;
     g.epi = EPI_NONE; g.split_k = 1; g.a_vec = g.b_vec = 1; g.alpha = 1.0f;

@@ -2,6 +2,7 @@
 device-side dropout seed state.  Part of uc2_amd.ops (see ops/__init__.py)."""
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ..config import state
@@ -139,6 +140,15 @@ _cur_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_d
 def device_guard(t):
     """with device_guard(x): launches go to x's device and to the stream that is current there (nothing to do on the current device)"""
     return _NO_GUARD if t.get_device() == _cur_device() else torch.cuda.device(t.device)
+
+
+def once(backward):
+    """once_differentiable (a second differentiation raises) for backward passes that are asked for a graph; without its wrapping, 4 us a call, otherwise"""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 # --------------------------------------------------------------------------------------

@@ -6,12 +6,11 @@ maximum pass, single tokens and first calls are as exact as any other, and an ou
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import call, dt, ptr, stream
 from ..config import state
-from .base import _Timed, _require_cuda, device_guard
+from .base import _Timed, _require_cuda, device_guard, once
 from .linear import colsum_accum
 
 BLOCK = 128
@@ -141,7 +140,7 @@ class LinearBlockFp8Fn(torch.autograd.Function):
         return y if len(shp) == 2 else y.view(*shp[:-1], weight.shape[0])
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dy):
         x2, wt, st = ctx.saved_tensors
         shp, (N, K), wtype = ctx.cfg
@@ -241,7 +240,7 @@ class RMSNormFn(torch.autograd.Function):
         return y if residual is None else (y, s)
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dy, ds=None):
         s, weight, rstd = ctx.saved_tensors
         M, H = s.shape

@@ -3,12 +3,11 @@ uc2_amd.ops.  Beside AttentionGeneralFn (fp32 math, one thread per row, the addi
 import struct
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import check, dt, ptr, stream
 from ..config import state
-from .base import _Timed, _require_cuda, device_guard, rng
+from .base import _Timed, _require_cuda, device_guard, once, rng
 
 # Uc2CrossAttn and Uc2CrossAttnGrad (include/uc2_hip.h), packed in native alignment: a ctypes.Structure of as many fields takes 5 us to fill
 _ATTN = struct.Struct("@7i2f3P9qPqPP3qPPQ")
@@ -68,7 +67,7 @@ class CrossAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dout):
         q, k, v, key_mask, k_lens, out, lse, seed = ctx.saved_tensors
         scale, drop_p, site = ctx.cfg
