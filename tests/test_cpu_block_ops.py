@@ -152,3 +152,12 @@ def test_oracle_attention_is_softmax():
     got, _ = R.attention(q, k, v, 0.2, None, None, dout)
     for a, b in zip(got, want):
         assert torch.allclose(a, b.detach(), atol=1e-12)
+
+
+def test_saved_pointers_are_read_from_the_call_structure():
+    from uc2_amd.ops.cross import _PTRS
+    names = [n for n, _ in _CrossAttn._fields_]
+    packed = _ATTN.pack(*range(1, 8), 0.5, 0.25, *range(10, 32))
+    value = dict(zip(names, (*range(1, 8), 0.5, 0.25, *range(10, 32))))
+    assert _PTRS.size == _ATTN.size
+    assert _PTRS.unpack(packed) == tuple(value[n] for n in ("q", "k", "v", "key_mask", "k_lens", "out", "lse", "seed", "site"))

@@ -576,6 +576,22 @@ def test_operators_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(o1, step())) and all(torch.equal(a, b) for a, b in zip(o2, train()))
 
 
+def test_saved_tensors_that_come_back_as_copies():
+    """saved-tensor hooks (offloading): the backward reads what they bring, not the tensors of the forward"""
+    q, k, v, dout = attn_inputs(2, 9, 70, 4, 2, 64, BF16)
+    want = run_attn(q, k, v, dout)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(DEV)):
+        qg, kg, vg = (t.detach().requires_grad_() for t in (q, k, v))
+        o = ops.cross_attention(qg, kg, vg)
+        x, g = normal((9, 96), 1).requires_grad_(), torch.ones(96, device=DEV, requires_grad=True)
+        y, s = ops.rms_norm(x, g, residual=x.detach())
+    got = torch.autograd.grad(o, [qg, kg, vg], dout)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[1:]))
+    x2 = x.detach().clone().requires_grad_()
+    y2, s2 = ops.rms_norm(x2, g, residual=x2.detach())
+    assert torch.equal(torch.autograd.grad([y, s], [x], [y, s])[0], torch.autograd.grad([y2, s2], [x2], [y2, s2])[0])
+
+
 def test_second_derivatives_are_refused():
     q, k, v, dout = attn_inputs(1, 3, 9, 2, 2, 64, F32)
     x, g = normal((4, 96), 1).requires_grad_(), torch.ones(96, device=DEV, requires_grad=True)

@@ -136,14 +136,14 @@ class LinearBlockFp8Fn(torch.autograd.Function):
             a = _quant_rows(x2)
             y = _gemm(a.data, a.scale, w.data, w.scale, bias)
         ctx.save_for_backward(x2 if need_dw else None, wt[0], wt[1])
-        ctx.cfg = (shp, weight.shape, weight.dtype)
+        ctx.cfg = (shp, weight.shape, weight.dtype, _lib.load().uc2_linear_wgrad_workspace(x2.shape[0], *weight.shape) if need_dw else 0)
         return y if len(shp) == 2 else y.view(*shp[:-1], weight.shape[0])
 
     @staticmethod
     @once
     def backward(ctx, dy):
         x2, wt, st = ctx.saved_tensors
-        shp, (N, K), wtype = ctx.cfg
+        shp, (N, K), wtype, n = ctx.cfg
         need_dx, need_dw, need_db = ctx.needs_input_grad
         dy2 = _float_matrix(dy, "linear_fp8_block")
         M = dy2.shape[0]
@@ -157,7 +157,6 @@ class LinearBlockFp8Fn(torch.autograd.Function):
             if need_dw and M:
                 dw = dy2.new_empty((N, K), dtype=torch.float32)
                 db = dy2.new_empty(N, dtype=torch.float32) if need_db else None
-                n = _lib.load().uc2_linear_wgrad_workspace(M, N, K)
                 ws = dy2.new_empty(n, dtype=torch.uint8) if n else None
                 call("uc2_linear_wgrad", M, N, K, dy2.data_ptr(), max(dy2.stride(0), N), x2.data_ptr(), max(x2.stride(0), K), dw.data_ptr(), K, ptr(db), ptr(ws), n, stream())
             else:
@@ -233,6 +232,7 @@ class RMSNormFn(torch.autograd.Function):
             s, y, rstd, _ = _rms_fwd(x, weight, eps, residual, True, grad, False)
         if grad:
             ctx.save_for_backward(s, weight.contiguous(), rstd)
+            ctx.ws = _lib.load().uc2_rms_bwd_workspace(*s.shape)
         ctx.set_materialize_grads(False)
         ctx.shp = x.shape
         if x.dim() != 2:
@@ -255,7 +255,7 @@ class RMSNormFn(torch.autograd.Function):
             n = 0
             if need_dw:
                 dw = torch.empty_like(weight)
-                n = _lib.load().uc2_rms_bwd_workspace(M, H)
+                n = ctx.ws
                 ws = s.new_empty(n, dtype=torch.uint8)
             timed = _Timed("rms_bwd", s.element_size() * M * H * (3 + (ds2 is not None))) if state.hbm_timer is not None else None
             call("uc2_rms_bwd", dt(s.dtype), M, H, dy2.data_ptr(), ptr(ds2), s.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), ptr(dw), ptr(ws), n,

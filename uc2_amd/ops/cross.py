@@ -12,6 +12,8 @@ from .base import _Timed, _require_cuda, device_guard, once, rng
 # Uc2CrossAttn and Uc2CrossAttnGrad (include/uc2_hip.h), packed in native alignment: a ctypes.Structure of as many fields takes 5 us to fill
 _ATTN = struct.Struct("@7i2f3P9qPqPP3qPPQ")
 _GRAD = struct.Struct("@P3q3P9q")
+# its pointers q, k, v, key_mask, k_lens, out, lse, seed (the order they are saved in) and what is left of it
+_PTRS = struct.Struct("@40x3P72xP8xPP24xPPQ")
 
 
 def _rows16(x):
@@ -35,16 +37,8 @@ def _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site):
                       out.data_ptr(), os[0], os[1], os[2], 0 if lse is None else lse.data_ptr(), 0 if seed is None else seed.data_ptr(), site)
 
 
-def _run(name, nbytes, device, desc, grad=None):
-    lib = _lib.load()
-    n = lib.uc2_xattn_workspace(desc, 0 if grad is None else 1)
-    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    timed = _Timed(name, nbytes) if state.hbm_timer is not None else None
-    rc = lib.uc2_xattn_fwd(desc, ptr(ws), n, stream()) if grad is None else lib.uc2_xattn_bwd(desc, grad, ptr(ws), n, stream())
-    if timed is not None:
-        timed.__exit__()
-    if rc:
-        check(rc)
+def _timed(name, nbytes):
+    return _Timed(name, nbytes) if state.hbm_timer is not None else None
 
 
 class CrossAttentionFn(torch.autograd.Function):
@@ -52,6 +46,7 @@ class CrossAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, key_mask, k_lens, scale, drop_p, seed, site):
+        lib = _lib.load()
         with device_guard(q):
             q, k, v = _rows16(q), _rows16(k), _rows16(v)
             B, Lq, nh, D = q.shape
@@ -59,26 +54,44 @@ class CrossAttentionFn(torch.autograd.Function):
             grad = need[0] or need[1] or need[2]
             out = q.new_empty((B, Lq, nh, D))
             lse = q.new_empty((B, k.shape[2], Lq, nh // k.shape[2]), dtype=torch.float32) if grad else None
-            _run("xattn_fwd", q.element_size() * (2 * q.numel() + k.numel() + v.numel()), q.device,
-                 _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site))
+            desc = _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site)
+            n = lib.uc2_xattn_workspace(desc, 0)
+            ws = q.new_empty(n, dtype=torch.uint8) if n else None
+            timed = _timed("xattn_fwd", q.element_size() * (2 * q.numel() + k.numel() + v.numel()))
+            rc = lib.uc2_xattn_fwd(desc, ptr(ws), n, stream())
+            if timed is not None:
+                timed.__exit__()
+        if rc:
+            check(rc)
         if grad:
             ctx.save_for_backward(q, k, v, key_mask, k_lens, out, lse, seed)
-            ctx.cfg = (scale, drop_p, site)
+            # what the backward would work out again on a thread that has just been woken up: the call structure, as long as the tensors that come
+            # back are the ones in it, and the workspace's size
+            ctx.cfg = (scale, drop_p, site, desc, lib.uc2_xattn_workspace(desc, 1))
         return out
 
     @staticmethod
     @once
     def backward(ctx, dout):
-        q, k, v, key_mask, k_lens, out, lse, seed = ctx.saved_tensors
-        scale, drop_p, site = ctx.cfg
+        saved = ctx.saved_tensors
+        q, k, v, key_mask, k_lens, out, lse, seed = saved
+        scale, drop_p, site, desc, n = ctx.cfg
+        lib = _lib.load()
         with device_guard(q):
             dout = _rows16(dout)
             dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+            ws = q.new_empty(n, dtype=torch.uint8)
+            if _PTRS.unpack(desc)[:-1] != tuple([0 if t is None else t.data_ptr() for t in saved]):      # (saved-tensor hooks may bring copies)
+                desc = _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site)
             gs, qs, ks = dout.stride(), dq.stride(), dk.stride()
             grad = _GRAD.pack(dout.data_ptr(), gs[0], gs[1], gs[2], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
                               ks[0], ks[1], ks[2])
-            _run("xattn_bwd", q.element_size() * (4 * q.numel() + 2 * (k.numel() + v.numel())), q.device,
-                 _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site), grad)
+            timed = _timed("xattn_bwd", q.element_size() * (4 * q.numel() + 2 * (k.numel() + v.numel())))
+            rc = lib.uc2_xattn_bwd(desc, grad, ws.data_ptr(), n, stream())
+            if timed is not None:
+                timed.__exit__()
+        if rc:
+            check(rc)
         return dq, dk, dv, None, None, None, None, None, None
 
 
