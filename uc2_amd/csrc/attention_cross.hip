@@ -27,15 +27,19 @@ typedef __attribute__((ext_vector_type(4))) __bf16 xa_bf16x4;
 struct XaView { const char* p; long long sb, sl, sh; };          // byte strides of batch, row, head
 struct XaOut { char* p; long long sb, sl, sh; };
 
+// a kernel's work: owned tiles per (batch, key head), splits of the streamed axis, blocks; partials [splits][B nkv][rows][..] (dkv: dK, then dV, per split)
+struct XaSide { int tiles, splits, blocks; float* part; };
+
 struct XaArgs {
   int B, Lq, Lk, nkv, G, R;                                       // R = Lq G packed rows per (batch, key head)
-  int tiles, splits, BH;                                          // owned tiles per (batch, key head), splits of the streamed axis, B nkv
+  int BH;                                                         // B nkv
+  XaSide fwd, dq, dkv;
   XaView q, k, v, o, dout;
-  XaOut out, dq, dk, dv;
+  XaOut out, gq, gk, gv;
   const float* kmask; long long kmask_sb; const int* klens;
   float scale, scale2;                                            // scale2 = scale log2 e
-  float* lse; float* delta;                                       // [B nkv][R], lse in base 2
-  float* part; float* pml;                                        // partials: [splits][B nkv][rows][..], maxima and sums [splits][B nkv][R][2]
+  float* lse;                                                     // [B nkv][R], base 2
+  float* pml;                                                     // the forward's maxima and sums [splits][B nkv][R][2]
   uint32_t thresh; float keep_scale; const uint64_t* seed_ptr; uint64_t seed_imm; int nh;
 };
 
@@ -210,6 +214,41 @@ template <typename T, int D, int NT, bool PACKED> struct XaStage {
   }
 };
 
+// delta of a staged tile of packed rows: the chunks of `out` beside XaStage's of dout, multiplied on the way into LDS and summed over a row's CPR
+// neighbouring threads
+template <typename T, int D, int NT> struct XaDelta {
+  typedef XaCfg<T, D> C;
+  static constexpr int N = C::TT * C::CPR / NT;
+  typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+  u32x4 z[N];
+  const char* p; int t;
+  __device__ __forceinline__ void init(const XaArgs& a, int b, int kvh, int t_) { t = t_; p = a.o.p + b * a.o.sb + (long long)(kvh * a.G) * a.o.sh; }
+  __device__ __forceinline__ void load(const XaArgs& a, int tt) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int idx = t + n * NT, r = min(tt * C::TT + idx / C::CPR, a.R - 1), c = idx % C::CPR;
+      int i, g;
+      xa_split(a, r, i, g);
+      z[n] = *reinterpret_cast<const u32x4*>(p + (long long)i * a.o.sl + (long long)g * a.o.sh + c * 16);
+    }
+  }
+  __device__ __forceinline__ void store(const XaArgs& a, const u32x4 (&y)[N], float* d, int tt) {
+    constexpr int E = 16 / sizeof(T);
+    typedef T V __attribute__((ext_vector_type(E)));
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int idx = t + n * NT, row = idx / C::CPR;
+      const V o = __builtin_bit_cast(V, z[n]), g = __builtin_bit_cast(V, y[n]);
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) s = fmaf((float)o[e], (float)g[e], s);
+#pragma unroll
+      for (int k = 1; k < C::CPR; k <<= 1) s += __shfl_xor(s, k);
+      if (idx % C::CPR == 0) d[row] = tt * C::TT + row < a.R ? s : 0.f;
+    }
+  }
+};
+
 // owned vectors of the lane: column r (query row or key), zeros where it takes no part
 template <typename T, int D, bool PACKED>
 __device__ __forceinline__ void xa_own(const XaArgs& a, const XaView& X, int b, int kvh, int r, bool take, int lane, typename XaMma<T, D>::Frag (&f)[XaCfg<T, D>::KS]) {
@@ -239,9 +278,8 @@ template <typename T, int DB> __device__ __forceinline__ void xa_put_row(char* r
 
 // block -> (batch and key head, owned tile, split): blocks go to the 8 XCDs in turn, the tiles and splits of one (batch, key head) share its
 // streamed rows, so they are put on one XCD and its L2 (worth nothing below 8 heads: plain order there)
-__device__ __forceinline__ bool xa_block(const XaArgs& a, int& bh, int& tile, int& split) {
-  const int per = a.tiles * a.splits;
-  int blk = blockIdx.x;
+__device__ __forceinline__ bool xa_block(const XaArgs& a, const XaSide& side, int blk, int& bh, int& tile, int& split) {
+  const int per = side.tiles * side.splits;
   if (a.BH >= 8) {
     const int x = blk & 7, n = blk >> 3, grp = n / per;
     bh = grp * 8 + x;
@@ -250,8 +288,8 @@ __device__ __forceinline__ bool xa_block(const XaArgs& a, int& bh, int& tile, in
     bh = blk / per;
     blk -= bh * per;
   }
-  tile = blk / a.splits;
-  split = blk - tile * a.splits;
+  tile = blk / side.splits;
+  split = blk - tile * side.splits;
   return bh < a.BH;
 }
 __device__ __forceinline__ int xa_len(const XaArgs& a, int b) { return a.klens ? max(0, min(a.klens[b], a.Lk)) : a.Lk; }
@@ -264,11 +302,11 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
   __shared__ __attribute__((aligned(16))) float lb[2][C::TT];
   __shared__ __attribute__((aligned(16))) uint32_t lh[2][DROP ? C::TT : 4];
   int bh, tile, split;
-  if (!xa_block(a, bh, tile, split)) return;
+  if (!xa_block(a, a.fwd, blockIdx.x, bh, tile, split)) return;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, b = bh / a.nkv, kvh = bh - b * a.nkv;
   const int r = (tile * NS + w) * 32 + (lane & 31);
   const bool mine = r < a.R, live = (tile * NS + w) * 32 < a.R;      // live: the wave has a row (the others only stage)
-  const int len = xa_len(a, b), nt = (len + C::TT - 1) / C::TT, per = (nt + a.splits - 1) / a.splits;
+  const int len = xa_len(a, b), nt = (len + C::TT - 1) / C::TT, per = (nt + a.fwd.splits - 1) / a.fwd.splits;
   const int t0 = split * per, t1 = min(nt, t0 + per);
   const uint64_t seed = DROP ? a.seed_imm + (a.seed_ptr ? *a.seed_ptr : 0ull) : 0ull;
   uint32_t hq = 0;
@@ -365,7 +403,7 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
   }
   l += __shfl_xor(l, 32);
   if (!mine) return;
-  if (a.splits == 1) {
+  if (a.fwd.splits == 1) {
     int i, g;
     xa_split(a, r, i, g);
     const float inv = l > 0.f ? 1.0f / l : (l == l ? 0.f : l);     // no key: zeros; NaN stays NaN
@@ -373,7 +411,7 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
     if (a.lse && lane < 32) a.lse[(size_t)bh * a.R + r] = m + __log2f(l);
   } else {
     const size_t row = ((size_t)split * a.BH + bh) * a.R + r;
-    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.part + row * D), o, 1.0f, lane);
+    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.fwd.part + row * D), o, 1.0f, lane);
     if (lane < 32) { a.pml[2 * row] = m; a.pml[2 * row + 1] = l; }
   }
 }
@@ -385,7 +423,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a) {
   if (row >= rows) return;
   const int lane = threadIdx.x & 63, bh = (int)(row / a.R), r = (int)(row - (long long)bh * a.R);
   float m = -INFINITY, l = 0.f;
-  if (lane < a.splits) { const float2 v = *reinterpret_cast<const float2*>(a.pml + 2 * (lane * rows + row)); m = v.x; l = v.y; }
+  if (lane < a.fwd.splits) { const float2 v = *reinterpret_cast<const float2*>(a.pml + 2 * (lane * rows + row)); m = v.x; l = v.y; }
   const float top = wave_max(m), mu = top == -INFINITY ? 0.f : top;
   const float f = __builtin_amdgcn_exp2f(m - mu);
   l = wave_sum(f * l);
@@ -393,9 +431,9 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a) {
   float o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  const float* p = a.part + row * D + (D >= 64 ? lane : lane % D);
+  const float* p = a.fwd.part + row * D + (D >= 64 ? lane : lane % D);
 #pragma unroll 8
-  for (int s = 0; s < a.splits; ++s) {
+  for (int s = 0; s < a.fwd.splits; ++s) {
     const float w = __shfl(f, s);
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = fmaf(w, p[s * rows * D + 64 * e], o[e]);
@@ -410,21 +448,27 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a) {
   if (a.lse && lane == 0) a.lse[row] = top + __log2f(l);
 }
 
-// dQ (owned query rows, streamed keys) and delta[r] = dout . out, which the dK / dV kernel reads
+// The backward is one launch of two kinds of workgroups, dK / dV and dQ: neither needs the other (each forms delta[r] = dout . out itself), so a short
+// problem pays one launch and one latency instead of two.
+template <typename T, int D, bool DROP> struct XaLds {
+  typedef XaCfg<T, D> C;
+  __attribute__((aligned(16))) char x[2][C::TT * C::RB], y[2][C::TT * C::RB];
+  __attribute__((aligned(16))) float s[2][C::TT], d[2][C::TT];
+  __attribute__((aligned(16))) uint32_t h[2][DROP ? C::TT : 4];
+};
+
+// dQ (owned query rows, streamed keys)
 //   dx = p (dp - delta),  dp = dout v^T (dropped as the forward's weights were),  dq = scale dx k
 template <typename T, int D, int NS, bool DROP>
-__global__ __launch_bounds__(NS * 64) void xattn_dq_kernel(XaArgs a) {
+__device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP>& sh) {
   typedef XaCfg<T, D> C;
   typedef XaMma<T, D> M;
-  __shared__ __attribute__((aligned(16))) char lk[2][C::TT * C::RB], lv[2][C::TT * C::RB];
-  __shared__ __attribute__((aligned(16))) float lb[2][C::TT];
-  __shared__ __attribute__((aligned(16))) uint32_t lh[2][DROP ? C::TT : 4];
   int bh, tile, split;
-  if (!xa_block(a, bh, tile, split)) return;
+  if (!xa_block(a, a.dq, blk, bh, tile, split)) return;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, b = bh / a.nkv, kvh = bh - b * a.nkv;
   const int r = (tile * NS + w) * 32 + (lane & 31);
   const bool mine = r < a.R, live = (tile * NS + w) * 32 < a.R;      // live: the wave has a row (the others only stage)
-  const int len = xa_len(a, b), nt = (len + C::TT - 1) / C::TT, per = (nt + a.splits - 1) / a.splits;
+  const int len = xa_len(a, b), nt = (len + C::TT - 1) / C::TT, per = (nt + a.dq.splits - 1) / a.dq.splits;
   const int t0 = split * per, t1 = min(nt, t0 + per);
   const uint64_t seed = DROP ? a.seed_imm + (a.seed_ptr ? *a.seed_ptr : 0ull) : 0ull;
   uint32_t hq = 0;
@@ -446,7 +490,6 @@ __global__ __launch_bounds__(NS * 64) void xattn_dq_kernel(XaArgs a) {
   if (mine) {
     lse = a.lse[(size_t)bh * a.R + r];
     if (lse == -INFINITY) lse = INFINITY;                          // a row without any key: p = 0
-    if (split == 0 && lane < 32) a.delta[(size_t)bh * a.R + r] = delta;
   }
   const float nlse = -lse;
   f32x16 dq[C::DB];
@@ -466,8 +509,8 @@ __global__ __launch_bounds__(NS * 64) void xattn_dq_kernel(XaArgs a) {
     }
   };
   auto put = [&](int tt, int buf) __attribute__((always_inline)) {
-    st.store(lk[buf], lv[buf], tt, kmask);
-    if (t < C::TT) { lb[buf][t] = bias; if (DROP) lh[buf][t] = hash; }
+    st.store(sh.x[buf], sh.y[buf], tt, kmask);
+    if (t < C::TT) { sh.s[buf][t] = bias; if (DROP) sh.h[buf][t] = hash; }
   };
   if (t0 < t1) { fetch(t0); put(t0, 0); }
   __syncthreads();
@@ -478,15 +521,15 @@ __global__ __launch_bounds__(NS * 64) void xattn_dq_kernel(XaArgs a) {
 #pragma unroll
     for (int n = 0; n < C::NB; ++n) {
       if (!live || tt * C::TT + n * 32 >= len) break;
-      const f32x16 s = M::rows(lk[buf], n, q, lane);
-      const f32x16 dp = M::rows(lv[buf], n, go, lane);
+      const f32x16 s = M::rows(sh.x[buf], n, q, lane);
+      const f32x16 dp = M::rows(sh.y[buf], n, go, lane);
       float ds[16];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         f32x4 bv = {nlse, nlse, nlse, nlse};
         uint4 hk = {0, 0, 0, 0};
-        if (masked) bv += *reinterpret_cast<const f32x4*>(&lb[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
-        if (DROP) hk = *reinterpret_cast<const uint4*>(&lh[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+        if (masked) bv += *reinterpret_cast<const f32x4*>(&sh.s[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+        if (DROP) hk = *reinterpret_cast<const uint4*>(&sh.h[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
         const uint32_t hh[4] = {hk.x, hk.y, hk.z, hk.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -495,39 +538,36 @@ __global__ __launch_bounds__(NS * 64) void xattn_dq_kernel(XaArgs a) {
           ds[4 * k + e] = p * (d - delta);
         }
       }
-      M::cols(lk[buf], n, ds, dq, lane);
+      M::cols(sh.x[buf], n, ds, dq, lane);
     }
     if (tt + 1 < t1) put(tt + 1, buf ^ 1);
     __syncthreads();
     buf ^= 1;
   }
   if (!mine) return;
-  if (a.splits == 1) {
+  if (a.dq.splits == 1) {
     int i, g;
     xa_split(a, r, i, g);
-    xa_put_row<T, C::DB>(a.dq.p + b * a.dq.sb + (long long)i * a.dq.sl + (long long)(kvh * a.G + g) * a.dq.sh, dq, a.scale, lane);
+    xa_put_row<T, C::DB>(a.gq.p + b * a.gq.sb + (long long)i * a.gq.sl + (long long)(kvh * a.G + g) * a.gq.sh, dq, a.scale, lane);
   } else {
-    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.part + (((size_t)split * a.BH + bh) * a.R + r) * D), dq, a.scale, lane);
+    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.dq.part + (((size_t)split * a.BH + bh) * a.R + r) * D), dq, a.scale, lane);
   }
 }
 
 // dK, dV (owned keys, streamed packed query rows):  dv = p^T dout,  dk = scale dx^T q
 template <typename T, int D, int NS, bool DROP>
-__global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
+__device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DROP>& sh) {
   typedef XaCfg<T, D> C;
   typedef XaMma<T, D> M;
-  __shared__ __attribute__((aligned(16))) char lq[2][C::TT * C::RB], lg[2][C::TT * C::RB];
-  __shared__ __attribute__((aligned(16))) float ls[2][C::TT], ld[2][C::TT];
-  __shared__ __attribute__((aligned(16))) uint32_t lh[2][DROP ? C::TT : 4];
   int bh, tile, split;
-  if (!xa_block(a, bh, tile, split)) return;
+  if (!xa_block(a, a.dkv, blk, bh, tile, split)) return;
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, b = bh / a.nkv, kvh = bh - b * a.nkv;
   const int key = (tile * NS + w) * 32 + (lane & 31);
   const int len = xa_len(a, b);
   const float bias = xa_key_bias(a, b, key, len);
   const bool part = bias != -INFINITY, live = (tile * NS + w) * 32 < len;      // live: the wave has a key
   const int nt = tile * NS * 32 < len ? (a.R + C::TT - 1) / C::TT : 0;          // a tile behind the length: zeros
-  const int per = (nt + a.splits - 1) / a.splits;
+  const int per = (nt + a.dkv.splits - 1) / a.dkv.splits;
   const int t0 = split * per, t1 = min(nt, t0 + per);
   const uint64_t seed = DROP ? a.seed_imm + (a.seed_ptr ? *a.seed_ptr : 0ull) : 0ull;
   const uint32_t hk = DROP ? attn_line_hash(seed, bh, key, UC2_ATTN_SALT_K) : 0u;
@@ -542,23 +582,26 @@ __global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
     for (int e = 0; e < 16; ++e) { dk[db][e] = 0.f; dv[db][e] = 0.f; }
   XaStage<T, D, NS * 64, true> st;
   st.init(a, a.q, a.dout, b, kvh, a.R, t);
-  float lse = 0.f, delta = 0.f; uint32_t hash = 0;
+  XaDelta<T, D, NS * 64> dl8;
+  dl8.init(a, b, kvh, t);
+  float lse = 0.f; uint32_t hash = 0;
   auto fetch = [&](int tt) __attribute__((always_inline)) {
     st.load(a, a.q, a.dout, tt);
+    dl8.load(a, tt);
     if (t < C::TT) {
       const int r = tt * C::TT + t;
-      lse = INFINITY; delta = 0.f;                                 // behind the last row, and rows without any key: p = 0
+      lse = INFINITY;                                              // behind the last row, and rows without any key: p = 0
       if (r < a.R) {
         lse = a.lse[(size_t)bh * a.R + r];
         if (lse == -INFINITY) lse = INFINITY;
-        delta = a.delta[(size_t)bh * a.R + r];
         if (DROP) { int i, g; xa_split(a, r, i, g); hash = attn_line_hash(seed, b * a.nh + kvh * a.G + g, i, UC2_ATTN_SALT_Q); }
       }
     }
   };
   auto put = [&](int tt, int buf) __attribute__((always_inline)) {
-    st.store(lq[buf], lg[buf], tt, nullptr);
-    if (t < C::TT) { ls[buf][t] = -lse; ld[buf][t] = delta; if (DROP) lh[buf][t] = hash; }
+    st.store(sh.x[buf], sh.y[buf], tt, nullptr);
+    dl8.store(a, st.y, sh.d[buf], tt);
+    if (t < C::TT) { sh.s[buf][t] = -lse; if (DROP) sh.h[buf][t] = hash; }
   };
   if (t0 < t1) { fetch(t0); put(t0, 0); }
   __syncthreads();
@@ -568,17 +611,17 @@ __global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
 #pragma unroll
     for (int n = 0; n < C::NB; ++n) {
       if (!live || tt * C::TT + n * 32 >= a.R) break;
-      const f32x16 s = M::rows(lq[buf], n, kf, lane);
-      const f32x16 dp = M::rows(lg[buf], n, vf, lane);
+      const f32x16 s = M::rows(sh.x[buf], n, kf, lane);
+      const f32x16 dp = M::rows(sh.y[buf], n, vf, lane);
       float p[16], ds[16];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int at = n * 32 + 8 * k + 4 * (lane >> 5);
-        f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[buf][at]);
-        const f32x4 dl = *reinterpret_cast<const f32x4*>(&ld[buf][at]);
+        f32x4 lv = *reinterpret_cast<const f32x4*>(&sh.s[buf][at]);
+        const f32x4 dl = *reinterpret_cast<const f32x4*>(&sh.d[buf][at]);
         if (a.kmask) lv += f32x4{bias, bias, bias, bias};
         uint4 hv = {0, 0, 0, 0};
-        if (DROP) hv = *reinterpret_cast<const uint4*>(&lh[buf][at]);
+        if (DROP) hv = *reinterpret_cast<const uint4*>(&sh.h[buf][at]);
         const uint32_t hh[4] = {hv.x, hv.y, hv.z, hv.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -589,8 +632,8 @@ __global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
           ds[4 * k + e] = x * (d - dl[e]);
         }
       }
-      M::cols(lg[buf], n, p, dv, lane);
-      M::cols(lq[buf], n, ds, dk, lane);
+      M::cols(sh.y[buf], n, p, dv, lane);
+      M::cols(sh.x[buf], n, ds, dk, lane);
     }
     if (tt + 1 < t1) put(tt + 1, buf ^ 1);
     __syncthreads();
@@ -603,39 +646,53 @@ __global__ __launch_bounds__(NS * 64) void xattn_dkv_kernel(XaArgs a) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) { dk[db][e] = 0.f; dv[db][e] = 0.f; }
   }
-  if (a.splits == 1) {
-    xa_put_row<T, C::DB>(a.dk.p + b * a.dk.sb + (long long)key * a.dk.sl + kvh * a.dk.sh, dk, a.scale, lane);
-    xa_put_row<T, C::DB>(a.dv.p + b * a.dv.sb + (long long)key * a.dv.sl + kvh * a.dv.sh, dv, 1.0f, lane);
+  if (a.dkv.splits == 1) {
+    xa_put_row<T, C::DB>(a.gk.p + b * a.gk.sb + (long long)key * a.gk.sl + kvh * a.gk.sh, dk, a.scale, lane);
+    xa_put_row<T, C::DB>(a.gv.p + b * a.gv.sb + (long long)key * a.gv.sl + kvh * a.gv.sh, dv, 1.0f, lane);
   } else {
     const size_t n = (size_t)a.BH * a.Lk, row = (size_t)bh * a.Lk + key;
-    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.part + (split * 2 * n + row) * D), dk, a.scale, lane);
-    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.part + ((split * 2 + 1) * n + row) * D), dv, 1.0f, lane);
+    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.dkv.part + (split * 2 * n + row) * D), dk, a.scale, lane);
+    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.dkv.part + ((split * 2 + 1) * n + row) * D), dv, 1.0f, lane);
   }
 }
 
-// sum of the splits' gradients in split order.  which: 0 = dQ (packed rows), 1 = dK and dV
+template <typename T, int D, int NS, bool DROP>
+__global__ __launch_bounds__(NS * 64) void xattn_bwd_kernel(XaArgs a) {
+  __shared__ XaLds<T, D, DROP> sh;
+  if ((int)blockIdx.x < a.dkv.blocks) xa_dkv<T, D, NS, DROP>(a, blockIdx.x, sh);
+  else xa_dq<T, D, NS, DROP>(a, blockIdx.x - a.dkv.blocks, sh);
+}
+
+// sums of the splits' gradients in split order: dK and dV, then dQ, where they were split
 template <typename T, int D>
-__global__ __launch_bounds__(256) void xattn_sum_kernel(XaArgs a, int which, int len) {
-  const long long rows = (long long)a.BH * len, all = rows * (which ? 2 : 1);
-  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x, row = idx / (D / 4);
-  if (row >= all) return;
+__global__ __launch_bounds__(256) void xattn_sum_kernel(XaArgs a) {
+  const long long rk = a.dkv.splits > 1 ? (long long)a.BH * a.Lk : 0, rq = a.dq.splits > 1 ? (long long)a.BH * a.R : 0;
+  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
+  long long row = idx / (D / 4);
+  if (row >= 2 * rk + rq) return;
   const int c = (int)(idx - row * (D / 4)) * 4;
+  const bool isq = row >= 2 * rk;
+  if (isq) row -= 2 * rk;
+  const XaSide& side = isq ? a.dq : a.dkv;
+  const long long all = isq ? rq : 2 * rk;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < a.splits; ++k) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + ((size_t)k * all + row) * D + c);
+#pragma unroll 4
+  for (int k = 0; k < side.splits; ++k) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(side.part + ((size_t)k * all + row) * D + c);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] += v[e];
   }
-  const long long lr = row >= rows ? row - rows : row;
+  const int len = isq ? a.R : a.Lk;
+  const long long lr = !isq && row >= rk ? row - rk : row;
   const int bh = (int)(lr / len), r = (int)(lr - (long long)bh * len), b = bh / a.nkv, kvh = bh - b * a.nkv;
   char* p;
-  if (which) {
-    const XaOut& x = row >= rows ? a.dv : a.dk;
-    p = x.p + b * x.sb + (long long)r * x.sl + kvh * x.sh;
-  } else {
+  if (isq) {
     int i, g;
     xa_split(a, r, i, g);
-    p = a.dq.p + b * a.dq.sb + (long long)i * a.dq.sl + (long long)(kvh * a.G + g) * a.dq.sh;
+    p = a.gq.p + b * a.gq.sb + (long long)i * a.gq.sl + (long long)(kvh * a.G + g) * a.gq.sh;
+  } else {
+    const XaOut& x = row >= rk ? a.gv : a.gk;
+    p = x.p + b * x.sb + (long long)r * x.sl + kvh * x.sh;
   }
   xa_put4(reinterpret_cast<T*>(p) + c, s[0], s[1], s[2], s[3]);
 }
@@ -646,8 +703,8 @@ static int xa_tt(int dtype, int D) { return D * (dtype ? 2 : 4) <= 128 ? 64 : 32
 // vectors of 128, whose staging by one wave alone spills
 static int xa_ns(int dtype, int D, int cols) { return cols <= 32 && !(dtype == 0 && D == 128) ? 1 : cols <= 64 ? 2 : 4; }
 // splits of the streamed axis: until the launch has about 2048 waves (8 per CU), each split at least two tiles
-static int xa_splits(const Uc2CrossAttn* p, int cols, int streamed) {
-  const int ns = xa_ns(p->dtype, p->D, cols), tt = xa_tt(p->dtype, p->D);
+static int xa_splits(const Uc2CrossAttn* p, int ns, int cols, int streamed) {
+  const int tt = xa_tt(p->dtype, p->D);
   const long long bh = (long long)p->B * p->nkv;
   const long long waves = bh * ((cols + 32 * ns - 1) / (32 * ns)) * ns, nt = (streamed + tt - 1) / tt;
   long long s = waves > 0 ? 2048 / waves : 1;
@@ -655,17 +712,19 @@ static int xa_splits(const Uc2CrossAttn* p, int cols, int streamed) {
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 static size_t xa_up(size_t n) { return (n + 255) & ~(size_t)255; }
-struct XaPlan { int s_fwd, s_dq, s_dkv; size_t fwd, part_dq, part_dkv, delta, bwd; };
+struct XaPlan { int ns_bwd, s_fwd, s_dq, s_dkv; size_t fwd, part_dkv, bwd; };
 static XaPlan xa_plan(const Uc2CrossAttn* p) {
   XaPlan r{};
   const long long bh = (long long)p->B * p->nkv, R = (long long)p->Lq * (p->nh / p->nkv);
-  r.s_fwd = r.s_dq = xa_splits(p, (int)R, p->Lk);
-  r.s_dkv = xa_splits(p, p->Lk, (int)R);
+  r.s_fwd = xa_splits(p, xa_ns(p->dtype, p->D, (int)R), (int)R, p->Lk);
   if (r.s_fwd > 1) r.fwd = xa_up((size_t)r.s_fwd * bh * R * p->D * 4) + xa_up((size_t)r.s_fwd * bh * R * 8);
-  r.delta = xa_up((size_t)bh * R * 4);
-  r.part_dq = r.s_dq > 1 ? (size_t)r.s_dq * bh * R * p->D * 4 : 0;
-  r.part_dkv = r.s_dkv > 1 ? (size_t)r.s_dkv * 2 * bh * p->Lk * p->D * 4 : 0;
-  r.bwd = r.delta + xa_up(r.part_dq > r.part_dkv ? r.part_dq : r.part_dkv);     // the two kernels follow one another: one area
+  const int nq = xa_ns(p->dtype, p->D, (int)R), nk = xa_ns(p->dtype, p->D, p->Lk);
+  r.ns_bwd = nq > nk ? nq : nk;                                   // one launch: one size of workgroup
+  if (p->dtype == 0 && p->D == 128) r.ns_bwd = 4;                 // (staging of three tensors by two waves spills)
+  r.s_dq = xa_splits(p, r.ns_bwd, (int)R, p->Lk);
+  r.s_dkv = xa_splits(p, r.ns_bwd, p->Lk, (int)R);
+  r.part_dkv = r.s_dkv > 1 ? xa_up((size_t)r.s_dkv * 2 * bh * p->Lk * p->D * 4) : 0;
+  r.bwd = r.part_dkv + (r.s_dq > 1 ? (size_t)r.s_dq * bh * R * p->D * 4 : 0);
   return r;
 }
 static bool xa_str_ok(long long sb, long long sl, long long sh, int el) {      // 16-byte rows
@@ -713,10 +772,12 @@ static XaArgs xa_args(const Uc2CrossAttn* p) {
   a.thresh = drop_thresh(p->drop_p); a.keep_scale = 1.0f / (1.0f - p->drop_p); a.seed_ptr = p->seed; a.seed_imm = p->site;
   return a;
 }
-static int xa_grid(XaArgs& a, int cols, int ns) {                  // blocks, or 0 where they pass a launch's limit
-  a.tiles = (cols + 32 * ns - 1) / (32 * ns);
-  const long long n = (long long)(a.BH >= 8 ? (a.BH + 7) / 8 * 8 : a.BH) * a.tiles * a.splits;
-  return n < (1ll << 31) ? (int)n : 0;
+static bool xa_side(const XaArgs& a, XaSide& side, int cols, int ns, int splits) {      // false: more blocks than a launch takes
+  side.tiles = (cols + 32 * ns - 1) / (32 * ns);
+  side.splits = splits;
+  const long long n = (long long)(a.BH >= 8 ? (a.BH + 7) / 8 * 8 : a.BH) * side.tiles * splits;
+  side.blocks = (int)n;
+  return n < (1ll << 30);
 }
 #define XA_LAUNCH(KERN, TT_, DD_, NN_, grid)                                                                                        \
   do {                                                                                                                              \
@@ -749,18 +810,18 @@ extern "C" int uc2_xattn_fwd(const Uc2CrossAttn* attn, void* ws, size_t ws_bytes
   UC2_CHECK_ARG(pl.fwd == 0 || (ws && ws_bytes >= pl.fwd && ((uintptr_t)ws & 15) == 0));
   hipStream_t st = (hipStream_t)stream;
   XaArgs a = xa_args(p);
-  a.splits = pl.s_fwd;
-  if (a.splits > 1) {
-    a.part = (float*)ws;
-    a.pml = (float*)((char*)ws + xa_up((size_t)a.splits * a.BH * a.R * p->D * 4));
+  const int ns = xa_ns(p->dtype, p->D, a.R);
+  UC2_CHECK_ARG(xa_side(a, a.fwd, a.R, ns, pl.s_fwd));
+  if (pl.s_fwd > 1) {
+    a.fwd.part = (float*)ws;
+    a.pml = (float*)((char*)ws + xa_up((size_t)pl.s_fwd * a.BH * a.R * p->D * 4));
   }
-  const int ns = xa_ns(p->dtype, p->D, a.R), grid = xa_grid(a, a.R, ns);
-  UC2_CHECK_ARG(grid > 0);
+  const int grid = a.fwd.blocks;
 #define XA_GO(T_, D_) XA_NS(xattn_fwd_kernel, T_, D_)
   XA_TD(XA_GO);
 #undef XA_GO
   UC2_LAUNCH_CHECK();
-  if (a.splits > 1) {
+  if (pl.s_fwd > 1) {
     const long long blocks = ((long long)a.BH * a.R + 3) / 4;
     UC2_CHECK_ARG(blocks < (1ll << 31));
 #define XA_GO(T_, D_) hipLaunchKernelGGL((xattn_join_kernel<T_, D_>), dim3((unsigned)blocks), dim3(256), 0, st, a)
@@ -791,44 +852,26 @@ extern "C" int uc2_xattn_bwd(const Uc2CrossAttn* attn, const Uc2CrossAttnGrad* g
   hipStream_t st = (hipStream_t)stream;
   XaArgs a = xa_args(p);
   a.dout = {(const char*)g->dout, g->dout_sb * el, g->dout_sl * el, g->dout_sh * el};
-  a.dq = {(char*)g->dq, g->dq_sb * el, g->dq_sl * el, g->dq_sh * el};
-  a.dk = {(char*)g->dk, g->dk_sb * el, g->dk_sl * el, g->dk_sh * el};
-  a.dv = {(char*)g->dv, g->dv_sb * el, g->dv_sl * el, g->dv_sh * el};
-  a.delta = (float*)ws;
-  a.part = (float*)((char*)ws + pl.delta);
-  if (p->Lq > 0) {
-    a.splits = pl.s_dq;
-    const int ns = xa_ns(p->dtype, p->D, a.R), grid = xa_grid(a, a.R, ns);
-    UC2_CHECK_ARG(grid > 0);
-#define XA_GO(T_, D_) XA_NS(xattn_dq_kernel, T_, D_)
+  a.gq = {(char*)g->dq, g->dq_sb * el, g->dq_sl * el, g->dq_sh * el};
+  a.gk = {(char*)g->dk, g->dk_sb * el, g->dk_sl * el, g->dk_sh * el};
+  a.gv = {(char*)g->dv, g->dv_sb * el, g->dv_sl * el, g->dv_sh * el};
+  const int ns = pl.ns_bwd;
+  UC2_CHECK_ARG(xa_side(a, a.dkv, a.Lk, ns, pl.s_dkv) && xa_side(a, a.dq, a.R, ns, pl.s_dq));
+  a.dkv.part = (float*)ws;
+  a.dq.part = (float*)((char*)ws + pl.part_dkv);
+  const int grid = a.dkv.blocks + a.dq.blocks;
+  if (grid == 0) return 0;                                        // (neither queries nor keys)
+#define XA_GO(T_, D_) XA_NS(xattn_bwd_kernel, T_, D_)
+  XA_TD(XA_GO);
+#undef XA_GO
+  UC2_LAUNCH_CHECK();
+  const long long rows = (pl.s_dkv > 1 ? 2ll * a.BH * a.Lk : 0) + (pl.s_dq > 1 ? (long long)a.BH * a.R : 0), blocks = (rows * (p->D / 4) + 255) / 256;
+  UC2_CHECK_ARG(blocks < (1ll << 31));
+  if (blocks > 0) {
+#define XA_GO(T_, D_) hipLaunchKernelGGL((xattn_sum_kernel<T_, D_>), dim3((unsigned)blocks), dim3(256), 0, st, a)
     XA_TD(XA_GO);
 #undef XA_GO
     UC2_LAUNCH_CHECK();
-    if (a.splits > 1) {
-      const long long blocks = ((long long)a.BH * a.R * (p->D / 4) + 255) / 256;
-      UC2_CHECK_ARG(blocks < (1ll << 31));
-#define XA_GO(T_, D_) hipLaunchKernelGGL((xattn_sum_kernel<T_, D_>), dim3((unsigned)blocks), dim3(256), 0, st, a, 0, a.R)
-      XA_TD(XA_GO);
-#undef XA_GO
-      UC2_LAUNCH_CHECK();
-    }
-  }
-  if (p->Lk > 0) {
-    a.splits = pl.s_dkv;
-    const int ns = xa_ns(p->dtype, p->D, a.Lk), grid = xa_grid(a, a.Lk, ns);
-    UC2_CHECK_ARG(grid > 0);
-#define XA_GO(T_, D_) XA_NS(xattn_dkv_kernel, T_, D_)
-    XA_TD(XA_GO);
-#undef XA_GO
-    UC2_LAUNCH_CHECK();
-    if (a.splits > 1) {
-      const long long blocks = (2ll * a.BH * a.Lk * (p->D / 4) + 255) / 256;
-      UC2_CHECK_ARG(blocks < (1ll << 31));
-#define XA_GO(T_, D_) hipLaunchKernelGGL((xattn_sum_kernel<T_, D_>), dim3((unsigned)blocks), dim3(256), 0, st, a, 1, a.Lk)
-      XA_TD(XA_GO);
-#undef XA_GO
-      UC2_LAUNCH_CHECK();
-    }
   }
   return 0;
 }
