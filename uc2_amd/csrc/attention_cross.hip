@@ -416,27 +416,40 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
   }
 }
 
-// joins the splits of the forward (64 at most): a wave per row; lane s first holds split s's factor, then every lane sums its elements over the splits
-template <typename T, int D>
+// joins the splits of the forward (64 at most): W waves per row; lane s of each first holds split s's factor, then the waves share the splits, a lane
+// summing its elements, and are added in wave order (one wave for 32 splits of 256 rows took 11 us: four trips to memory one after the other)
+template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a) {
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (long long)a.BH * a.R;
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 63, bh = (int)(row / a.R), r = (int)(row - (long long)bh * a.R);
+  constexpr int E = D / 64 > 0 ? D / 64 : 1;
+  __shared__ float red[W > 1 ? W * 64 * E : 1];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, w = W > 1 ? wv : 0;
+  const long long row = W > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * 4 + wv, rows = (long long)a.BH * a.R;
+  if (row >= rows) return;                                        // (W > 1: uniform)
+  const int bh = (int)(row / a.R), r = (int)(row - (long long)bh * a.R);
   float m = -INFINITY, l = 0.f;
   if (lane < a.fwd.splits) { const float2 v = *reinterpret_cast<const float2*>(a.pml + 2 * (lane * rows + row)); m = v.x; l = v.y; }
-  const float top = wave_max(m), mu = top == -INFINITY ? 0.f : top;
-  const float f = __builtin_amdgcn_exp2f(m - mu);
-  l = wave_sum(f * l);
-  constexpr int E = D / 64 > 0 ? D / 64 : 1;
   float o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
+  const float top = wave_max(m), mu = top == -INFINITY ? 0.f : top;
+  const float f = __builtin_amdgcn_exp2f(m - mu);
+  l = wave_sum(f * l);
   const float* p = a.fwd.part + row * D + (D >= 64 ? lane : lane % D);
 #pragma unroll 8
-  for (int s = 0; s < a.fwd.splits; ++s) {
-    const float w = __shfl(f, s);
+  for (int s = w; s < a.fwd.splits; s += W) {
+    const float x = __shfl(f, s);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(w, p[s * rows * D + 64 * e], o[e]);
+    for (int e = 0; e < E; ++e) o[e] = fmaf(x, p[s * rows * D + 64 * e], o[e]);
+  }
+  if (W > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) red[(w * E + e) * 64 + lane] = o[e];
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int k = 1; k < W; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += red[(k * E + e) * 64 + lane];
   }
   const float inv = l > 0.f ? 1.0f / l : (l == l ? 0.f : l);
   const int b = bh / a.nkv, kvh = bh - b * a.nkv;
@@ -822,9 +835,13 @@ extern "C" int uc2_xattn_fwd(const Uc2CrossAttn* attn, void* ws, size_t ws_bytes
 #undef XA_GO
   UC2_LAUNCH_CHECK();
   if (pl.s_fwd > 1) {
-    const long long blocks = ((long long)a.BH * a.R + 3) / 4;
+    // four waves per row from 8 splits on
+    const bool wide = pl.s_fwd >= 8;
+    const long long rows = (long long)a.BH * a.R, blocks = wide ? rows : (rows + 3) / 4;
     UC2_CHECK_ARG(blocks < (1ll << 31));
-#define XA_GO(T_, D_) hipLaunchKernelGGL((xattn_join_kernel<T_, D_>), dim3((unsigned)blocks), dim3(256), 0, st, a)
+#define XA_GO(T_, D_)                                                                                                               \
+  if (wide) hipLaunchKernelGGL((xattn_join_kernel<T_, D_, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a);                         \
+  else hipLaunchKernelGGL((xattn_join_kernel<T_, D_, 1>), dim3((unsigned)blocks), dim3(256), 0, st, a)
     XA_TD(XA_GO);
 #undef XA_GO
     UC2_LAUNCH_CHECK();
