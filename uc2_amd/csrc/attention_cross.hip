@@ -715,12 +715,14 @@ static int xa_tt(int dtype, int D) { return D * (dtype ? 2 : 4) <= 128 ? 64 : 32
 // waves of a workgroup: as many 32-column waves as there are columns, up to 4 (they share the streamed tile); two at least for fp32
 // vectors of 128, whose staging by one wave alone spills
 static int xa_ns(int dtype, int D, int cols) { return cols <= 32 && !(dtype == 0 && D == 128) ? 1 : cols <= 64 ? 2 : 4; }
-// splits of the streamed axis: until the launch has about 2048 waves (8 per CU), each split at least two tiles
+// splits of the streamed axis, each two tiles at least: until the launch has 1024 waves, one per SIMD (4 x 512 x 512, 12 heads, forward and backward 40 us;
+// up to 2048: 63 us, for the partials and their sum); workgroups of one wave, whose tiles wait for memory alone, to 2048 (16 x 1 x 16384: 32 us
+// against 35)
 static int xa_splits(const Uc2CrossAttn* p, int ns, int cols, int streamed) {
   const int tt = xa_tt(p->dtype, p->D);
   const long long bh = (long long)p->B * p->nkv;
   const long long waves = bh * ((cols + 32 * ns - 1) / (32 * ns)) * ns, nt = (streamed + tt - 1) / tt;
-  long long s = waves > 0 ? 2048 / waves : 1;
+  long long s = waves > 0 ? (ns > 1 ? 1024 : 2048) / waves : 1;
   if (s > nt / 2) s = nt / 2;
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
