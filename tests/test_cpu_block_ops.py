@@ -42,10 +42,11 @@ def test_cross_attention_argument_errors(bad):
 def test_cross_attention_backward_argument_errors():
     lib = _lib.load()
     g = dict(dout=P, dout_sb=768, dout_sl=256, dout_sh=64, dq=P, dk=P, dv=P, dq_sb=768, dq_sl=256, dq_sh=64, dk_sb=640, dk_sl=128, dk_sh=64, dv_sb=640, dv_sl=128, dv_sh=64)
-    need = lib.uc2_xattn_workspace(ctypes.byref(attn()), 1)
-    assert need > 0
-    for a, gb, ws, n in ((attn(lse=0), g, P, need), (attn(), dict(g, dq=0), P, need), (attn(), dict(g, dk=0), P, need), (attn(), dict(g, dout_sl=3), P, need),
-                         (attn(), dict(g, dv=P + 4), P, need), (attn(), g, None, need), (attn(), g, P, need - 1), (attn(), g, P + 4, need)):
+    many = lambda **kw: attn(Lk=5000, **kw)  # noqa: E731          (its keys are split: it needs a workspace)
+    need = lib.uc2_xattn_workspace(ctypes.byref(many()), 1)
+    assert need > 0 and lib.uc2_xattn_workspace(ctypes.byref(attn()), 1) == 0
+    for a, gb, ws, n in ((many(lse=0), g, P, need), (many(), dict(g, dq=0), P, need), (many(), dict(g, dk=0), P, need), (many(), dict(g, dout_sl=3), P, need),
+                         (many(), dict(g, dv=P + 4), P, need), (many(), g, None, need), (many(), g, P, need - 1), (many(), g, P + 4, need), (attn(lse=0), g, None, 0)):
         assert lib.uc2_xattn_bwd(ctypes.byref(a), ctypes.byref(_CrossAttnGrad(**gb)), ws, n, None) == -1
     assert lib.uc2_xattn_bwd(ctypes.byref(attn()), None, P, need, None) == -1
     assert lib.uc2_xattn_fwd(None, None, 0, None) == -1
@@ -97,6 +98,53 @@ def test_rms_argument_errors():
         a[i] = bad
         assert lib.uc2_rms_bwd(*a) == -1, (i, bad)
     assert lib.uc2_rms_bwd_workspace(0, 128) == 0 and lib.uc2_rms_bwd_workspace(4, 20000) == 0
+
+
+def test_linear_wgrad_argument_errors():
+    lib = _lib.load()
+    n = lib.uc2_linear_wgrad_workspace(4000, 40, 72)
+    assert n > 0 and lib.uc2_linear_wgrad_workspace(200, 40, 72) == 0             # (few rows are not split)
+    ok = [4000, 40, 72, P, 40, P, 72, P, 72, P, P, n, None]
+    for i, bad in ((0, 0), (0, -1), (1, 0), (2, 0), (3, None), (3, P + 1), (4, 39), (5, None), (5, P + 1), (6, 71), (7, None), (7, P + 2), (8, 71), (9, P + 2), (10, None), (10, P + 8),
+                   (11, n - 1)):
+        a = list(ok)
+        a[i] = bad
+        assert lib.uc2_linear_wgrad(*a) == -1, (i, bad)
+    assert lib.uc2_linear_wgrad_workspace(0, 40, 72) == 0 and lib.uc2_linear_wgrad_workspace(4000, 1 << 30, 1 << 30) == 0
+
+
+def test_a_leaf_remembers_the_stream_of_its_first_graph(monkeypatch):
+    """note_leaves and refuse_foreign_capture on the streams and captures they are told of"""
+    from uc2_amd.ops.base import note_leaves, once
+    now = [1, False]
+    monkeypatch.setattr(_lib, "stream", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[1])
+
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, y):
+            note_leaves(ctx)
+            return x + 2 * y
+
+        @staticmethod
+        @once
+        def backward(ctx, d):
+            return d, 2 * d
+    x, y = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+    eager = Twice.apply(x, y)
+    now[:] = [7, True]
+    with pytest.raises(_lib.Uc2Error, match="eager graph"):
+        Twice.apply(x, x.detach().clone()).sum().backward()
+    with pytest.raises(_lib.Uc2Error, match="eager graph"):
+        torch.autograd.grad(Twice.apply(torch.ones(3), y).sum(), [y])
+    Twice.apply(x.detach().requires_grad_(), x.detach()).sum().backward()
+    now[1] = False
+    Twice.apply(x, y).sum().backward()                     # eager on another stream: torch joins the streams
+    del eager
+    now[1] = True
+    x.grad = y.grad = None
+    Twice.apply(x, y).sum().backward()                     # a graph of its own
+    assert bool((x.grad == 1).all()) and bool((y.grad == 2).all())
 
 
 def test_cpu_tensors_are_refused():

@@ -152,6 +152,41 @@ def test_linear_block_forward_and_gradients(M, N, K, wtype):
     R.assert_within(db, dy.double().sum(0), M * R.U[F32] * dy.double().abs().sum(0) + 1e-30, "db")
 
 
+def wgrad(M, N, K, dy, x, bias=True, lddw=None):
+    """uc2_linear_wgrad on rows dy [M, N] and x [M, K] of any stride -> (dw [N, K], db)"""
+    lddw = lddw or K
+    dw = torch.full((N, lddw), 7.0, device=DEV)
+    db = torch.empty(N, device=DEV) if bias else None
+    n = _lib.load().uc2_linear_wgrad_workspace(M, N, K)
+    ws = torch.empty(n, dtype=torch.uint8, device=DEV)
+    _lib.call("uc2_linear_wgrad", M, N, K, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), dw.data_ptr(), lddw, _lib.ptr(db), ws.data_ptr(), n, _lib.stream())
+    assert bool((dw[:, K:] == 7).all())
+    return dw[:, :K], db
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 8, 8), (2, 7, 300), (65, 300, 3), (513, 1, 1000), (700, 9, 130), (4097, 257, 100), (5000, 5, 6), (1024, 256, 256), (1280, 512, 256),
+                                   (1152, 256, 512), (40000, 64, 40)])
+@pytest.mark.parametrize("odd", [False, True])
+def test_linear_wgrad(M, N, K, odd):
+    """odd: rows of an odd stride behind an odd offset, dw in wider rows.  Bound as above: M fp32 additions"""
+    dy, x = normal((M, N + 3 * odd), 1, BF16)[:, odd:N + odd], normal((M, K + 5 * odd), 2, BF16)[:, 3 * odd:K + 3 * odd]
+    dw, db = wgrad(M, N, K, dy, x, True, K + odd)
+    want, mag = R.mm(dy.double().t(), x.double()), R.mm(dy.double().abs().t(), x.double().abs())
+    R.assert_within(dw, want, 2 * M * R.U[F32] * mag + 1e-30, "dw")
+    R.assert_within(db, dy.double().sum(0), M * R.U[F32] * dy.double().abs().sum(0) + 1e-30, "db")
+    again, db2 = wgrad(M, N, K, dy, x)
+    assert torch.equal(again, dw) and torch.equal(db2, db)
+    assert torch.equal(wgrad(M, N, K, dy, x, False)[0], dw)
+
+
+def test_linear_wgrad_nan_stays_in_its_row_and_column():
+    dy, x = normal((1500, 40), 1, BF16), normal((1500, 72), 2, BF16)
+    dy[700, 3] = math.nan
+    dw, db = wgrad(1500, 40, 72, dy, x)
+    bad = torch.isnan(dw)
+    assert bool(bad[3].all()) and int(bad.sum()) == 72 and bool(torch.isnan(db)[3]) and int(torch.isnan(db).sum()) == 1
+
+
 def test_linear_block_leading_dimensions_and_partial_gradients():
     x, w = normal((3, 5, 256), 1, BF16), normal((130, 256), 2)
     y = ops.linear_fp8_block(x, w)
@@ -574,6 +609,83 @@ def test_operators_in_a_graph():
         g1.replay(), g2.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(o1, step())) and all(torch.equal(a, b) for a, b in zip(o2, train()))
+
+
+def test_training_in_a_graph():
+    """forward and backward of the sublayer's three operators captured together, gradients into .grad; replayed on new inputs with eager work between"""
+    B, Lq, Lk, H, nh, nkv, D = 2, 9, 1500, 96, 4, 2, 32
+    x, enc, dy = normal((B, Lq, H), 1, BF16), normal((B, Lk, H), 2, BF16), normal((B, Lq, H), 3, BF16)
+    mask = torch.zeros(B, 1, 1, Lk, device=DEV)
+    P = [1 + normal((H,), 4, F32, 0.1), normal((nh * D, H), 5, F32, 0.2), normal((2 * nkv * D, H), 6, F32, 0.1), normal((H, nh * D), 7, F32, 0.1), normal((H,), 8)]
+
+    def step(leaves):
+        gain, wq, wkv, wo, bo = leaves
+        y, s = ops.rms_norm(x, gain, residual=x)
+        kv = ops.linear_fp8_block(enc, wkv).view(B, Lk, 2, nkv, D)
+        o = ops.cross_attention(ops.linear_fp8_block(y, wq).view(B, Lq, nh, D), kv[:, :, 0], kv[:, :, 1], key_mask=mask)
+        out = s + ops.linear_fp8_block(o.view(B, Lq, nh * D), wo, bo)
+        out.backward(dy)
+        return out.detach()
+
+    def eager():
+        leaves = [p.detach().clone().requires_grad_() for p in P]
+        out = step(leaves)
+        return [out] + [p.grad for p in leaves]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        eager()
+    torch.cuda.synchronize()
+    leaves = [p.detach().requires_grad_() for p in P]                                    # no graph of theirs is alive
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(leaves)
+    for i in range(4):
+        x.copy_(normal(x.shape, 10 + i)), dy.copy_(normal(dy.shape, 20 + i)), mask.masked_fill_(torch.rand(mask.shape, generator=gen(i), device=DEV) < 0.1, -1e30)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip([out] + [p.grad for p in leaves], eager()))
+
+
+def test_capture_beside_an_eager_graph_of_the_same_leaves_is_refused(monkeypatch):
+    """(nothing is captured here: the operators are told so on another stream, and refuse before anything is launched)"""
+    q, k, v, _ = attn_inputs(1, 3, 9, 2, 2, 64, BF16)
+    x, xb, w, g = normal((4, 96), 1), normal((4, 96), 1, BF16), normal((8, 96), 2), torch.ones(96, device=DEV)
+    side = torch.cuda.Stream()
+    for f, *leaves in ((ops.cross_attention, q, k, v), (ops.rms_norm, x, g), (ops.linear_fp8_block, xb, w)):
+        leaves = [t.detach().requires_grad_() for t in leaves]
+        eager = f(*leaves)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            out = f(*leaves)
+            own = [t.detach().requires_grad_() for t in leaves]
+            out2 = f(*own)
+            d = torch.ones_like(out)
+            with monkeypatch.context() as m:
+                m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+                with pytest.raises(_lib.Uc2Error, match="eager graph"):
+                    torch.autograd.grad(out, leaves, d)
+                b = torch.autograd.grad(out2, own, d)
+        torch.cuda.synchronize()
+        assert all(torch.equal(s, t) for s, t in zip(b, torch.autograd.grad(eager, leaves, d)))
+
+
+def test_saved_tensors_that_come_back_where_they_were_with_other_strides():
+    buf = normal((2, 9, 3, 4, 64), 1, BF16)
+    q, (_, k, v, dout) = buf[:, :, 0], attn_inputs(2, 9, 70, 4, 2, 64, BF16)[0:4]
+    want = run_attn(q.clone(), k, v, dout)
+
+    def pack(t):
+        return t.clone(memory_format=torch.contiguous_format), t.data_ptr()
+
+    def unpack(p):
+        if p[1] != buf.data_ptr():
+            return p[0]
+        buf.view(-1)[:p[0].numel()].copy_(p[0].view(-1))
+        return buf.view(-1)[:p[0].numel()].view(p[0].shape)
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        qg = q.detach().requires_grad_()
+        o = ops.cross_attention(qg, k, v)
+    assert torch.equal(torch.autograd.grad(o, [qg], dout)[0], want[1])
 
 
 def test_saved_tensors_that_come_back_as_copies():

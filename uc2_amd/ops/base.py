@@ -142,11 +142,32 @@ def device_guard(t):
     return _NO_GUARD if t.get_device() == _cur_device() else torch.cuda.device(t.device)
 
 
+def note_leaves(ctx):
+    """in a forward that will be differentiated, on the device of its tensors: each leaf among the inputs remembers the stream that its gradient's accumulation
+    belongs to, that of the first of its graphs alive"""
+    for node, _ in ctx.next_functions:
+        if type(node).__name__ == "AccumulateGrad":
+            node.metadata.setdefault("uc2_stream", _lib.stream())
+
+
+def refuse_foreign_capture(ctx):
+    """A captured backward pass hands its gradients to the accumulations of its leaves.  While an eager graph of a leaf lives, that accumulation belongs
+    to the eager stream: the capture would reach over to it and end the process, so it is refused before."""
+    here = _lib.stream()
+    for node, _ in ctx.next_functions:
+        if type(node).__name__ == "AccumulateGrad" and node.metadata.get("uc2_stream", here) != here:
+            raise _lib.Uc2Error("a backward pass cannot be captured while an eager graph of the same leaves is alive: delete its outputs first, or capture with "
+                                "leaves of its own (x.detach().requires_grad_())")
+
+
 def once(backward):
-    """once_differentiable (a second differentiation raises) for backward passes that are asked for a graph; without its wrapping, 4 us a call, otherwise"""
+    """once_differentiable (a second differentiation raises) for backward passes that are asked for a graph; without its wrapping, 4 us a call, otherwise.
+    The forward calls note_leaves."""
     guarded = once_differentiable(backward)
 
     def run(ctx, *grads):
+        if torch.cuda.is_current_stream_capturing():
+            refuse_foreign_capture(ctx)
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
 

@@ -10,7 +10,7 @@ import torch
 from .. import _lib
 from .._lib import call, dt, ptr, stream
 from ..config import state
-from .base import _Timed, _require_cuda, device_guard, once
+from .base import _Timed, _require_cuda, device_guard, note_leaves, once
 from .linear import colsum_accum
 
 BLOCK = 128
@@ -135,6 +135,7 @@ class LinearBlockFp8Fn(torch.autograd.Function):
             w, wt = _quant_weight(weight, True) if need_dx else (_quant_weight(weight, False), (None, None))
             a = _quant_rows(x2)
             y = _gemm(a.data, a.scale, w.data, w.scale, bias)
+            note_leaves(ctx)
         ctx.save_for_backward(x2 if need_dw else None, wt[0], wt[1])
         ctx.cfg = (shp, weight.shape, weight.dtype, _lib.load().uc2_linear_wgrad_workspace(x2.shape[0], *weight.shape) if need_dw else 0)
         return y if len(shp) == 2 else y.view(*shp[:-1], weight.shape[0])
@@ -230,6 +231,7 @@ class RMSNormFn(torch.autograd.Function):
         grad = True in ctx.needs_input_grad
         with device_guard(x):
             s, y, rstd, _ = _rms_fwd(x, weight, eps, residual, True, grad, False)
+            note_leaves(ctx)
         if grad:
             ctx.save_for_backward(s, weight.contiguous(), rstd)
             ctx.ws = _lib.load().uc2_rms_bwd_workspace(*s.shape)

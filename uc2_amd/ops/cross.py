@@ -7,7 +7,7 @@ import torch
 from .. import _lib
 from .._lib import check, dt, ptr, stream
 from ..config import state
-from .base import _Timed, _require_cuda, device_guard, once, rng
+from .base import _Timed, _require_cuda, device_guard, note_leaves, once, rng
 
 # Uc2CrossAttn and Uc2CrossAttnGrad (include/uc2_hip.h), packed in native alignment: a ctypes.Structure of as many fields takes 5 us to fill
 _ATTN = struct.Struct("@7i2f3P9qPqPP3qPPQ")
@@ -37,6 +37,10 @@ def _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site):
                       out.data_ptr(), os[0], os[1], os[2], 0 if lse is None else lse.data_ptr(), 0 if seed is None else seed.data_ptr(), site)
 
 
+def _strides(q, k, v, key_mask):
+    return q.stride(), k.stride(), v.stride(), None if key_mask is None else key_mask.stride()
+
+
 def _timed(name, nbytes):
     return _Timed(name, nbytes) if state.hbm_timer is not None else None
 
@@ -61,13 +65,14 @@ class CrossAttentionFn(torch.autograd.Function):
             rc = lib.uc2_xattn_fwd(desc, ptr(ws), n, stream())
             if timed is not None:
                 timed.__exit__()
+            note_leaves(ctx)
         if rc:
             check(rc)
         if grad:
             ctx.save_for_backward(q, k, v, key_mask, k_lens, out, lse, seed)
             # what the backward would work out again on a thread that has just been woken up: the call structure, as long as the tensors that come
             # back are the ones in it, and the workspace's size
-            ctx.cfg = (scale, drop_p, site, desc, lib.uc2_xattn_workspace(desc, 1))
+            ctx.cfg = (scale, drop_p, site, desc, _strides(q, k, v, key_mask), lib.uc2_xattn_workspace(desc, 1))
         return out
 
     @staticmethod
@@ -75,14 +80,16 @@ class CrossAttentionFn(torch.autograd.Function):
     def backward(ctx, dout):
         saved = ctx.saved_tensors
         q, k, v, key_mask, k_lens, out, lse, seed = saved
-        scale, drop_p, site, desc, n = ctx.cfg
+        scale, drop_p, site, desc, strides, n = ctx.cfg
         lib = _lib.load()
         with device_guard(q):
             dout = _rows16(dout)
+            # saved-tensor hooks may bring copies: elsewhere, or where the tensor itself had been with other strides
+            if _PTRS.unpack(desc)[:-1] != tuple([0 if t is None else t.data_ptr() for t in saved]) or strides != _strides(q, k, v, key_mask):
+                q, k, v, out, lse = _rows16(q), _rows16(k), _rows16(v), _rows16(out), lse.contiguous()
+                desc = _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site)
             dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
             ws = q.new_empty(n, dtype=torch.uint8)
-            if _PTRS.unpack(desc)[:-1] != tuple([0 if t is None else t.data_ptr() for t in saved]):      # (saved-tensor hooks may bring copies)
-                desc = _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site)
             gs, qs, ks = dout.stride(), dq.stride(), dk.stride()
             grad = _GRAD.pack(dout.data_ptr(), gs[0], gs[1], gs[2], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
                               ks[0], ks[1], ks[2])
