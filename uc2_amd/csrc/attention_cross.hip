@@ -63,14 +63,15 @@ template <int CPR> __device__ __forceinline__ int xa_swz(int row) {
   return ((row & 1) << 3) | ((row & 2) << 1) | ((row & 4) >> 1) | ((row & 8) >> 3);
 }
 
+__device__ __forceinline__ f32x16 xa_all(float x) { return f32x16{x, x, x, x, x, x, x, x, x, x, x, x, x, x, x, x}; }
+__device__ __forceinline__ f32x16 xa_zero() { return xa_all(0.f); }
 template <typename T, int D> struct XaMma;
 template <int D> struct XaMma<bf16, D> {
   typedef XaCfg<bf16, D> C;
   typedef bf16x8 Frag;
-  // acc[16] = rows blk*32.. of the tile (lane's row: lane & 31) against the owned vectors
-  static __device__ __forceinline__ f32x16 rows(const char* lds, int blk, const Frag (&own)[C::KS], int lane) {
+  // acc[16] += rows blk*32.. of the tile (lane's row: lane & 31) against the owned vectors
+  static __device__ __forceinline__ f32x16 rows(const char* lds, int blk, const Frag (&own)[C::KS], int lane, f32x16 acc = xa_zero()) {
     const int row = blk * 32 + (lane & 31), h = lane >> 5, sw = xa_swz<C::CPR>(row);
-    f32x16 acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < C::KS; ++s) {
       const bf16x8 a = *reinterpret_cast<const bf16x8*>(lds + row * C::RB + (((2 * s + h) ^ sw) << 4));
@@ -102,9 +103,8 @@ template <int D> struct XaMma<bf16, D> {
 template <int D> struct XaMma<float, D> {
   typedef XaCfg<float, D> C;
   typedef f32x4 Frag;
-  static __device__ __forceinline__ f32x16 rows(const char* lds, int blk, const Frag (&own)[C::KS], int lane) {
+  static __device__ __forceinline__ f32x16 rows(const char* lds, int blk, const Frag (&own)[C::KS], int lane, f32x16 acc = xa_zero()) {
     const int row = blk * 32 + (lane & 31), h = lane >> 5, sw = xa_swz<C::CPR>(row);
-    f32x16 acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < C::KS; ++s) {
       const f32x4 a = *reinterpret_cast<const f32x4*>(lds + row * C::RB + (((2 * s + h) ^ sw) << 4));
@@ -214,7 +214,7 @@ template <typename T, int D, int NT, bool PACKED> struct XaStage {
   }
 };
 
-// delta of a staged tile of packed rows: the chunks of `out` beside XaStage's of dout, multiplied on the way into LDS and summed over a row's CPR
+// -delta of a staged tile of packed rows: the chunks of `out` beside XaStage's of dout, multiplied on the way into LDS and summed over a row's CPR
 // neighbouring threads
 template <typename T, int D, int NT> struct XaDelta {
   typedef XaCfg<T, D> C;
@@ -244,7 +244,7 @@ template <typename T, int D, int NT> struct XaDelta {
       for (int e = 0; e < E; ++e) s = fmaf((float)o[e], (float)g[e], s);
 #pragma unroll
       for (int k = 1; k < C::CPR; k <<= 1) s += __shfl_xor(s, k);
-      if (idx % C::CPR == 0) d[row] = tt * C::TT + row < a.R ? s : 0.f;
+      if (idx % C::CPR == 0) d[row] = tt * C::TT + row < a.R ? -s : 0.f;
     }
   }
 };
@@ -505,6 +505,7 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
     if (lse == -INFINITY) lse = INFINITY;                          // a row without any key: p = 0
   }
   const float nlse = -lse;
+  const f32x16 ndelta = xa_all(DROP ? 0.f : -delta);              // dp's sums start at -delta (dropout scales dp first)
   f32x16 dq[C::DB];
 #pragma unroll
   for (int db = 0; db < C::DB; ++db)
@@ -535,7 +536,7 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
     for (int n = 0; n < C::NB; ++n) {
       if (!live || tt * C::TT + n * 32 >= len) break;
       const f32x16 s = M::rows(sh.x[buf], n, q, lane);
-      const f32x16 dp = M::rows(sh.y[buf], n, go, lane);
+      const f32x16 dp = M::rows(sh.y[buf], n, go, lane, ndelta);
       float ds[16];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -547,8 +548,7 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * k + e], a.scale2, bv[e]));
-          const float d = DROP ? (attn_keep(hq, hh[e], a.thresh) ? dp[4 * k + e] * a.keep_scale : 0.f) : dp[4 * k + e];
-          ds[4 * k + e] = p * (d - delta);
+          ds[4 * k + e] = p * (DROP ? (attn_keep(hq, hh[e], a.thresh) ? dp[4 * k + e] * a.keep_scale : 0.f) - delta : dp[4 * k + e]);
         }
       }
       M::cols(sh.x[buf], n, ds, dq, lane);
@@ -625,24 +625,43 @@ __device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DRO
     for (int n = 0; n < C::NB; ++n) {
       if (!live || tt * C::TT + n * 32 >= a.R) break;
       const f32x16 s = M::rows(sh.x[buf], n, kf, lane);
-      const f32x16 dp = M::rows(sh.y[buf], n, vf, lane);
+      // the rows' -log-sum-exp and -delta; without dropout dp's sums start at -delta (dropout scales dp first, and loads both late, for the registers)
+      f32x4 lv[4], dl[4];
+      f32x16 nd = xa_zero();
+      auto line = [&](int k) __attribute__((always_inline)) {
+        lv[k] = *reinterpret_cast<const f32x4*>(&sh.s[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+        dl[k] = *reinterpret_cast<const f32x4*>(&sh.d[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+      };
+      if (!DROP) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          line(k);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) nd[4 * k + e] = dl[k][e];
+        }
+      }
+      const f32x16 dp = M::rows(sh.y[buf], n, vf, lane, nd);
+      if (!DROP && a.kmask) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) lv[k] += f32x4{bias, bias, bias, bias};
+      }
       float p[16], ds[16];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int at = n * 32 + 8 * k + 4 * (lane >> 5);
-        f32x4 lv = *reinterpret_cast<const f32x4*>(&sh.s[buf][at]);
-        const f32x4 dl = *reinterpret_cast<const f32x4*>(&sh.d[buf][at]);
-        if (a.kmask) lv += f32x4{bias, bias, bias, bias};
         uint4 hv = {0, 0, 0, 0};
-        if (DROP) hv = *reinterpret_cast<const uint4*>(&sh.h[buf][at]);
+        if (DROP) {
+          line(k);
+          if (a.kmask) lv[k] += f32x4{bias, bias, bias, bias};
+          hv = *reinterpret_cast<const uint4*>(&sh.h[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+        }
         const uint32_t hh[4] = {hv.x, hv.y, hv.z, hv.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[4 * k + e], a.scale2, lv[e]));
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[4 * k + e], a.scale2, lv[k][e]));
           float d = dp[4 * k + e], y = x;
-          if (DROP) { const bool keep = attn_keep(hh[e], hk, a.thresh); d = keep ? d * a.keep_scale : 0.f; y = keep ? x * a.keep_scale : 0.f; }
+          if (DROP) { const bool keep = attn_keep(hh[e], hk, a.thresh); d = (keep ? d * a.keep_scale : 0.f) + dl[k][e]; y = keep ? x * a.keep_scale : 0.f; }
           p[4 * k + e] = y;
-          ds[4 * k + e] = x * (d - dl[e]);
+          ds[4 * k + e] = x * d;
         }
       }
       M::cols(sh.y[buf], n, p, dv, lane);
