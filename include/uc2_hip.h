@@ -349,7 +349,8 @@ int uc2_attn_general_probs_mean(int dtype, int B, int Lq, int Lk, int nh, int D,
  *   k_lens [B] int32 on the device, or NULL: keys at and behind k_lens[b] (clamped to 0 .. Lk) take no part.  key_mask [B, Lk] fp32
  *   additive (row stride key_mask_sb), or NULL: a key whose entry is <= -1e30 takes no part.  What the rows of such keys hold reaches
  *   nothing (NaN included), their dk / dv are zero; a row without any key gives zeros and passes no gradient.  lse [B, nkv, Lq, G] fp32: base-2
- *   log-sum-exp of each row (-inf: no key), for the backward; NULL in a forward that has none.  Dropout on the normalised weights, keep(row, key)
+ *   log-sum-exp of each row (-inf: no key), for the backward; NULL in a forward that has none.  out_f32 [B, nkv, Lq, G, D] fp32: bf16's output
+ *   before its rounding, which the backward reads in place of out (NULL: no backward, or fp32, whose backward reads out).  Dropout on the normalised weights, keep(row, key)
  *   a function of (*seed + site, batch, head, query, key head, key) as in uc2_attn_general_fwd (the same mask where nkv == nh).
  *   fp32 softmax and sums; bf16 rounds the weights (and their gradients) to bf16 where they enter the second matrix product.  No atomics:
  *   results repeat bit for bit.  ws: uc2_xattn_workspace bytes (0: may be NULL), not shared by calls that may overlap. */
@@ -361,7 +362,7 @@ typedef struct Uc2CrossAttn {
   const float* key_mask; long long key_mask_sb;
   const int* k_lens;
   void* out; long long o_sb, o_sl, o_sh;
-  float* lse;
+  float *lse, *out_f32;
   const uint64_t* seed; uint64_t site;
 } Uc2CrossAttn;
 typedef struct Uc2CrossAttnGrad {

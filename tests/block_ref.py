@@ -132,8 +132,8 @@ def attention(q, k, v, scale, key_mask=None, k_lens=None, dout=None, keep=None):
     dp = mm(dO, V.transpose(2, 3)) * kp
     delta = (dO * o).sum(-1, keepdim=True)
     ds = p * (dp - delta)
-    # an error of ds: of p, of delta (out's bound, and its sum over D), of dp's sum over D, and ds's own rounding
-    edelta = (dO.abs() * eo).sum(-1, keepdim=True) + 2 * D * u32 * (dO.abs() * o.abs()).sum(-1, keepdim=True)
+    # an error of ds: of p, of delta (out's bound before its rounding, and its sum over D), of dp's sum over D, and ds's own rounding
+    edelta = (dO.abs() * (eo - u * o.abs() + 4 * u32 * o.abs())).sum(-1, keepdim=True) + 2 * D * u32 * (dO.abs() * o.abs()).sum(-1, keepdim=True)
     eds = p * (edelta + 2 * D * u32 * mm(dO.abs(), V.abs().transpose(2, 3)) * kp) + (ep + up) * ds.abs() + (ep * p + tiny) * (dp.abs() + delta.abs()) + tiny
     dq = mm(ds, K) * scale
     edq = mm(eds + 2 * Lk * u32 * ds.abs(), K.abs()) * abs(scale) + u * dq.abs()

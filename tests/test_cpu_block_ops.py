@@ -16,7 +16,7 @@ I, F, A, L = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong
 class _CrossAttn(ctypes.Structure):             # Uc2CrossAttn
     _fields_ = ([(n, I) for n in "dtype B Lq Lk nh nkv D".split()] + [("scale", F), ("drop_p", F)] + [(n, A) for n in "qkv"]
                 + [(n, L) for n in "q_sb q_sl q_sh k_sb k_sl k_sh v_sb v_sl v_sh".split()]
-                + [("key_mask", A), ("key_mask_sb", L), ("k_lens", A), ("out", A), ("o_sb", L), ("o_sl", L), ("o_sh", L), ("lse", A), ("seed", A), ("site", ctypes.c_uint64)])
+                + [("key_mask", A), ("key_mask_sb", L), ("k_lens", A), ("out", A), ("o_sb", L), ("o_sl", L), ("o_sh", L), ("lse", A), ("out_f32", A), ("seed", A), ("site", ctypes.c_uint64)])
 
 
 class _CrossAttnGrad(ctypes.Structure):         # Uc2CrossAttnGrad
@@ -26,7 +26,7 @@ class _CrossAttnGrad(ctypes.Structure):         # Uc2CrossAttnGrad
 
 def attn(**kw):
     d = dict(dtype=1, B=2, Lq=3, Lk=5, nh=4, nkv=2, D=64, scale=0.125, drop_p=0.0, q=P, k=P, v=P, q_sb=768, q_sl=256, q_sh=64, k_sb=640, k_sl=128, k_sh=64, v_sb=640,
-             v_sl=128, v_sh=64, out=P, o_sb=768, o_sl=256, o_sh=64, lse=P)
+             v_sl=128, v_sh=64, out=P, o_sb=768, o_sl=256, o_sh=64, lse=P, out_f32=P)
     d.update(kw)
     return _CrossAttn(**d)
 
@@ -46,7 +46,8 @@ def test_cross_attention_backward_argument_errors():
     need = lib.uc2_xattn_workspace(ctypes.byref(many()), 1)
     assert need > 0 and lib.uc2_xattn_workspace(ctypes.byref(attn()), 1) == 0
     for a, gb, ws, n in ((many(lse=0), g, P, need), (many(), dict(g, dq=0), P, need), (many(), dict(g, dk=0), P, need), (many(), dict(g, dout_sl=3), P, need),
-                         (many(), dict(g, dv=P + 4), P, need), (many(), g, None, need), (many(), g, P, need - 1), (many(), g, P + 4, need), (attn(lse=0), g, None, 0)):
+                         (many(), dict(g, dv=P + 4), P, need), (many(), g, None, need), (many(), g, P, need - 1), (many(), g, P + 4, need), (attn(lse=0), g, None, 0),
+                         (attn(out_f32=0), g, None, 0), (attn(out_f32=P + 4), g, None, 0), (attn(dtype=0, out=0), g, None, 0)):
         assert lib.uc2_xattn_bwd(ctypes.byref(a), ctypes.byref(_CrossAttnGrad(**gb)), ws, n, None) == -1
     assert lib.uc2_xattn_bwd(ctypes.byref(attn()), None, P, need, None) == -1
     assert lib.uc2_xattn_fwd(None, None, 0, None) == -1
@@ -171,9 +172,9 @@ def test_structures_match_the_header(tmp_path):
     want = [int(x) for x in subprocess.check_output([str(tmp_path / "s")]).split()]
     here = [getattr(c, n).offset for c in (_CrossAttn, _CrossAttnGrad) for n, _ in c._fields_] + [ctypes.sizeof(_CrossAttn), ctypes.sizeof(_CrossAttnGrad)]
     assert want == here and [_ATTN.size, _GRAD.size] == here[-2:]
-    packed = _CrossAttn.from_buffer_copy(_ATTN.pack(*range(1, 8), 0.5, 0.25, *range(10, 32)))
+    packed = _CrossAttn.from_buffer_copy(_ATTN.pack(*range(1, 8), 0.5, 0.25, *range(10, 33)))
     got = [getattr(packed, n) for n, _ in _CrossAttn._fields_]
-    assert got == [*range(1, 8), 0.5, 0.25, *range(10, 32)]
+    assert got == [*range(1, 8), 0.5, 0.25, *range(10, 33)]
     packed = _CrossAttnGrad.from_buffer_copy(_GRAD.pack(*range(1, 17)))
     assert [getattr(packed, n) for n, _ in _CrossAttnGrad._fields_] == list(range(1, 17))
 
@@ -205,7 +206,7 @@ def test_oracle_attention_is_softmax():
 def test_saved_pointers_are_read_from_the_call_structure():
     from uc2_amd.ops.cross import _PTRS
     names = [n for n, _ in _CrossAttn._fields_]
-    packed = _ATTN.pack(*range(1, 8), 0.5, 0.25, *range(10, 32))
-    value = dict(zip(names, (*range(1, 8), 0.5, 0.25, *range(10, 32))))
+    packed = _ATTN.pack(*range(1, 8), 0.5, 0.25, *range(10, 33))
+    value = dict(zip(names, (*range(1, 8), 0.5, 0.25, *range(10, 33))))
     assert _PTRS.size == _ATTN.size
-    assert _PTRS.unpack(packed) == tuple(value[n] for n in ("q", "k", "v", "key_mask", "k_lens", "out", "lse", "seed", "site"))
+    assert _PTRS.unpack(packed) == tuple(value[n] for n in ("q", "k", "v", "key_mask", "k_lens", "out", "lse", "out_f32", "seed", "site"))

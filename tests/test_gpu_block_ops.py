@@ -379,6 +379,24 @@ def test_cross_attention_large_scores_and_scale(dtype):
     check_attn(q, k, v, dout, scale=-0.1)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,Lq,Lk,nh,nkv,D", [(3, 70, 1, 4, 2, 64), (2, 3, 300, 4, 4, 128), (1, 1, 5000, 4, 1, 32)])
+def test_cross_attention_one_key(dtype, B, Lq, Lk, nh, nkv, D):
+    """one key that takes part: out is its value, dq and dk are zero.  What is left: the weight is 1 within (2 + |x|) roundings of fp32 (score x, its
+    log-sum-exp), 1 in bf16, and dp and delta are sums of D products each: of sum |dout v| at most 2 D + 2 |x| + 8 of fp32's roundings"""
+    q, k, v, dout = attn_inputs(B, Lq, Lk, nh, nkv, D, dtype)
+    lens = torch.ones(B, dtype=torch.int32, device=DEV)
+    o, dq, dk, dv = run_attn(q, k, v, dout, k_lens=lens)
+    rep = lambda t: t[:, :1].double().repeat_interleave(nh // nkv, 2).expand(B, Lq, nh, D)  # noqa: E731
+    Q, K, V, dO = q.double(), rep(k), rep(v), dout.double()
+    x = (Q * K).abs().sum(-1, keepdim=True) * D ** -0.5
+    off = (2 * D + 2 * x + 8) * R.U[F32] * (dO * V).abs().sum(-1, keepdim=True)
+    R.assert_within(o, V, (R.U[dtype] * (dtype == BF16) + (4 + 2 * x) * R.U[F32]) * V.abs(), "out")
+    R.assert_within(dq, torch.zeros_like(Q), off * D ** -0.5 * K.abs(), "dq")
+    R.assert_within(dk[:, :1], torch.zeros_like(dk[:, :1]).double(), (off * D ** -0.5 * Q.abs()).view(B, Lq, nkv, -1, D).sum((1, 3))[:, None], "dk")
+    assert not dk[:, 1:].any() and not dv[:, 1:].any()
+
+
 def test_cross_attention_views():
     """heads before positions, fused projections, expanded keys, unaligned slices (copied), a gradient that is a broadcast"""
     B, Lq, Lk, nh, D = 2, 19, 70, 4, 64

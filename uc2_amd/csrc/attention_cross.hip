@@ -35,6 +35,7 @@ struct XaArgs {
   int BH;                                                         // B nkv
   XaSide fwd, dq, dkv;
   XaView q, k, v, o, dout;
+  float* o32;                                                     // bf16: the output before its rounding, [B nkv][R][D], for delta
   XaOut out, gq, gk, gv;
   const float* kmask; long long kmask_sb; const int* klens;
   float scale, scale2;                                            // scale2 = scale log2 e
@@ -214,34 +215,43 @@ template <typename T, int D, int NT, bool PACKED> struct XaStage {
   }
 };
 
-// -delta of a staged tile of packed rows: the chunks of `out` beside XaStage's of dout, multiplied on the way into LDS and summed over a row's CPR
-// neighbouring threads
+// -delta of a staged tile of packed rows: the values of `out` (bf16: before their rounding, see xa_delta_row) beside XaStage's chunks of dout, multiplied
+// on the way into LDS and summed over a row's CPR neighbouring threads
 template <typename T, int D, int NT> struct XaDelta {
   typedef XaCfg<T, D> C;
-  static constexpr int N = C::TT * C::CPR / NT;
+  static constexpr int N = C::TT * C::CPR / NT, E = 16 / sizeof(T);
   typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
-  u32x4 z[N];
+  f32x4 z[N][E / 4];
   const char* p; int t;
-  __device__ __forceinline__ void init(const XaArgs& a, int b, int kvh, int t_) { t = t_; p = a.o.p + b * a.o.sb + (long long)(kvh * a.G) * a.o.sh; }
+  __device__ __forceinline__ void init(const XaArgs& a, int bh, int b, int kvh, int t_) {
+    t = t_;
+    p = sizeof(T) == 2 ? reinterpret_cast<const char*>(a.o32 + (size_t)bh * a.R * D) : a.o.p + b * a.o.sb + (long long)(kvh * a.G) * a.o.sh;
+  }
   __device__ __forceinline__ void load(const XaArgs& a, int tt) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int idx = t + n * NT, r = min(tt * C::TT + idx / C::CPR, a.R - 1), c = idx % C::CPR;
-      int i, g;
-      xa_split(a, r, i, g);
-      z[n] = *reinterpret_cast<const u32x4*>(p + (long long)i * a.o.sl + (long long)g * a.o.sh + c * 16);
+      const char* at = p;
+      if (sizeof(T) == 2) {
+        at += ((long long)r * D + c * 8) * 4;
+      } else {
+        int i, g;
+        xa_split(a, r, i, g);
+        at += (long long)i * a.o.sl + (long long)g * a.o.sh + c * 16;
+      }
+#pragma unroll
+      for (int j = 0; j < E / 4; ++j) z[n][j] = reinterpret_cast<const f32x4*>(at)[j];
     }
   }
   __device__ __forceinline__ void store(const XaArgs& a, const u32x4 (&y)[N], float* d, int tt) {
-    constexpr int E = 16 / sizeof(T);
     typedef T V __attribute__((ext_vector_type(E)));
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int idx = t + n * NT, row = idx / C::CPR;
-      const V o = __builtin_bit_cast(V, z[n]), g = __builtin_bit_cast(V, y[n]);
+      const V g = __builtin_bit_cast(V, y[n]);
       float s = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) s = fmaf((float)o[e], (float)g[e], s);
+      for (int e = 0; e < E; ++e) s = fmaf(z[n][e / 4][e % 4], (float)g[e], s);
 #pragma unroll
       for (int k = 1; k < C::CPR; k <<= 1) s += __shfl_xor(s, k);
       if (idx % C::CPR == 0) d[row] = tt * C::TT + row < a.R ? -s : 0.f;
@@ -262,6 +272,26 @@ __device__ __forceinline__ void xa_own(const XaArgs& a, const XaView& X, int b, 
 #pragma unroll
     for (int s = 0; s < XaCfg<T, D>::KS; ++s) f[s] = __builtin_bit_cast(Frag, uint4{0, 0, 0, 0});
   }
+}
+// delta[r] = dout . out of an owned row, with the output as it was before its rounding to bf16: a row's gradients of the scores, p (dp - delta), nearly
+// cancel where it has few keys or one that outweighs the others, and an output off by 2^-9 there left dq and dk off by 4e-3 to 8e-3 of their norm
+// (2 to 40 keys; with this 2.5e-3, what the roundings of the score gradients and of the result make; one key: 2^-24 in place of 2^-9 of dout . out)
+template <typename T, int D>
+__device__ __forceinline__ float xa_delta_row(const XaArgs& a, int bh, int b, int kvh, int r, bool take, int lane, const typename XaMma<T, D>::Frag (&go)[XaCfg<T, D>::KS]) {
+  constexpr int E = 16 / sizeof(T);
+  float s = 0.f;
+  if (take) {
+    const char* p = sizeof(T) == 2 ? reinterpret_cast<const char*>(a.o32 + ((size_t)bh * a.R + r) * D) : xa_row<true>(a, a.o, b, kvh, r);
+#pragma unroll
+    for (int k = 0; k < XaCfg<T, D>::KS; ++k)
+#pragma unroll
+      for (int j = 0; j < E / 4; ++j) {
+        const f32x4 o = reinterpret_cast<const f32x4*>(p + (2 * k + (lane >> 5)) * E * 4)[j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = fmaf(o[e], (float)go[k][4 * j + e], s);
+      }
+  }
+  return s + __shfl_xor(s, 32);
 }
 // 4 consecutive values of the head dimension
 __device__ __forceinline__ void xa_put4(bf16* p, float a, float b, float c, float d) {
@@ -409,6 +439,7 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
     const float inv = l > 0.f ? 1.0f / l : (l == l ? 0.f : l);     // no key: zeros; NaN stays NaN
     xa_put_row<T, C::DB>(a.out.p + b * a.out.sb + (long long)i * a.out.sl + (long long)(kvh * a.G + g) * a.out.sh, o, inv, lane);
     if (a.lse && lane < 32) a.lse[(size_t)bh * a.R + r] = m + __log2f(l);
+    if (sizeof(T) == 2 && a.o32) xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.o32 + ((size_t)bh * a.R + r) * D), o, inv, lane);
   } else {
     const size_t row = ((size_t)split * a.BH + bh) * a.R + r;
     xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.fwd.part + row * D), o, 1.0f, lane);
@@ -457,7 +488,11 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a) {
   xa_split(a, r, i, g);
   T* out = reinterpret_cast<T*>(a.out.p + b * a.out.sb + (long long)i * a.out.sl + (long long)(kvh * a.G + g) * a.out.sh);
 #pragma unroll
-  for (int e = 0; e < E; ++e) if (D >= 64 || lane < D) out[lane + 64 * e] = from_f<T>(o[e] * inv);
+  for (int e = 0; e < E; ++e)
+    if (D >= 64 || lane < D) {
+      out[lane + 64 * e] = from_f<T>(o[e] * inv);
+      if (sizeof(T) == 2 && a.o32) a.o32[row * D + lane + 64 * e] = o[e] * inv;
+    }
   if (a.lse && lane == 0) a.lse[row] = top + __log2f(l);
 }
 
@@ -490,16 +525,8 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
   typename M::Frag q[C::KS], go[C::KS];
   xa_own<T, D, true>(a, a.q, b, kvh, r, mine, lane, q);
   xa_own<T, D, true>(a, a.dout, b, kvh, r, mine, lane, go);
-  float delta = 0.f, lse = INFINITY;
-  {
-    typename M::Frag of[C::KS];
-    xa_own<T, D, true>(a, a.o, b, kvh, r, mine, lane, of);
-#pragma unroll
-    for (int s = 0; s < C::KS; ++s)
-#pragma unroll
-      for (int j = 0; j < (int)(16 / sizeof(T)); ++j) delta = fmaf((float)of[s][j], (float)go[s][j], delta);
-    delta += __shfl_xor(delta, 32);
-  }
+  float lse = INFINITY;
+  const float delta = xa_delta_row<T, D>(a, bh, b, kvh, r, mine, lane, go);
   if (mine) {
     lse = a.lse[(size_t)bh * a.R + r];
     if (lse == -INFINITY) lse = INFINITY;                          // a row without any key: p = 0
@@ -596,7 +623,7 @@ __device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DRO
   XaStage<T, D, NS * 64, true> st;
   st.init(a, a.q, a.dout, b, kvh, a.R, t);
   XaDelta<T, D, NS * 64> dl8;
-  dl8.init(a, b, kvh, t);
+  dl8.init(a, bh, b, kvh, t);
   float lse = 0.f; uint32_t hash = 0;
   auto fetch = [&](int tt) __attribute__((always_inline)) {
     st.load(a, a.q, a.dout, tt);
@@ -784,12 +811,13 @@ static int xa_check(const Uc2CrossAttn* p) {
   UC2_CHECK_ARG(p->drop_p >= 0.f && p->drop_p < 1.f);
   return 0;
 }
-static int xa_ptrs(const Uc2CrossAttn* p) {
+static int xa_ptrs(const Uc2CrossAttn* p, bool backward) {
   const int el = p->dtype ? 2 : 4;
-  UC2_CHECK_ARG(p->q && p->out && (p->Lk == 0 || (p->k && p->v)));
+  UC2_CHECK_ARG(p->q && (p->out || (backward && p->dtype == 1 && p->out_f32)) && (p->Lk == 0 || (p->k && p->v)));
+  UC2_CHECK_ARG(!backward || p->dtype == 0 || p->out_f32);
   UC2_CHECK_ARG(xa_str_ok(p->q_sb, p->q_sl, p->q_sh, el) && xa_str_ok(p->k_sb, p->k_sl, p->k_sh, el) && xa_str_ok(p->v_sb, p->v_sl, p->v_sh, el));
   UC2_CHECK_ARG(xa_str_ok(p->o_sb, p->o_sl, p->o_sh, el));
-  UC2_CHECK_ARG((((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->out) & 15) == 0);
+  UC2_CHECK_ARG((((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->out | (uintptr_t)p->out_f32) & 15) == 0);
   return 0;
 }
 static XaArgs xa_args(const Uc2CrossAttn* p) {
@@ -803,7 +831,7 @@ static XaArgs xa_args(const Uc2CrossAttn* p) {
   a.o = {(const char*)p->out, p->o_sb * el, p->o_sl * el, p->o_sh * el};
   a.kmask = p->key_mask; a.kmask_sb = p->key_mask_sb; a.klens = p->k_lens;
   a.scale = p->scale; a.scale2 = p->scale * XA_LOG2E;
-  a.lse = p->lse;
+  a.lse = p->lse; a.o32 = p->out_f32;
   a.thresh = drop_thresh(p->drop_p); a.keep_scale = 1.0f / (1.0f - p->drop_p); a.seed_ptr = p->seed; a.seed_imm = p->site;
   return a;
 }
@@ -840,7 +868,7 @@ extern "C" int uc2_xattn_fwd(const Uc2CrossAttn* attn, void* ws, size_t ws_bytes
   if (int e = xa_check(attn)) return e;
   const Uc2CrossAttn norm = xa_norm(attn), *p = &norm;
   if (p->B == 0 || p->Lq == 0) return 0;
-  if (int e = xa_ptrs(p)) return e;
+  if (int e = xa_ptrs(p, false)) return e;
   const XaPlan pl = xa_plan(p);
   UC2_CHECK_ARG(pl.fwd == 0 || (ws && ws_bytes >= pl.fwd && ((uintptr_t)ws & 15) == 0));
   hipStream_t st = (hipStream_t)stream;
@@ -885,7 +913,7 @@ extern "C" int uc2_xattn_bwd(const Uc2CrossAttn* attn, const Uc2CrossAttnGrad* g
   UC2_CHECK_ARG(xa_str_ok(g->dout_sb, g->dout_sl, g->dout_sh, el) && xa_str_ok(g->dq_sb, g->dq_sl, g->dq_sh, el));
   UC2_CHECK_ARG(xa_str_ok(g->dk_sb, g->dk_sl, g->dk_sh, el) && xa_str_ok(g->dv_sb, g->dv_sl, g->dv_sh, el));
   UC2_CHECK_ARG((((uintptr_t)g->dout | (uintptr_t)g->dq | (uintptr_t)g->dk | (uintptr_t)g->dv) & 15) == 0);
-  if (p->Lq > 0) { if (int e = xa_ptrs(p)) return e; }
+  if (p->Lq > 0) { if (int e = xa_ptrs(p, true)) return e; }
   const XaPlan pl = xa_plan(p);
   UC2_CHECK_ARG(pl.bwd == 0 || (ws && ws_bytes >= pl.bwd && ((uintptr_t)ws & 15) == 0));
   hipStream_t st = (hipStream_t)stream;

@@ -10,10 +10,10 @@ from ..config import state
 from .base import _Timed, _require_cuda, device_guard, note_leaves, once, rng
 
 # Uc2CrossAttn and Uc2CrossAttnGrad (include/uc2_hip.h), packed in native alignment: a ctypes.Structure of as many fields takes 5 us to fill
-_ATTN = struct.Struct("@7i2f3P9qPqPP3qPPQ")
+_ATTN = struct.Struct("@7i2f3P9qPqPP3qPPPQ")
 _GRAD = struct.Struct("@P3q3P9q")
-# its pointers q, k, v, key_mask, k_lens, out, lse, seed (the order they are saved in) and what is left of it
-_PTRS = struct.Struct("@40x3P72xP8xPP24xPPQ")
+# its pointers q, k, v, key_mask, k_lens, out, lse, out_f32, seed and what is left of it
+_PTRS = struct.Struct("@40x3P72xP8xPP24xPPPQ")
 
 
 def _rows16(x):
@@ -28,13 +28,14 @@ def _rows16(x):
     return x.clone(memory_format=torch.contiguous_format)          # (contiguous() would hand an unaligned dense tensor back)
 
 
-def _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site):
+def _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, out_f32, seed, site):
     B, Lq, nh, D = q.shape
-    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), (0, 0, 0) if out is None else out.stride()
     return _ATTN.pack(dt(q.dtype), B, Lq, k.shape[1], nh, k.shape[2], D, scale, drop_p, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                       qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
                       0 if key_mask is None else key_mask.data_ptr(), 0 if key_mask is None else key_mask.stride(0), 0 if k_lens is None else k_lens.data_ptr(),
-                      out.data_ptr(), os[0], os[1], os[2], 0 if lse is None else lse.data_ptr(), 0 if seed is None else seed.data_ptr(), site)
+                      0 if out is None else out.data_ptr(), os[0], os[1], os[2], 0 if lse is None else lse.data_ptr(),
+                      0 if out_f32 is None else out_f32.data_ptr(), 0 if seed is None else seed.data_ptr(), site)
 
 
 def _strides(q, k, v, key_mask):
@@ -58,7 +59,8 @@ class CrossAttentionFn(torch.autograd.Function):
             grad = need[0] or need[1] or need[2]
             out = q.new_empty((B, Lq, nh, D))
             lse = q.new_empty((B, k.shape[2], Lq, nh // k.shape[2]), dtype=torch.float32) if grad else None
-            desc = _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site)
+            out_f32 = q.new_empty((B, k.shape[2], Lq, nh // k.shape[2], D), dtype=torch.float32) if grad and q.dtype == torch.bfloat16 else None
+            desc = _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, out_f32, seed, site)
             n = lib.uc2_xattn_workspace(desc, 0)
             ws = q.new_empty(n, dtype=torch.uint8) if n else None
             timed = _timed("xattn_fwd", q.element_size() * (2 * q.numel() + k.numel() + v.numel()))
@@ -69,7 +71,7 @@ class CrossAttentionFn(torch.autograd.Function):
         if rc:
             check(rc)
         if grad:
-            ctx.save_for_backward(q, k, v, key_mask, k_lens, out, lse, seed)
+            ctx.save_for_backward(q, k, v, key_mask, k_lens, out if out_f32 is None else out_f32, lse, seed)
             # what the backward would work out again on a thread that has just been woken up: the call structure, as long as the tensors that come
             # back are the ones in it, and the workspace's size
             ctx.cfg = (scale, drop_p, site, desc, _strides(q, k, v, key_mask), lib.uc2_xattn_workspace(desc, 1))
@@ -79,15 +81,17 @@ class CrossAttentionFn(torch.autograd.Function):
     @once
     def backward(ctx, dout):
         saved = ctx.saved_tensors
-        q, k, v, key_mask, k_lens, out, lse, seed = saved
+        q, k, v, key_mask, k_lens, out, lse, seed = saved                     # (out: before its rounding, if it was rounded)
         scale, drop_p, site, desc, strides, n = ctx.cfg
         lib = _lib.load()
         with device_guard(q):
             dout = _rows16(dout)
             # saved-tensor hooks may bring copies: elsewhere, or where the tensor itself had been with other strides
-            if _PTRS.unpack(desc)[:-1] != tuple([0 if t is None else t.data_ptr() for t in saved]) or strides != _strides(q, k, v, key_mask):
-                q, k, v, out, lse = _rows16(q), _rows16(k), _rows16(v), _rows16(out), lse.contiguous()
-                desc = _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, seed, site)
+            p = _PTRS.unpack(desc)
+            if (*p[:5], p[7] or p[5], p[6], p[8]) != tuple([0 if t is None else t.data_ptr() for t in saved]) or strides != _strides(q, k, v, key_mask):
+                q, k, v, lse = _rows16(q), _rows16(k), _rows16(v), lse.contiguous()
+                out, out_f32 = (None, out.clone(memory_format=torch.contiguous_format)) if q.dtype == torch.bfloat16 else (_rows16(out), None)
+                desc = _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, out_f32, seed, site)
             dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
             ws = q.new_empty(n, dtype=torch.uint8)
             gs, qs, ks = dout.stride(), dq.stride(), dk.stride()
