@@ -313,7 +313,8 @@ def check_attn(q, k, v, dout, key_mask=None, k_lens=None, scale=None, what=""):
 
 ATTN = [  # B, Lq, Lk, nh, nkv, D
     (1, 1, 1, 1, 1, 64), (2, 1, 300, 4, 1, 64), (3, 5, 31, 4, 2, 32), (2, 33, 65, 2, 2, 64), (1, 60, 100, 12, 12, 64), (2, 130, 64, 3, 3, 64), (1, 77, 211, 12, 4, 64),
-    (2, 17, 129, 4, 2, 128), (1, 200, 257, 2, 1, 128), (9, 10, 40, 2, 1, 32), (1, 257, 513, 2, 2, 64), (1, 1, 4097, 8, 2, 128), (1, 1000, 33, 2, 2, 32), (1, 1500, 1, 1, 1, 64)]
+    (2, 17, 129, 4, 2, 128), (1, 200, 257, 2, 1, 128), (9, 10, 40, 2, 1, 32), (1, 257, 513, 2, 2, 64), (1, 1, 4097, 8, 2, 128), (1, 1000, 33, 2, 2, 32), (1, 1500, 1, 1, 1, 64),
+    (2, 513, 1100, 4, 2, 64), (1, 900, 1201, 4, 4, 32), (2, 300, 2000, 4, 2, 128)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -323,7 +324,7 @@ def test_cross_attention_plain(dtype, B, Lq, Lk, nh, nkv, D):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("B,Lq,Lk,nh,nkv,D", [(5, 9, 200, 4, 2, 64), (4, 40, 130, 2, 2, 128), (6, 1, 1100, 4, 1, 32), (3, 300, 95, 3, 3, 64)])
+@pytest.mark.parametrize("B,Lq,Lk,nh,nkv,D", [(5, 9, 200, 4, 2, 64), (4, 40, 130, 2, 2, 128), (6, 1, 1100, 4, 1, 32), (3, 300, 95, 3, 3, 64), (5, 450, 1000, 4, 2, 64)])
 def test_cross_attention_lengths(dtype, B, Lq, Lk, nh, nkv, D):
     """lengths of zero and one, inside and at the end of tiles, over and under the range (clamped), with NaN and infinities behind them"""
     q, k, v, dout = attn_inputs(B, Lq, Lk, nh, nkv, D, dtype)
@@ -339,7 +340,7 @@ def test_cross_attention_lengths(dtype, B, Lq, Lk, nh, nkv, D):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("B,Lq,Lk,nh,nkv,D", [(4, 9, 200, 4, 2, 64), (4, 70, 60, 2, 2, 128), (4, 1, 900, 4, 1, 32)])
+@pytest.mark.parametrize("B,Lq,Lk,nh,nkv,D", [(4, 9, 200, 4, 2, 64), (4, 70, 60, 2, 2, 128), (4, 1, 900, 4, 1, 32), (4, 300, 1000, 4, 2, 64)])
 def test_cross_attention_key_mask(dtype, B, Lq, Lk, nh, nkv, D):
     """-inf, -1e30 and the lowest fp32 remove a key with whatever it holds; finite entries weigh; a row of nothing gives zeros"""
     q, k, v, dout = attn_inputs(B, Lq, Lk, nh, nkv, D, dtype)
@@ -465,9 +466,10 @@ def test_cross_attention_gradient_against_differences():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_cross_attention_dropout(dtype):
+@pytest.mark.parametrize("B,Lq,Lk", [(2, 40, 90), (3, 800, 700)])
+def test_cross_attention_dropout(dtype, B, Lq, Lk):
     """the mask of the general kernels (equal head counts); its rate, and the gradients under it"""
-    B, Lq, Lk, nh, D, p = 2, 40, 90, 3, 64, 0.25
+    nh, D, p = 3, 64, 0.25
     q, k, v, dout = attn_inputs(B, Lq, Lk, nh, nh, D, dtype)
     seed = torch.tensor([12345678901], device=DEV)
     # the multipliers themselves: uniform weights (q = 0) against unit values one key at a time

@@ -36,6 +36,7 @@ struct XaArgs {
   XaSide fwd, dq, dkv;
   XaView q, k, v, o, dout;
   float* o32;                                                     // bf16: the output before its rounding, [B nkv][R][D], for delta
+  float* delta;                                                   // [B nkv][R], where a kernel of its own forms them
   XaOut out, gq, gk, gv;
   const float* kmask; long long kmask_sb; const int* klens;
   float scale, scale2;                                            // scale2 = scale log2 e
@@ -496,8 +497,8 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a) {
   if (a.lse && lane == 0) a.lse[row] = top + __log2f(l);
 }
 
-// The backward is one launch of two kinds of workgroups, dK / dV and dQ: neither needs the other (each forms delta[r] = dout . out itself), so a short
-// problem pays one launch and one latency instead of two.
+// The backward is one launch of two kinds of workgroups, dK / dV and dQ: neither needs the other (each forms delta[r] = dout . out itself, but for long
+// key axes), so a short problem pays one launch and one latency instead of two.
 template <typename T, int D, bool DROP> struct XaLds {
   typedef XaCfg<T, D> C;
   __attribute__((aligned(16))) char x[2][C::TT * C::RB], y[2][C::TT * C::RB];
@@ -507,7 +508,7 @@ template <typename T, int D, bool DROP> struct XaLds {
 
 // dQ (owned query rows, streamed keys)
 //   dx = p (dp - delta),  dp = dout v^T (dropped as the forward's weights were),  dq = scale dx k
-template <typename T, int D, int NS, bool DROP>
+template <typename T, int D, int NS, bool DROP, bool PRE>
 __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP>& sh) {
   typedef XaCfg<T, D> C;
   typedef XaMma<T, D> M;
@@ -526,7 +527,7 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
   xa_own<T, D, true>(a, a.q, b, kvh, r, mine, lane, q);
   xa_own<T, D, true>(a, a.dout, b, kvh, r, mine, lane, go);
   float lse = INFINITY;
-  const float delta = xa_delta_row<T, D>(a, bh, b, kvh, r, mine, lane, go);
+  const float delta = !PRE ? xa_delta_row<T, D>(a, bh, b, kvh, r, mine, lane, go) : mine ? a.delta[(size_t)bh * a.R + r] : 0.f;
   if (mine) {
     lse = a.lse[(size_t)bh * a.R + r];
     if (lse == -INFINITY) lse = INFINITY;                          // a row without any key: p = 0
@@ -595,7 +596,7 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
 }
 
 // dK, dV (owned keys, streamed packed query rows):  dv = p^T dout,  dk = scale dx^T q
-template <typename T, int D, int NS, bool DROP>
+template <typename T, int D, int NS, bool DROP, bool PRE>
 __device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DROP>& sh) {
   typedef XaCfg<T, D> C;
   typedef XaMma<T, D> M;
@@ -623,13 +624,14 @@ __device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DRO
   XaStage<T, D, NS * 64, true> st;
   st.init(a, a.q, a.dout, b, kvh, a.R, t);
   XaDelta<T, D, NS * 64> dl8;
-  dl8.init(a, bh, b, kvh, t);
-  float lse = 0.f; uint32_t hash = 0;
+  if (!PRE) dl8.init(a, bh, b, kvh, t);
+  float lse = 0.f, delta = 0.f; uint32_t hash = 0;
   auto fetch = [&](int tt) __attribute__((always_inline)) {
     st.load(a, a.q, a.dout, tt);
-    dl8.load(a, tt);
+    if (!PRE) dl8.load(a, tt);
     if (t < C::TT) {
       const int r = tt * C::TT + t;
+      if (PRE) delta = a.delta[(size_t)bh * a.R + min(r, a.R - 1)];
       lse = INFINITY;                                              // behind the last row, and rows without any key: p = 0
       if (r < a.R) {
         lse = a.lse[(size_t)bh * a.R + r];
@@ -640,8 +642,8 @@ __device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DRO
   };
   auto put = [&](int tt, int buf) __attribute__((always_inline)) {
     st.store(sh.x[buf], sh.y[buf], tt, nullptr);
-    dl8.store(a, st.y, sh.d[buf], tt);
-    if (t < C::TT) { sh.s[buf][t] = -lse; if (DROP) sh.h[buf][t] = hash; }
+    if (!PRE) dl8.store(a, st.y, sh.d[buf], tt);
+    if (t < C::TT) { sh.s[buf][t] = -lse; if (PRE) sh.d[buf][t] = tt * C::TT + t < a.R ? -delta : 0.f; if (DROP) sh.h[buf][t] = hash; }
   };
   if (t0 < t1) { fetch(t0); put(t0, 0); }
   __syncthreads();
@@ -715,11 +717,36 @@ __device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DRO
   }
 }
 
-template <typename T, int D, int NS, bool DROP>
+template <typename T, int D, int NS, bool DROP, bool PRE = false>
 __global__ __launch_bounds__(NS * 64) void xattn_bwd_kernel(XaArgs a) {
   __shared__ XaLds<T, D, DROP> sh;
-  if ((int)blockIdx.x < a.dkv.blocks) xa_dkv<T, D, NS, DROP>(a, blockIdx.x, sh);
-  else xa_dq<T, D, NS, DROP>(a, blockIdx.x - a.dkv.blocks, sh);
+  if ((int)blockIdx.x < a.dkv.blocks) xa_dkv<T, D, NS, DROP, PRE>(a, blockIdx.x, sh);
+  else xa_dq<T, D, NS, DROP, PRE>(a, blockIdx.x - a.dkv.blocks, sh);
+}
+
+// delta of every row, where many workgroups would form it again: CPR lanes per row
+template <typename T, int D>
+__global__ __launch_bounds__(256) void xattn_delta_kernel(XaArgs a) {
+  typedef XaCfg<T, D> C;
+  constexpr int E = 16 / sizeof(T);
+  typedef T V __attribute__((ext_vector_type(E)));
+  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x, row = idx / C::CPR, rows = (long long)a.BH * a.R;
+  const int c = (int)(idx % C::CPR);
+  float s = 0.f;
+  if (row < rows) {
+    const int bh = (int)(row / a.R), r = (int)(row - (long long)bh * a.R), b = bh / a.nkv, kvh = bh - b * a.nkv;
+    const char* p = sizeof(T) == 2 ? reinterpret_cast<const char*>(a.o32 + row * D) : xa_row<true>(a, a.o, b, kvh, r);
+    const V g = *reinterpret_cast<const V*>(xa_row<true>(a, a.dout, b, kvh, r) + c * 16);
+#pragma unroll
+    for (int j = 0; j < E / 4; ++j) {
+      const f32x4 o = reinterpret_cast<const f32x4*>(p + c * E * 4)[j];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = fmaf(o[e], (float)g[4 * j + e], s);
+    }
+  }
+#pragma unroll
+  for (int k = 1; k < C::CPR; k <<= 1) s += __shfl_xor(s, k);
+  if (row < rows && c == 0) a.delta[row] = s;
 }
 
 // sums of the splits' gradients in split order: dK and dV, then dQ, where they were split
@@ -774,7 +801,7 @@ static int xa_splits(const Uc2CrossAttn* p, int ns, int cols, int streamed) {
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 static size_t xa_up(size_t n) { return (n + 255) & ~(size_t)255; }
-struct XaPlan { int ns_bwd, s_fwd, s_dq, s_dkv; size_t fwd, part_dkv, bwd; };
+struct XaPlan { int ns_bwd, s_fwd, s_dq, s_dkv; bool pre; size_t fwd, delta, part_dkv, bwd; };
 static XaPlan xa_plan(const Uc2CrossAttn* p) {
   XaPlan r{};
   const long long bh = (long long)p->B * p->nkv, R = (long long)p->Lq * (p->nh / p->nkv);
@@ -786,7 +813,11 @@ static XaPlan xa_plan(const Uc2CrossAttn* p) {
   r.s_dq = xa_splits(p, r.ns_bwd, (int)R, p->Lk);
   r.s_dkv = xa_splits(p, r.ns_bwd, p->Lk, (int)R);
   r.part_dkv = r.s_dkv > 1 ? xa_up((size_t)r.s_dkv * 2 * bh * p->Lk * p->D * 4) : 0;
-  r.bwd = r.part_dkv + (r.s_dq > 1 ? (size_t)r.s_dq * bh * R * p->D * 4 : 0);
+  // delta by a kernel of its own where five workgroups or more stream the same rows and there is work to hide a launch in (2 x 2048 x 4096, 16 heads, forward
+  // and backward 377 us against 398; 8 x 100 x 600, 12 heads 46.5 against 47; 128 x 2000, 4 heads 25 against 23.6)
+  r.pre = r.ns_bwd == 4 && p->Lk > 512 && bh * R * p->Lk >= (1 << 22);
+  r.delta = r.pre ? xa_up((size_t)bh * R * 4) : 0;
+  r.bwd = r.delta + r.part_dkv + (r.s_dq > 1 ? (size_t)r.s_dq * bh * R * p->D * 4 : 0);
   return r;
 }
 static bool xa_str_ok(long long sb, long long sl, long long sh, int el) {      // 16-byte rows
@@ -847,10 +878,11 @@ static bool xa_side(const XaArgs& a, XaSide& side, int cols, int ns, int splits)
     if (a.thresh) hipLaunchKernelGGL((KERN<TT_, DD_, NN_, true>), dim3(grid), dim3(NN_ * 64), 0, st, a);                             \
     else hipLaunchKernelGGL((KERN<TT_, DD_, NN_, false>), dim3(grid), dim3(NN_ * 64), 0, st, a);                                     \
   } while (0)
-#define XA_NS(KERN, TT_, DD_)                                                                                                       \
+#define XA_NS(KERN, TT_, DD_, MOST)      /* MOST: bytes of the rows that two waves may stage */                                       \
   do {                                                                                                                              \
     if constexpr (DD_ * sizeof(TT_) <= 256) { if (ns == 1) { XA_LAUNCH(KERN, TT_, DD_, 1, grid); break; } }                          \
-    if (ns == 2) XA_LAUNCH(KERN, TT_, DD_, 2, grid); else XA_LAUNCH(KERN, TT_, DD_, 4, grid); \
+    if constexpr (DD_ * sizeof(TT_) <= MOST) { if (ns == 2) { XA_LAUNCH(KERN, TT_, DD_, 2, grid); break; } }                         \
+    XA_LAUNCH(KERN, TT_, DD_, 4, grid);                                                                                             \
   } while (0)
 #define XA_TD(WHAT)                                                                                                                 \
   do {                                                                                                                              \
@@ -880,7 +912,7 @@ extern "C" int uc2_xattn_fwd(const Uc2CrossAttn* attn, void* ws, size_t ws_bytes
     a.pml = (float*)((char*)ws + xa_up((size_t)pl.s_fwd * a.BH * a.R * p->D * 4));
   }
   const int grid = a.fwd.blocks;
-#define XA_GO(T_, D_) XA_NS(xattn_fwd_kernel, T_, D_)
+#define XA_GO(T_, D_) XA_NS(xattn_fwd_kernel, T_, D_, 512)
   XA_TD(XA_GO);
 #undef XA_GO
   UC2_LAUNCH_CHECK();
@@ -924,13 +956,24 @@ extern "C" int uc2_xattn_bwd(const Uc2CrossAttn* attn, const Uc2CrossAttnGrad* g
   a.gv = {(char*)g->dv, g->dv_sb * el, g->dv_sl * el, g->dv_sh * el};
   const int ns = pl.ns_bwd;
   UC2_CHECK_ARG(xa_side(a, a.dkv, a.Lk, ns, pl.s_dkv) && xa_side(a, a.dq, a.R, ns, pl.s_dq));
-  a.dkv.part = (float*)ws;
-  a.dq.part = (float*)((char*)ws + pl.part_dkv);
+  a.delta = (float*)ws;
+  a.dkv.part = (float*)((char*)ws + pl.delta);
+  a.dq.part = (float*)((char*)ws + pl.delta + pl.part_dkv);
   const int grid = a.dkv.blocks + a.dq.blocks;
   if (grid == 0) return 0;                                        // (neither queries nor keys)
-#define XA_GO(T_, D_) XA_NS(xattn_bwd_kernel, T_, D_)
-  XA_TD(XA_GO);
+  if (pl.pre && a.R > 0) {
+    const long long lanes = (long long)a.BH * a.R * (p->D * el / 16), n = (lanes + 255) / 256;
+    UC2_CHECK_ARG(n < (1ll << 31));
+#define XA_GO(T_, D_) hipLaunchKernelGGL((xattn_delta_kernel<T_, D_>), dim3((unsigned)n), dim3(256), 0, st, a);                    \
+    if (a.thresh) hipLaunchKernelGGL((xattn_bwd_kernel<T_, D_, 4, true, true>), dim3(grid), dim3(256), 0, st, a);                   \
+    else hipLaunchKernelGGL((xattn_bwd_kernel<T_, D_, 4, false, true>), dim3(grid), dim3(256), 0, st, a)
+    XA_TD(XA_GO);
 #undef XA_GO
+  } else {
+#define XA_GO(T_, D_) XA_NS(xattn_bwd_kernel, T_, D_, 256)
+    XA_TD(XA_GO);
+#undef XA_GO
+  }
   UC2_LAUNCH_CHECK();
   const long long rows = (pl.s_dkv > 1 ? 2ll * a.BH * a.Lk : 0) + (pl.s_dq > 1 ? (long long)a.BH * a.R : 0), blocks = (rows * (p->D / 4) + 255) / 256;
   UC2_CHECK_ARG(blocks < (1ll << 31));
