@@ -140,11 +140,18 @@ template <bool PACKED> __device__ __forceinline__ const char* xa_row(const XaArg
   xa_split(a, r, i, g);
   return x.p + b * x.sb + (long long)i * x.sl + (long long)(kvh * a.G + g) * x.sh;
 }
-__device__ __forceinline__ float xa_key_bias(const XaArgs& a, int b, int key, int len) {     // base-2 additive mask; -inf: no part
-  if (key >= len) return -INFINITY;
-  if (!a.kmask) return 0.f;
-  const float m = a.kmask[b * a.kmask_sb + key];
-  return m <= XA_REMOVED ? -INFINITY : m * XA_LOG2E;
+// base-2 additive mask of a key from the mask's entry (read apart: a tile's loads are issued together and nothing waits for one of them before put()
+// does); -inf: no part
+__device__ __forceinline__ float xa_key_raw(const XaArgs& a, int b, int key, int len) { return a.kmask ? a.kmask[b * a.kmask_sb + min(key, len - 1)] : 0.f; }
+__device__ __forceinline__ float xa_key_bias(const XaArgs& a, float raw, int key, int len) {
+  return key >= len || (a.kmask && raw <= XA_REMOVED) ? -INFINITY : raw * XA_LOG2E;
+}
+// A fragment read from memory in front of a loop that has loads in flight: waited for here, or the compiler, which cannot tell the first round from the others,
+// waits for every load of the loop in front of the fragment's first use (one tile's whole latency in each round: 2 x 2048 x 4096, 16 heads, forward
+// XXF us instead of 112)
+template <typename F, int N> __device__ __forceinline__ void xa_arrived(F (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
 }
 
 // Staging of TT rows x D of two tensors by NT threads, through registers.  A thread's chunks lie at the same 32-bit offsets from the tile's first row in every
@@ -195,14 +202,12 @@ template <typename T, int D, int NT, bool PACKED> struct XaStage {
       }
     }
   }
-  // mask: the key mask's row, or null
-  __device__ __forceinline__ void store(char* lx, char* ly, int tt, const float* mask) {
-    const int row0 = tt * C::TT;
-    if (mask || row0 + C::TT > limit) {                           // (uniform)
+  // fix (uniform): some row of the tile takes no part; bit r of part: row r does
+  __device__ __forceinline__ void store(char* lx, char* ly, bool fix, unsigned long long part) {
+    if (fix) {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const int r = row0 + (t + n * NT) / C::CPR;
-        const bool keep = r < limit && !(mask && mask[min(r, limit - 1)] <= XA_REMOVED);
+        const bool keep = (part >> ((t + n * NT) / C::CPR)) & 1;
         if (!keep) { x[n] = u32x4{0, 0, 0, 0}; y[n] = u32x4{0, 0, 0, 0}; }
       }
     }
@@ -353,20 +358,18 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
   float m = -INFINITY, l = 0.f;
   XaStage<T, D, NS * 64, false> st;
   st.init(a, a.k, a.v, b, kvh, len, t);
-  const float* kmask = a.kmask ? a.kmask + b * a.kmask_sb : nullptr;
-  float bias = 0.f; uint32_t hash = 0;
+  float raw = 0.f;                                                // (in every wave: it clears its own rows by it)
   auto fetch = [&](int tt) __attribute__((always_inline)) {
     st.load(a, a.k, a.v, tt);
-    if (t < C::TT) {
-      bias = xa_key_bias(a, b, tt * C::TT + t, len);
-      if (DROP) hash = attn_line_hash(seed, bh, tt * C::TT + t, UC2_ATTN_SALT_K);
-    }
+    raw = xa_key_raw(a, b, tt * C::TT + (lane & (C::TT - 1)), len);
   };
   auto put = [&](int tt, int buf) __attribute__((always_inline)) {
-    st.store(lk[buf], lv[buf], tt, kmask);
-    if (t < C::TT) { lb[buf][t] = bias; if (DROP) lh[buf][t] = hash; }
+    const float bias = xa_key_bias(a, raw, tt * C::TT + (lane & (C::TT - 1)), len);
+    st.store(lk[buf], lv[buf], a.kmask != nullptr || (tt + 1) * C::TT > len, __ballot(bias != -INFINITY));
+    if (t < C::TT) { lb[buf][t] = bias; if (DROP) lh[buf][t] = attn_line_hash(seed, bh, tt * C::TT + t, UC2_ATTN_SALT_K); }
   };
   if (t0 < t1) { fetch(t0); put(t0, 0); }
+  xa_arrived(q);
   __syncthreads();
   int buf = 0;
   for (int tt = t0; tt < t1; ++tt) {
@@ -541,20 +544,19 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
     for (int e = 0; e < 16; ++e) dq[db][e] = 0.f;
   XaStage<T, D, NS * 64, false> st;
   st.init(a, a.k, a.v, b, kvh, len, t);
-  const float* kmask = a.kmask ? a.kmask + b * a.kmask_sb : nullptr;
-  float bias = 0.f; uint32_t hash = 0;
+  float raw = 0.f;                                                // (in every wave: it clears its own rows by it)
   auto fetch = [&](int tt) __attribute__((always_inline)) {
     st.load(a, a.k, a.v, tt);
-    if (t < C::TT) {
-      bias = xa_key_bias(a, b, tt * C::TT + t, len);
-      if (DROP) hash = attn_line_hash(seed, bh, tt * C::TT + t, UC2_ATTN_SALT_K);
-    }
+    raw = xa_key_raw(a, b, tt * C::TT + (lane & (C::TT - 1)), len);
   };
   auto put = [&](int tt, int buf) __attribute__((always_inline)) {
-    st.store(sh.x[buf], sh.y[buf], tt, kmask);
-    if (t < C::TT) { sh.s[buf][t] = bias; if (DROP) sh.h[buf][t] = hash; }
+    const float bias = xa_key_bias(a, raw, tt * C::TT + (lane & (C::TT - 1)), len);
+    st.store(sh.x[buf], sh.y[buf], a.kmask != nullptr || (tt + 1) * C::TT > len, __ballot(bias != -INFINITY));
+    if (t < C::TT) { sh.s[buf][t] = bias; if (DROP) sh.h[buf][t] = attn_line_hash(seed, bh, tt * C::TT + t, UC2_ATTN_SALT_K); }
   };
   if (t0 < t1) { fetch(t0); put(t0, 0); }
+  xa_arrived(q);
+  xa_arrived(go);
   __syncthreads();
   int buf = 0;
   for (int tt = t0; tt < t1; ++tt) {
@@ -605,7 +607,7 @@ __device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DRO
   const int t = threadIdx.x, lane = t & 63, w = t >> 6, b = bh / a.nkv, kvh = bh - b * a.nkv;
   const int key = (tile * NS + w) * 32 + (lane & 31);
   const int len = xa_len(a, b);
-  const float bias = xa_key_bias(a, b, key, len);
+  const float bias = len > 0 ? xa_key_bias(a, xa_key_raw(a, b, key, len), key, len) : -INFINITY;
   const bool part = bias != -INFINITY, live = (tile * NS + w) * 32 < len;      // live: the wave has a key
   const int nt = tile * NS * 32 < len ? (a.R + C::TT - 1) / C::TT : 0;          // a tile behind the length: zeros
   const int per = (nt + a.dkv.splits - 1) / a.dkv.splits;
@@ -625,27 +627,27 @@ __device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DRO
   st.init(a, a.q, a.dout, b, kvh, a.R, t);
   XaDelta<T, D, NS * 64> dl8;
   if (!PRE) dl8.init(a, bh, b, kvh, t);
-  float lse = 0.f, delta = 0.f; uint32_t hash = 0;
+  float lse = 0.f, delta = 0.f;
   auto fetch = [&](int tt) __attribute__((always_inline)) {
     st.load(a, a.q, a.dout, tt);
     if (!PRE) dl8.load(a, tt);
-    if (t < C::TT) {
-      const int r = tt * C::TT + t;
-      if (PRE) delta = a.delta[(size_t)bh * a.R + min(r, a.R - 1)];
-      lse = INFINITY;                                              // behind the last row, and rows without any key: p = 0
-      if (r < a.R) {
-        lse = a.lse[(size_t)bh * a.R + r];
-        if (lse == -INFINITY) lse = INFINITY;
-        if (DROP) { int i, g; xa_split(a, r, i, g); hash = attn_line_hash(seed, b * a.nh + kvh * a.G + g, i, UC2_ATTN_SALT_Q); }
-      }
-    }
+    const size_t at = (size_t)bh * a.R + min(tt * C::TT + (lane & (C::TT - 1)), a.R - 1);
+    lse = a.lse[at];
+    if (PRE) delta = a.delta[at];
   };
   auto put = [&](int tt, int buf) __attribute__((always_inline)) {
-    st.store(sh.x[buf], sh.y[buf], tt, nullptr);
+    st.store(sh.x[buf], sh.y[buf], (tt + 1) * C::TT > a.R, (1ull << min(63, a.R - tt * C::TT)) - 1);      // (fewer rows than a tile's 32 or 64)
     if (!PRE) dl8.store(a, st.y, sh.d[buf], tt);
-    if (t < C::TT) { sh.s[buf][t] = -lse; if (PRE) sh.d[buf][t] = tt * C::TT + t < a.R ? -delta : 0.f; if (DROP) sh.h[buf][t] = hash; }
+    const int r = tt * C::TT + t;
+    if (t < C::TT) {
+      sh.s[buf][t] = r >= a.R || lse == -INFINITY ? -INFINITY : -lse;      // behind the last row, and rows without any key: p = 0
+      if (PRE) sh.d[buf][t] = r < a.R ? -delta : 0.f;
+      if (DROP && r < a.R) { int i, g; xa_split(a, r, i, g); sh.h[buf][t] = attn_line_hash(seed, b * a.nh + kvh * a.G + g, i, UC2_ATTN_SALT_Q); }
+    }
   };
   if (t0 < t1) { fetch(t0); put(t0, 0); }
+  xa_arrived(kf);
+  xa_arrived(vf);
   __syncthreads();
   int buf = 0;
   for (int tt = t0; tt < t1; ++tt) {
