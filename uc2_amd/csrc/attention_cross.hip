@@ -82,23 +82,32 @@ template <int D> struct XaMma<bf16, D> {
     return acc;
   }
   // out[db] (head dimension x owned columns) += tile rows^T x w[16] (the accumulator order of rows())
-  static __device__ __forceinline__ void cols(const char* lds, int blk, const float (&w)[16], f32x16 (&out)[C::DB], int lane) {
+  typedef bf16x8 Turned[C::DB];                                   // 16 rows of the tile, transposed
+  static __device__ __forceinline__ void turn(const char* lds, int blk, int ks, Turned& a, int lane) {
     const int h = lane >> 5, i = lane & 15, dh = (lane >> 4) & 1;
+    const int row0 = blk * 32 + 16 * ks + 4 * h + (i >> 2), row1 = row0 + 8;
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db) {
+      const int c = 4 * db + 2 * dh + ((i >> 1) & 1), sub = (i & 1) * 8;
+      typedef __attribute__((address_space(3))) short4v* lp;
+      const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + row0 * C::RB + ((c ^ xa_swz<C::CPR>(row0)) << 4) + sub));
+      const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + row1 * C::RB + ((c ^ xa_swz<C::CPR>(row1)) << 4) + sub));
+      a[db] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+  static __device__ __forceinline__ void cols(const Turned& a, int ks, const float (&w)[16], f32x16 (&out)[C::DB]) {
+    bf16x8 b;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = (bf16)w[8 * ks + j];
+#pragma unroll
+    for (int db = 0; db < C::DB; ++db) out[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[db], b, out[db], 0, 0, 0);
+  }
+  static __device__ __forceinline__ void cols(const char* lds, int blk, const float (&w)[16], f32x16 (&out)[C::DB], int lane) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      bf16x8 b;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) b[j] = (bf16)w[8 * ks + j];
-      const int row0 = blk * 32 + 16 * ks + 4 * h + (i >> 2), row1 = row0 + 8;
-#pragma unroll
-      for (int db = 0; db < C::DB; ++db) {
-        const int c = 4 * db + 2 * dh + ((i >> 1) & 1), sub = (i & 1) * 8;
-        typedef __attribute__((address_space(3))) short4v* lp;
-        const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + row0 * C::RB + ((c ^ xa_swz<C::CPR>(row0)) << 4) + sub));
-        const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + row1 * C::RB + ((c ^ xa_swz<C::CPR>(row1)) << 4) + sub));
-        const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        out[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, out[db], 0, 0, 0);
-      }
+      Turned a;
+      turn(lds, blk, ks, a, lane);
+      cols(a, ks, w, out);
     }
   }
 };
@@ -147,8 +156,7 @@ __device__ __forceinline__ float xa_key_bias(const XaArgs& a, float raw, int key
   return key >= len || (a.kmask && raw <= XA_REMOVED) ? -INFINITY : raw * XA_LOG2E;
 }
 // A fragment read from memory in front of a loop that has loads in flight: waited for here, or the compiler, which cannot tell the first round from the others,
-// waits for every load of the loop in front of the fragment's first use (one tile's whole latency in each round: 2 x 2048 x 4096, 16 heads, forward
-// XXF us instead of 112)
+// waits for every load of the loop in front of the fragment's first use (2048 x 4096, 16 heads of 128, forward: 138 us, so 123)
 template <typename F, int N> __device__ __forceinline__ void xa_arrived(F (&f)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
@@ -328,6 +336,12 @@ __device__ __forceinline__ bool xa_block(const XaArgs& a, const XaSide& side, in
   split = blk - tile * side.splits;
   return bh < a.BH;
 }
+// over the wave's two halves
+__device__ __forceinline__ float xa_max2(float x) {
+  typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
+  const u32x2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
 __device__ __forceinline__ int xa_len(const XaArgs& a, int b) { return a.klens ? max(0, min(a.klens[b], a.Lk)) : a.Lk; }
 
 template <typename T, int D, int NS, bool DROP>
@@ -374,35 +388,12 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
   int buf = 0;
   for (int tt = t0; tt < t1; ++tt) {
     if (tt + 1 < t1) fetch(tt + 1);
-    if (live) {
-    f32x16 s[C::NB];
-    const int left = len - tt * C::TT;                            // keys from this tile on: a block of 32 behind them is not computed
-#pragma unroll
-    for (int n = 0; n < C::NB; ++n) if (n == 0 || n * 32 < left) s[n] = M::rows(lk[buf], n, q, lane);
-    // the tile's maximum of x = scale2 s (+ mask), in base 2
     const bool masked = a.kmask != nullptr || (tt + 1) * C::TT > len || a.scale2 < 0.f;      // (uniform)
-    float mx = -INFINITY;
-    if (masked) {
-#pragma unroll
-      for (int n = 0; n < C::NB; ++n)
-        if (n == 0 || n * 32 < left)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const f32x4 bv = *reinterpret_cast<const f32x4*>(&lb[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { s[n][4 * k + e] = fmaf(s[n][4 * k + e], a.scale2, bv[e]); mx = fmaxf(mx, s[n][4 * k + e]); }
-        }
-    } else {
-#pragma unroll
-      for (int n = 0; n < C::NB; ++n)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[n][e]);
-      mx *= a.scale2;
-    }
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
     // m is the maximum the weights are taken against: brought up only once a row's has grown by 2^8 (weights up to 256 lose nothing in fp32 or bf16,
     // and the output and sum are rescaled in the first tiles only)
-    if (__any(mx > m + 8.f)) {
+    auto raise = [&](float mx) __attribute__((always_inline)) {
+      mx = xa_max2(mx);
+      if (!__any(mx > m + 8.f)) return;
       const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       l *= al;
 #pragma unroll
@@ -410,12 +401,8 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[db][e] *= al;
       m = mn;
-    }
-    const float mu = m == -INFINITY ? 0.f : m, sc = masked ? 1.f : a.scale2;
-#pragma unroll
-    for (int n = 0; n < C::NB; ++n) {
-      if (n > 0 && n * 32 >= left) break;
-      float p[16];
+    };
+    auto weigh = [&](int n, const f32x16& s, float sc, float mu, float (&p)[16]) __attribute__((always_inline)) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint4 hk = {0, 0, 0, 0};
@@ -423,13 +410,67 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
         const uint32_t hh[4] = {hk.x, hk.y, hk.z, hk.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float v = __builtin_amdgcn_exp2f(fmaf(s[n][4 * k + e], sc, -mu));
+          const float v = __builtin_amdgcn_exp2f(fmaf(s[4 * k + e], sc, -mu));
           l += v;
           p[4 * k + e] = DROP ? (attn_keep(hq, hh[e], a.thresh) ? v * a.keep_scale : 0.f) : v;
         }
       }
-      M::cols(lv[buf], n, p, o, lane);
-    }
+    };
+    if (live && !masked && sizeof(T) == 2) {
+      if constexpr (sizeof(T) == 2) {
+        // a whole tile: its LDS reads issued in front of what waits for them, the values' during the first product (2 x 2048 x 4096, 16 heads: 112 -> 106 us)
+        f32x16 s[C::NB];
+        typename M::Turned v[C::NB][2];
+#pragma unroll
+        for (int n = 0; n < C::NB; ++n) s[n] = M::rows(lk[buf], n, q, lane);
+#pragma unroll
+        for (int n = 0; n < C::NB; ++n) { M::turn(lv[buf], n, 0, v[n][0], lane); M::turn(lv[buf], n, 1, v[n][1], lane); }
+        __builtin_amdgcn_sched_group_barrier(0x100, C::NB * C::KS, 0);
+#pragma unroll
+        for (int i = 0; i < C::NB * C::KS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, C::NB * C::DB * 4 / (C::NB * C::KS), 0);
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[n][e]);
+        raise(mx * a.scale2);
+        const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int n = 0; n < C::NB; ++n) {
+          float p[16];
+          weigh(n, s[n], a.scale2, mu, p);
+          M::cols(v[n][0], 0, p, o);
+          M::cols(v[n][1], 1, p, o);
+        }
+      }
+    } else if (live) {
+      f32x16 s[C::NB];
+      const int left = len - tt * C::TT;                          // keys from this tile on: a block of 32 behind them is not computed
+      float mx = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < C::NB; ++n) {
+        if (n > 0 && n * 32 >= left) break;
+        s[n] = M::rows(lk[buf], n, q, lane);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {                             // x = scale2 s + mask, in base 2
+          f32x4 bv = {0.f, 0.f, 0.f, 0.f};
+          if (masked) bv = *reinterpret_cast<const f32x4*>(&lb[buf][n * 32 + 8 * k + 4 * (lane >> 5)]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { s[n][4 * k + e] = fmaf(s[n][4 * k + e], a.scale2, bv[e]); mx = fmaxf(mx, s[n][4 * k + e]); }
+        }
+      }
+      raise(mx);
+      const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int n = 0; n < C::NB; ++n) {
+        if (n > 0 && n * 32 >= left) break;
+        float p[16];
+        weigh(n, s[n], 1.f, mu, p);
+        M::cols(lv[buf], n, p, o, lane);
+      }
     }
     if (tt + 1 < t1) put(tt + 1, buf ^ 1);
     __syncthreads();
