@@ -114,6 +114,7 @@ template <int D> struct XaMma<bf16, D> {
 template <int D> struct XaMma<float, D> {
   typedef XaCfg<float, D> C;
   typedef f32x4 Frag;
+  struct Turned {};                                               // (read value by value)
   static __device__ __forceinline__ f32x16 rows(const char* lds, int blk, const Frag (&own)[C::KS], int lane, f32x16 acc = xa_zero()) {
     const int row = blk * 32 + (lane & 31), h = lane >> 5, sw = xa_swz<C::CPR>(row);
 #pragma unroll
@@ -137,6 +138,20 @@ template <int D> struct XaMma<float, D> {
     }
   }
 };
+
+template <typename T, int D> __device__ __forceinline__ void xa_turn(const char* lds, int blk, typename XaMma<T, D>::Turned (&a)[2], int lane) {
+  XaMma<T, D>::turn(lds, blk, 0, a[0], lane);
+  XaMma<T, D>::turn(lds, blk, 1, a[1], lane);
+}
+// the order of a block's start: READS reads of LDS, then PRODUCTS matrix instructions with MORE reads (for the second products) between them
+template <int READS, int PRODUCTS, int MORE> __device__ __forceinline__ void xa_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+  for (int i = 0; i < PRODUCTS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, (MORE + PRODUCTS - 1) / PRODUCTS, 0);
+  }
+}
 
 // position of packed row r: (query i, head g of the group)
 __device__ __forceinline__ void xa_split(const XaArgs& a, int r, int& i, int& g) {
@@ -424,13 +439,8 @@ __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
 #pragma unroll
         for (int n = 0; n < C::NB; ++n) s[n] = M::rows(lk[buf], n, q, lane);
 #pragma unroll
-        for (int n = 0; n < C::NB; ++n) { M::turn(lv[buf], n, 0, v[n][0], lane); M::turn(lv[buf], n, 1, v[n][1], lane); }
-        __builtin_amdgcn_sched_group_barrier(0x100, C::NB * C::KS, 0);
-#pragma unroll
-        for (int i = 0; i < C::NB * C::KS; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, C::NB * C::DB * 4 / (C::NB * C::KS), 0);
-        }
+        for (int n = 0; n < C::NB; ++n) xa_turn<T, D>(lv[buf], n, v[n], lane);
+        xa_ahead<C::NB * C::KS, C::NB * C::KS, C::NB * C::DB * 4>();
         float mx = -INFINITY;
 #pragma unroll
         for (int n = 0; n < C::NB; ++n)
@@ -578,6 +588,7 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
   }
   const float nlse = -lse;
   const f32x16 ndelta = xa_all(DROP ? 0.f : -delta);              // dp's sums start at -delta (dropout scales dp first)
+  constexpr bool AHEAD = sizeof(T) == 2 && !DROP;
   f32x16 dq[C::DB];
 #pragma unroll
   for (int db = 0; db < C::DB; ++db)
@@ -608,6 +619,11 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
       if (!live || tt * C::TT + n * 32 >= len) break;
       const f32x16 s = M::rows(sh.x[buf], n, q, lane);
       const f32x16 dp = M::rows(sh.y[buf], n, go, lane, ndelta);
+      typename M::Turned tx[2];
+      if constexpr (AHEAD) {
+        xa_turn<T, D>(sh.x[buf], n, tx, lane);
+        xa_ahead<2 * C::KS, 2 * C::KS, 8 * C::DB>();
+      }
       float ds[16];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -622,7 +638,8 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
           ds[4 * k + e] = p * (DROP ? (attn_keep(hq, hh[e], a.thresh) ? dp[4 * k + e] * a.keep_scale : 0.f) - delta : dp[4 * k + e]);
         }
       }
-      M::cols(sh.x[buf], n, ds, dq, lane);
+      if constexpr (AHEAD) { M::cols(tx[0], 0, ds, dq); M::cols(tx[1], 1, ds, dq); }
+      else M::cols(sh.x[buf], n, ds, dq, lane);
     }
     if (tt + 1 < t1) put(tt + 1, buf ^ 1);
     __syncthreads();
