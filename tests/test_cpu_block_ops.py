@@ -117,7 +117,7 @@ def test_linear_wgrad_argument_errors():
 def test_a_leaf_remembers_the_stream_of_its_first_graph(monkeypatch):
     """note_leaves and refuse_foreign_capture on the streams and captures they are told of"""
     from uc2_amd.ops.base import note_leaves, once
-    now = [1, False]
+    now = [0, False]                                       # (0: the default stream)
     monkeypatch.setattr(_lib, "stream", lambda: now[0])
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[1])
 
@@ -145,6 +145,12 @@ def test_a_leaf_remembers_the_stream_of_its_first_graph(monkeypatch):
     now[1] = True
     x.grad = y.grad = None
     Twice.apply(x, y).sum().backward()                     # a graph of its own
+    x.grad = y.grad = None
+    now[:] = [5, False]
+    warm = Twice.apply(x, y)                               # a warm-up on another stream, whose outputs are kept
+    now[:] = [7, True]
+    Twice.apply(x, y).sum().backward()
+    del warm
     assert bool((x.grad == 1).all()) and bool((y.grad == 2).all())
 
 

@@ -83,7 +83,8 @@ def test_quantize_strided_rows():
 # ---- product --------------------------------------------------------------------------------------------------------------------
 GEMM_SIZES = [(1, 1, 1), (1, 1024, 4096), (8, 4096, 1024), (16, 17, 128), (17, 130, 256), (33, 1000, 300), (64, 255, 1024), (65, 129, 640),
               (128, 128, 128), (200, 777, 1000), (256, 256, 512), (512, 768, 768), (1030, 516, 384), (2048, 2304, 768), (1024, 1024, 1152),
-              (4096, 2304, 768), (8300, 1100, 512), (33000, 256, 256), (4200, 2304, 1000), (4096, 2304, 1152)]
+              (4096, 2304, 768), (8300, 1100, 512), (33000, 256, 256), (4200, 2304, 1000), (4096, 2304, 1152),
+              (4096, 2048, 4096), (4100, 2310, 3840)]                     # (scales of more than 28 blocks)
 
 
 @pytest.mark.parametrize("M,N,K", GEMM_SIZES)
@@ -152,10 +153,10 @@ def test_linear_block_forward_and_gradients(M, N, K, wtype):
     R.assert_within(db, dy.double().sum(0), M * R.U[F32] * dy.double().abs().sum(0) + 1e-30, "db")
 
 
-def wgrad(M, N, K, dy, x, bias=True, lddw=None):
+def wgrad(M, N, K, dy, x, bias=True, lddw=None, off=0):
     """uc2_linear_wgrad on rows dy [M, N] and x [M, K] of any stride -> (dw [N, K], db)"""
     lddw = lddw or K
-    dw = torch.full((N, lddw), 7.0, device=DEV)
+    dw = torch.full((N * lddw + off,), 7.0, device=DEV)[off:].view(N, lddw)
     db = torch.empty(N, device=DEV) if bias else None
     n = _lib.load().uc2_linear_wgrad_workspace(M, N, K)
     ws = torch.empty(n, dtype=torch.uint8, device=DEV)
@@ -177,6 +178,25 @@ def test_linear_wgrad(M, N, K, odd):
     again, db2 = wgrad(M, N, K, dy, x)
     assert torch.equal(again, dw) and torch.equal(db2, db)
     assert torch.equal(wgrad(M, N, K, dy, x, False)[0], dw)
+
+
+def test_linear_wgrad_into_a_result_of_any_alignment():
+    M, N, K = 1280, 512, 256                                     # (whole tiles)
+    dy, x = normal((M, N), 1, BF16), normal((M, K), 2, BF16)
+    want, mag = R.mm(dy.double().t(), x.double()), R.mm(dy.double().abs().t(), x.double().abs())
+    for off in (0, 1, 2):
+        R.assert_within(wgrad(M, N, K, dy, x, off=off)[0], want, 2 * M * R.U[F32] * mag, "off by %d" % off)
+
+
+@pytest.mark.parametrize("M,N", [(1, 1), (300, 5), (5000, 777), (9000, 2304)])
+def test_linear_block_bias_gradient_alone(M, N):
+    """a bias that is trained beside a weight that is not: in a fixed order too"""
+    x, w, dy = normal((M, 64), 1, BF16), normal((N, 64), 2), normal((M, N), 3, BF16)
+    b = torch.zeros(N, device=DEV, requires_grad=True)
+    db, = torch.autograd.grad(ops.linear_fp8_block(x, w, b), [b], dy)
+    R.assert_within(db, dy.double().sum(0), M * R.U[F32] * dy.double().abs().sum(0) + 1e-30, "db")
+    for _ in range(3):
+        assert torch.equal(torch.autograd.grad(ops.linear_fp8_block(x, w, b), [b], dy)[0], db)
 
 
 def test_linear_wgrad_nan_stays_in_its_row_and_column():
@@ -502,6 +522,17 @@ def test_cross_attention_dropout(dtype, B, Lq, Lk):
     b = ops.cross_attention(q, k, v, drop_p=p)
     ops.rng.manual_seed(5)
     assert torch.equal(a, ops.cross_attention(q, k, v, drop_p=p)) and not torch.equal(a, b)
+
+
+def test_cross_attention_dropout_sites_and_expanded_masks():
+    q, k, v, _ = attn_inputs(3, 20, 50, 4, 2, 64, BF16)
+    with ops.rng.scope():
+        a, b, c = (ops.cross_attention(q, k, v, drop_p=0.3, site=s) for s in (1, 2, 1))
+    assert torch.equal(a, c) and not torch.equal(a, b)
+    mask = normal((1, 1, 1, 50), 9)
+    want = ops.cross_attention(q, k, v, key_mask=mask.expand(3, 1, 1, 50).contiguous())
+    assert torch.equal(ops.cross_attention(q, k, v, key_mask=mask.expand(3, 1, 1, 50)), want)
+    assert torch.equal(ops.cross_attention(q, k, v, key_mask=mask[0, 0].expand(3, 50).t().contiguous().t()), want)
 
 
 # ---- streams, graphs, together --------------------------------------------------------------------------------------------------

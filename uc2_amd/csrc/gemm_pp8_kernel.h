@@ -10,10 +10,11 @@
 #define PP16_AUX_TOUCH 1     // touch the lines of the epilogue's aux_in tile two k-tiles ahead (residual-add / gelu'-multiply / dGELU kinds)
 #endif
 // BLK: block scales (fp8_block.h) instead of the tensors' two: a k-tile of 128 bytes is one block, the matrix instruction takes the exponent bytes of
-// the lane's row and of the wave's 64 columns (one weight block).  The scales of 28 k-tiles wait in the wave's own transposition buffer, which only the epilogue uses: fetched by LDS-DMA between the epilogue's last read of it and its stores, so that the wait for
-// them leaves the stores in flight; a lane reads the four bytes of a half per k-tile (beside 16 times as many operand bytes).  As plain loads into
-// registers, with the waits that hipcc puts in front of their uses, they cost half of the main loop: 8192^3 at 1858 instead of 2600 TFLOP/s.
-// More k-tiles: the buffer is filled again every 28, in the open (~1 us of ~28).
+// the lane's row and of the wave's 64 columns (one weight block).  The scales of 28 k-tiles wait in the wave's own transposition buffer, which only
+// the epilogue uses: fetched by LDS-DMA between the epilogue's last read of it and its stores, so that the wait for them leaves the stores in flight;
+// a lane reads the four bytes of a half per k-tile (beside 16 times as many operand bytes).  8192^3: 2715 TFLOP/s, 3015 with per-tensor scales;
+// as plain loads into registers, with the waits that hipcc puts in front of their uses, 1858.  More k-tiles: the buffer is filled again every 28,
+// in the open (~1 us of ~28).
 template <bool TA, bool TB, bool TACC, int EPI, int HI, bool QOUT = false, bool BLK = false>
 __global__ __launch_bounds__(512, 2) void gemm_fp8_pp8_kernel(GemmArgs p) {
   static_assert(HI == 2 && TACC && !TA && !TB, "256-row tiles, transposed accumulators, k-contiguous e4m3 operands");

@@ -277,7 +277,7 @@ extern "C" int uc2_linear_wgrad(int M, int N, int K, const void* dy, long long l
   a.part = (float*)ws;
   hipStream_t st = (hipStream_t)stream;
   const int whole = wgrad_whole_splits(M, N, K);
-  if (whole && (lddy & 7) == 0 && (ldx & 7) == 0 && (((uintptr_t)dy | (uintptr_t)x) & 15) == 0 && 2ull * M * lddy < (1ull << 32) && 2ull * M * ldx < (1ull << 32)) {
+  if (whole && (lddy & 7) == 0 && (ldx & 7) == 0 && (((uintptr_t)dy | (uintptr_t)x | (uintptr_t)dw) & 15) == 0 && 2ull * M * lddy < (1ull << 32) && 2ull * M * ldx < (1ull << 32)) {
     const int e = uc2_gemm(1, 1, 1, N, K, M, dy, (int)lddy, x, (int)ldx, dw, K, 1, nullptr, 0, nullptr, nullptr, 0, 1, whole, 12, ws, (size_t)whole * N * K * 4,
                            1 /* UC2_GEMM_DEFER_REDUCE */, stream);
     if (e != 0) return e;

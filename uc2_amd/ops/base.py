@@ -151,13 +151,13 @@ def note_leaves(ctx):
 
 
 def refuse_foreign_capture(ctx):
-    """A captured backward pass hands its gradients to the accumulations of its leaves.  While an eager graph of a leaf lives, that accumulation belongs
-    to the eager stream: the capture would reach over to it and end the process, so it is refused before."""
-    here = _lib.stream()
+    """A captured backward pass hands its gradients to the accumulations of its leaves.  While an eager graph of a leaf from the default stream lives, that
+    accumulation belongs to the default stream, which no capture may reach over to: torch ends the process there, so it is refused before.  (A warm-up on
+    a stream of its own leaves nothing of the kind.)"""
     for node, _ in ctx.next_functions:
-        if type(node).__name__ == "AccumulateGrad" and node.metadata.get("uc2_stream", here) != here:
-            raise _lib.Uc2Error("a backward pass cannot be captured while an eager graph of the same leaves is alive: delete its outputs first, or capture with "
-                                "leaves of its own (x.detach().requires_grad_())")
+        if type(node).__name__ == "AccumulateGrad" and node.metadata.get("uc2_stream") == 0:
+            raise _lib.Uc2Error("a backward pass cannot be captured while an eager graph of the same leaves from the default stream is alive: delete its outputs "
+                                "first, warm up on a stream of its own, or capture with leaves of its own (x.detach().requires_grad_())")
 
 
 def once(backward):

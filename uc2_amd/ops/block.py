@@ -11,7 +11,6 @@ from .. import _lib
 from .._lib import call, dt, ptr, stream
 from ..config import state
 from .base import _Timed, _require_cuda, device_guard, note_leaves, once
-from .linear import colsum_accum
 
 BLOCK = 128
 
@@ -122,6 +121,25 @@ def gemm_fp8_block(a, b, bias=None):
         return _gemm(a8, sa, b8, sb, bias)
 
 
+def _wgrad(dy2, x2, K, n, db):
+    """(dW [N, K] fp32) of uc2_linear_wgrad on the first K columns of x2, with db written if there is one; n: its workspace's bytes"""
+    M, N = dy2.shape
+    dw = dy2.new_empty((N, K), dtype=torch.float32)
+    ws = dy2.new_empty(n, dtype=torch.uint8) if n else None
+    call("uc2_linear_wgrad", M, N, K, dy2.data_ptr(), max(dy2.stride(0), N), x2.data_ptr(), max(x2.stride(0), K), dw.data_ptr(), K, ptr(db), ptr(ws), n, stream())
+    return dw
+
+
+def _column_sums(dy2):
+    """sums over the rows in a fixed order: those of the weight gradient, beside its smallest product"""
+    M, N = dy2.shape
+    if M == 0:
+        return torch.zeros(N, dtype=torch.float32, device=dy2.device)
+    db, K = dy2.new_empty(N, dtype=torch.float32), min(N, 8)
+    _wgrad(dy2, dy2, K, _lib.load().uc2_linear_wgrad_workspace(M, N, K), db)
+    return db
+
+
 class LinearBlockFp8Fn(torch.autograd.Function):
     """y = q(x) q(W)^T + b, gradients straight through the quantisation: dx = q(dy) q(W) on the transposed copy of the same weight values,
     dW = dy^T x and db = sum dy from the unquantised bf16 tensors (the weight gradient stays bf16, as in the per-tensor mode)"""
@@ -156,17 +174,13 @@ class LinearBlockFp8Fn(torch.autograd.Function):
                 if len(shp) != 2:
                     dx = dx.view(shp)
             if need_dw and M:
-                dw = dy2.new_empty((N, K), dtype=torch.float32)
                 db = dy2.new_empty(N, dtype=torch.float32) if need_db else None
-                ws = dy2.new_empty(n, dtype=torch.uint8) if n else None
-                call("uc2_linear_wgrad", M, N, K, dy2.data_ptr(), max(dy2.stride(0), N), x2.data_ptr(), max(x2.stride(0), K), dw.data_ptr(), K, ptr(db), ptr(ws), n, stream())
+                dw = _wgrad(dy2, x2, K, n, db)
             else:
                 if need_dw:
                     dw = torch.zeros((N, K), dtype=torch.float32, device=dy2.device)
                 if need_db:
-                    db = torch.zeros(N, dtype=torch.float32, device=dy2.device)
-                    if M:
-                        colsum_accum(dy2, db)
+                    db = _column_sums(dy2)
             if dw is not None and wtype != torch.float32:
                 dw = dw.to(wtype)
         return dx, dw, db
