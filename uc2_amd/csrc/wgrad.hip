@@ -2,9 +2,11 @@
 //   dW[n][k] = sum over rows m of dY[m][n] X[m][k]   (fp32),   db[n] = sum over m of dY[m][n]
 // Both operands are contracted over their ROWS: 64-row slabs go row-major into LDS (through registers: unaligned and partial columns become
 // whole zero-padded chunks on the way) and are read transposed (ds_read_b64_tr_b16) into v_mfma_f32_32x32x16_bf16, both in the same row
-// order, which is all that a contraction asks for.  128 x 128 tiles, 2 x 2 waves.  The rows are split over workgroups until the chip is full; the parts
+// order, which is all that a contraction asks for.  128 x 128 tiles, 2 x 2 waves: 64 KiB of LDS, two workgroups per CU.  The rows are split over workgroups until the chip is full; the parts
 // (fp32) are added in split order by a second kernel: no atomics, the same bits every run.  The workgroups of the first column of tiles also
 // add up the dY values they stage anyway.
+// Bound by the matrix instructions and the parts: measured with db, 20000 x 1100 x 900 93 us (0.43 PF/s), 33280 x 4000 x 1000 480 us (0.55 PF/s); whole tiles
+// (below) 9984 x 2304 x 768 38 us and 9 for db and 14 for the sum of the parts.
 #include "../../include/uc2_hip.h"
 #include "common.h"
 #include "fp8_block.h"
