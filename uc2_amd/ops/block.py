@@ -121,12 +121,11 @@ def gemm_fp8_block(a, b, bias=None):
         return _gemm(a8, sa, b8, sb, bias)
 
 
-def _wgrad(dy2, x2, K, n, db):
-    """(dW [N, K] fp32) of uc2_linear_wgrad on the first K columns of x2, with db written if there is one; n: its workspace's bytes"""
+def _wgrad(dy2, x2, K, ws, n, db):
+    """(dW [N, K] fp32) of uc2_linear_wgrad on the first K columns of x2, with db written if there is one; n bytes of workspace at ws"""
     M, N = dy2.shape
     dw = dy2.new_empty((N, K), dtype=torch.float32)
-    ws = dy2.new_empty(n, dtype=torch.uint8) if n else None
-    call("uc2_linear_wgrad", M, N, K, dy2.data_ptr(), max(dy2.stride(0), N), x2.data_ptr(), max(x2.stride(0), K), dw.data_ptr(), K, ptr(db), ptr(ws), n, stream())
+    call("uc2_linear_wgrad", M, N, K, dy2.data_ptr(), max(dy2.stride(0), N), x2.data_ptr(), max(x2.stride(0), K), dw.data_ptr(), K, ptr(db), ws, n, stream())
     return dw
 
 
@@ -136,46 +135,78 @@ def _column_sums(dy2):
     if M == 0:
         return torch.zeros(N, dtype=torch.float32, device=dy2.device)
     db, K = dy2.new_empty(N, dtype=torch.float32), min(N, 8)
-    _wgrad(dy2, dy2, K, _lib.load().uc2_linear_wgrad_workspace(M, N, K), db)
+    n = _lib.load().uc2_linear_wgrad_workspace(M, N, K)
+    ws = dy2.new_empty(n, dtype=torch.uint8)
+    _wgrad(dy2, dy2, K, ws.data_ptr(), n, db)
     return db
+
+
+def _align(n):
+    return (n + 255) & ~255
+
+
+def _product(x2, b8, sb, N, bias, tmp, at):
+    """bf16 [M, N] = q(x2) b8^T + bias; q(x2) goes into the buffer tmp from byte `at` on (_product_bytes of it)"""
+    M, K = x2.shape
+    Kp = _up(K)
+    q = tmp.data_ptr() + at
+    qs = q + _align(M * Kp)
+    out = x2.new_empty((M, N))
+    call("uc2_fp8_quant_rows", dt(x2.dtype), M, K, x2.data_ptr(), max(x2.stride(0), K), q, qs, stream())
+    call("uc2_gemm_fp8_block", M, N, Kp, q, Kp, qs, max(M, 1), b8, Kp, sb, ptr(bias), out.data_ptr(), N, stream())
+    return out
+
+
+def _product_bytes(M, K):
+    Kp = _up(K)
+    return _align(M * Kp) + _align((Kp + 511) // 512 * M * 4)
 
 
 class LinearBlockFp8Fn(torch.autograd.Function):
     """y = q(x) q(W)^T + b, gradients straight through the quantisation: dx = q(dy) q(W) on the transposed copy of the same weight values,
-    dW = dy^T x and db = sum dy from the unquantised bf16 tensors (the weight gradient stays bf16, as in the per-tensor mode)"""
+    dW = dy^T x and db = sum dy from the unquantised bf16 tensors (the weight gradient stays bf16, as in the per-tensor mode).  What only one pass
+    needs lies in one buffer (an allocation costs 1.5 us, a small layer's forward and backward together some 120)."""
 
     @staticmethod
     def forward(ctx, x, weight, bias):
         shp = x.shape
         need_dx, need_dw = ctx.needs_input_grad[:2]
         x2, weight = _float_matrix(x, "linear_fp8_block"), _float_matrix(weight, "linear_fp8_block")
+        M, (N, K) = x2.shape[0], weight.shape
+        Np, Kp = _up(N), _up(K)
+        blocks = Np // BLOCK * (Kp // BLOCK)
         with device_guard(x2):
-            w, wt = _quant_weight(weight, True) if need_dx else (_quant_weight(weight, False), (None, None))
-            a = _quant_rows(x2)
-            y = _gemm(a.data, a.scale, w.data, w.scale, bias)
+            at = _align(N * Kp) + _align(blocks)
+            tmp = x2.new_empty(at + _product_bytes(M, K), dtype=torch.uint8)
+            wt = x2.new_empty(K * Np + blocks, dtype=torch.uint8) if need_dx else None           # W^T and its scales
+            w = tmp.data_ptr()
+            ws = w + _align(N * Kp)
+            call("uc2_fp8_quant_square", dt(weight.dtype), N, K, weight.data_ptr(), max(weight.stride(0), K), w, ws, ptr(wt), wt.data_ptr() + K * Np if need_dx else None, stream())
+            y = _product(x2, w, ws, N, bias, tmp, at)
             note_leaves(ctx)
-        ctx.save_for_backward(x2 if need_dw else None, wt[0], wt[1])
-        ctx.cfg = (shp, weight.shape, weight.dtype, _lib.load().uc2_linear_wgrad_workspace(x2.shape[0], *weight.shape) if need_dw else 0)
-        return y if len(shp) == 2 else y.view(*shp[:-1], weight.shape[0])
+        ctx.save_for_backward(x2 if need_dw else None, wt)
+        ctx.cfg = (shp, weight.shape, weight.dtype, _lib.load().uc2_linear_wgrad_workspace(M, N, K) if need_dw else 0)
+        return y if len(shp) == 2 else y.view(*shp[:-1], N)
 
     @staticmethod
     @once
     def backward(ctx, dy):
-        x2, wt, st = ctx.saved_tensors
+        x2, wt = ctx.saved_tensors
         shp, (N, K), wtype, n = ctx.cfg
         need_dx, need_dw, need_db = ctx.needs_input_grad
         dy2 = _float_matrix(dy, "linear_fp8_block")
         M = dy2.shape[0]
         dx = dw = db = None
         with device_guard(dy2):
+            at = _align(n)
+            tmp = dy2.new_empty(at + (_product_bytes(M, N) if need_dx else 0), dtype=torch.uint8)
             if need_dx:
-                a = _quant_rows(dy2)
-                dx = _gemm(a.data, a.scale, wt, st, None)
+                dx = _product(dy2, wt.data_ptr(), wt.data_ptr() + K * _up(N), K, None, tmp, at)
                 if len(shp) != 2:
                     dx = dx.view(shp)
             if need_dw and M:
                 db = dy2.new_empty(N, dtype=torch.float32) if need_db else None
-                dw = _wgrad(dy2, x2, K, n, db)
+                dw = _wgrad(dy2, x2, K, tmp.data_ptr(), n, db)
             else:
                 if need_dw:
                     dw = torch.zeros((N, K), dtype=torch.float32, device=dy2.device)
