@@ -198,7 +198,7 @@ int uc2_linear_wgrad(int M, int N, int K, const void* dy, long long lddy, const 
  *   rows contiguous, any alignment, H <= 16384.  y, rstd optional (y or q_out is given); q_out / q_scale: y as a rows operand of
  *   uc2_gemm_fp8_block, quantised from the fp32 values.
  *   backward: dx = rstd (g - h mean(g h)) + dsum, g = dy gamma, h = sum rstd -- the gradient of x and of residual alike; dsum (gradient that
- *   reaches the stream itself) may be NULL; dgamma [H] = sum over rows of dy h (written; may be NULL), in a fixed order through ws (uc2_rms_bwd_workspace). */
+ *   reaches the stream itself) may be NULL; dgamma [H] = sum over rows of dy h (written; may be NULL), in a fixed order through ws (uc2_rms_bwd_workspace bytes; 0: may be NULL). */
 int uc2_rms_fwd(int dtype, int M, int H, const void* x, const void* residual, const float* gamma, float eps, void* sum, void* y, float* rstd,
                 void* q_out, void* q_scale, void* stream);
 size_t uc2_rms_bwd_workspace(int M, int H);

@@ -92,12 +92,13 @@ def test_rms_argument_errors():
         a[i] = bad
         assert lib.uc2_rms_fwd(*a) == -1, (i, bad)
     assert lib.uc2_rms_fwd(1, 4, 128, P, None, P, 1e-6, None, None, None, None, None, None) == -1     # no output at all
-    n = lib.uc2_rms_bwd_workspace(4, 128)
-    ok = [1, 4, 128, P, P, P, P, P, P, P, P, n, None]
-    for i, bad in ((0, 5), (1, -1), (2, 16385), (3, None), (5, None), (6, None), (7, None), (8, None), (10, None), (10, P + 2), (11, n - 1)):
+    n = lib.uc2_rms_bwd_workspace(400, 128)
+    ok = [1, 400, 128, P, P, P, P, P, P, P, P, n, None]
+    for i, bad in ((0, 5), (1, -1), (2, 16385), (3, None), (5, None), (6, None), (7, None), (8, None), (9, P + 2), (10, None), (10, P + 2), (11, n - 1)):
         a = list(ok)
         a[i] = bad
         assert lib.uc2_rms_bwd(*a) == -1, (i, bad)
+    assert n > 0 and lib.uc2_rms_bwd_workspace(8, 128) == 0      # (few rows: one workgroup)
     assert lib.uc2_rms_bwd_workspace(0, 128) == 0 and lib.uc2_rms_bwd_workspace(4, 20000) == 0
 
 

@@ -303,7 +303,7 @@ class RMSNormFn(torch.autograd.Function):
             if need_dw:
                 dw = torch.empty_like(weight)
                 n = ctx.ws
-                ws = s.new_empty(n, dtype=torch.uint8)
+                ws = s.new_empty(n, dtype=torch.uint8) if n else None
             timed = _Timed("rms_bwd", s.element_size() * M * H * (3 + (ds2 is not None))) if state.hbm_timer is not None else None
             call("uc2_rms_bwd", dt(s.dtype), M, H, dy2.data_ptr(), ptr(ds2), s.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), ptr(dw), ptr(ws), n,
                  stream())
