@@ -418,6 +418,28 @@ def test_cross_attention_one_key(dtype, B, Lq, Lk, nh, nkv, D):
     assert not dk[:, 1:].any() and not dv[:, 1:].any()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Lq,Lk,nh,nkv,D", [(3, 1, 4, 4, 32), (70, 300, 4, 2, 64), (900, 40, 2, 1, 64), (2, 5000, 4, 1, 128), (600, 700, 3, 3, 32)])
+@pytest.mark.parametrize("drop", [0.0, 0.3])
+def test_cross_attention_one_key_has_no_gradient_of_its_scores(dtype, Lq, Lk, nh, nkv, D, drop):
+    """the softmax over one key is 1 whatever its score: dq and dk are zero, not what fp32 leaves of dp - delta; by length, by mask (the first key, one inside,
+    the last) and by both; sequences of two keys and more beside them keep their gradients"""
+    at = [0, Lk // 2, Lk - 1]
+    B = len(at) + 2
+    q, k, v, dout = attn_inputs(B, Lq, Lk, nh, nkv, D, dtype)
+    mask = torch.full((B, Lk), -math.inf, device=DEV)
+    for b, j in enumerate(at):
+        mask[b, j] = 0.5
+    mask[3, :2] = mask[4, :2] = 0.0
+    lens = torch.tensor([Lk, Lk, Lk, 1, Lk], device=DEV, dtype=torch.int32)
+    torch.manual_seed(0), ops.rng.manual_seed(3)
+    for kw in (dict(key_mask=mask, k_lens=lens), dict(k_lens=torch.tensor([1, 1, 1, 1, min(2, Lk)], device=DEV))):
+        o, dq, dk, dv = run_attn(q, k, v, dout, drop_p=drop, **kw)
+        assert not dq[:4].any() and not dk[:4].any() and o[:4].any() and dv[:4].any()
+        # one or two keys: a query's gradient of two is lost only if dropout takes both
+        assert Lk < 2 or bool(dq[4].any()) and bool(dk[4, :2].any())
+
+
 def test_cross_attention_views():
     """heads before positions, fused projections, expanded keys, unaligned slices (copied), a gradient that is a broadcast"""
     B, Lq, Lk, nh, D = 2, 19, 70, 4, 64

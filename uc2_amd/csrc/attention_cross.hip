@@ -310,7 +310,7 @@ __device__ __forceinline__ void xa_own(const XaArgs& a, const XaView& X, int b, 
 }
 // delta[r] = dout . out of an owned row, with the output as it was before its rounding to bf16: a row's gradients of the scores, p (dp - delta), nearly
 // cancel where it has few keys or one that outweighs the others, and an output off by 2^-9 there left dq and dk off by 4e-3 to 8e-3 of their norm
-// (2 to 40 keys; with this 2.5e-3, what the roundings of the score gradients and of the result make; one key: 2^-24 in place of 2^-9 of dout . out)
+// (2 to 40 keys; with this 2.5e-3, what the roundings of the score gradients and of the result make)
 template <typename T, int D>
 __device__ __forceinline__ float xa_delta_row(const XaArgs& a, int bh, int b, int kvh, int r, bool take, int lane, const typename XaMma<T, D>::Frag (&go)[XaCfg<T, D>::KS]) {
   constexpr int E = 16 / sizeof(T);
@@ -364,6 +364,15 @@ __device__ __forceinline__ float xa_max2(float x) {
   return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
 }
 __device__ __forceinline__ int xa_len(const XaArgs& a, int b) { return a.klens ? max(0, min(a.klens[b], a.Lk)) : a.Lk; }
+// Whether just one key of the sequence takes part.  The softmax over one key is constant, so dq and dk are zero; p (dp - delta) would leave fp32's rounding
+// noise there, dp and delta being sums of the same products in two orders.  Their last factor, the scale, is zero then (NaN stays NaN).  seen: the keys
+// that the wave has met (two: nothing is read; otherwise the mask is, up to its second key).
+__device__ __forceinline__ bool xa_alone(const XaArgs& a, int b, int len, int lane, int seen) {
+  if (!a.kmask) return len == 1;
+  int n = seen < 2 ? 0 : seen;
+  for (int j0 = 0; n < 2 && j0 < len; j0 += 64) n += __popcll(__ballot(j0 + lane < len && !(xa_key_raw(a, b, j0 + lane, len) <= XA_REMOVED)));
+  return n == 1;
+}
 
 template <typename T, int D, int NS, bool DROP>
 __global__ __launch_bounds__(NS * 64) void xattn_fwd_kernel(XaArgs a) {
@@ -567,7 +576,7 @@ template <typename T, int D, bool DROP> struct XaLds {
 };
 
 // dQ (owned query rows, streamed keys)
-//   dx = p (dp - delta),  dp = dout v^T (dropped as the forward's weights were),  dq = scale dx k
+//   dx = p (dp - delta),  dp = dout v^T (dropped as the forward's weights were),  dq = scale dx k  (zero where one key takes part: xa_alone)
 template <typename T, int D, int NS, bool DROP, bool PRE>
 __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP>& sh) {
   typedef XaCfg<T, D> C;
@@ -603,13 +612,16 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
   XaStage<T, D, NS * 64, false> st;
   st.init(a, a.k, a.v, b, kvh, len, t);
   float raw = 0.f;                                                // (in every wave: it clears its own rows by it)
+  int seen = 0;                                                   // keys of the split that take part
   auto fetch = [&](int tt) __attribute__((always_inline)) {
     st.load(a, a.k, a.v, tt);
     raw = xa_key_raw(a, b, tt * C::TT + (lane & (C::TT - 1)), len);
   };
   auto put = [&](int tt, int buf) __attribute__((always_inline)) {
     const float bias = xa_key_bias(a, raw, tt * C::TT + (lane & (C::TT - 1)), len);
-    st.store(sh.x[buf], sh.y[buf], a.kmask != nullptr || (tt + 1) * C::TT > len, __ballot(bias != -INFINITY));
+    const unsigned long long take = __ballot(bias != -INFINITY);
+    seen += __popcll(take << (64 - C::TT));
+    st.store(sh.x[buf], sh.y[buf], a.kmask != nullptr || (tt + 1) * C::TT > len, take);
     if (t < C::TT) { sh.s[buf][t] = bias; if (DROP) sh.h[buf][t] = attn_line_hash(seed, bh, tt * C::TT + t, UC2_ATTN_SALT_K); }
   };
   if (t0 < t1) { fetch(t0); put(t0, 0); }
@@ -651,13 +663,14 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
     __syncthreads();
     buf ^= 1;
   }
+  const float scale = xa_alone(a, b, len, lane, seen) ? 0.f : a.scale;
   if (!mine) return;
   if (a.dq.splits == 1) {
     int i, g;
     xa_split(a, r, i, g);
-    xa_put_row<T, C::DB>(a.gq.p + b * a.gq.sb + (long long)i * a.gq.sl + (long long)(kvh * a.G + g) * a.gq.sh, dq, a.scale, lane);
+    xa_put_row<T, C::DB>(a.gq.p + b * a.gq.sb + (long long)i * a.gq.sl + (long long)(kvh * a.G + g) * a.gq.sh, dq, scale, lane);
   } else {
-    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.dq.part + (((size_t)split * a.BH + bh) * a.R + r) * D), dq, a.scale, lane);
+    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.dq.part + (((size_t)split * a.BH + bh) * a.R + r) * D), dq, scale, lane);
   }
 }
 
@@ -766,6 +779,7 @@ __device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DRO
     __syncthreads();
     buf ^= 1;
   }
+  const float scale = xa_alone(a, b, len, lane, __popcll(__ballot(part && lane < 32))) ? 0.f : a.scale;
   if (key >= a.Lk) return;
   if (!part) {                                                     // (without a mask its column was computed: on zero vectors, into this lane alone)
 #pragma unroll
@@ -774,11 +788,11 @@ __device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DRO
       for (int e = 0; e < 16; ++e) { dk[db][e] = 0.f; dv[db][e] = 0.f; }
   }
   if (a.dkv.splits == 1) {
-    xa_put_row<T, C::DB>(a.gk.p + b * a.gk.sb + (long long)key * a.gk.sl + kvh * a.gk.sh, dk, a.scale, lane);
+    xa_put_row<T, C::DB>(a.gk.p + b * a.gk.sb + (long long)key * a.gk.sl + kvh * a.gk.sh, dk, scale, lane);
     xa_put_row<T, C::DB>(a.gv.p + b * a.gv.sb + (long long)key * a.gv.sl + kvh * a.gv.sh, dv, 1.0f, lane);
   } else {
     const size_t n = (size_t)a.BH * a.Lk, row = (size_t)bh * a.Lk + key;
-    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.dkv.part + (split * 2 * n + row) * D), dk, a.scale, lane);
+    xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.dkv.part + (split * 2 * n + row) * D), dk, scale, lane);
     xa_put_row<float, C::DB>(reinterpret_cast<char*>(a.dkv.part + ((split * 2 + 1) * n + row) * D), dv, 1.0f, lane);
   }
 }
