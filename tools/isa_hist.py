@@ -1,5 +1,5 @@
 """instruction histogram of one kernel of a gfx950 assembly dump (how profiles/r04_experiments.md sections 8-11 counted):
-    hipcc --offload-arch=gfx950 -O3 -std=c++17 [-mllvm -amdgpu-mfma-vgpr-form] -S --cuda-device-only uc2_amd/csrc/<file>.hip -o scratch/isa/<file>.s
+    hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops [-mllvm -amdgpu-mfma-vgpr-form] -S --cuda-device-only uc2_amd/csrc/<file>.hip -o scratch/isa/<file>.s
     python scratch/isa_hist.py scratch/isa/<file>.s <mangled-name-prefix> [top]
 prints totals (all / vector without MFMA / scalar / LDS / branches), the register and scratch figures and the most frequent opcodes"""
 import collections, re, sys

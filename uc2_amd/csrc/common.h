@@ -127,10 +127,8 @@ __device__ __forceinline__ void gelu_and_dgelu_bf(float x, float& g, float& d) {
   g = x * ph;
   d = fmaf(xc * sp, t, ph);
 }
-// The same arithmetic on a PAIR of values, written on 2-vectors so that hipcc emits v_pk_mul_f32 / v_pk_fma_f32 / v_pk_add_f32
-// (two values per full-rate issue slot) instead of v_fmaak / v_fmamk / v_mul per value: the scalar form's 12 full-rate
-// instructions per value came out as 11 issue slots + one v_mov (operand packing) in the GELU GEMM's epilogue, where the matrix
-// pipe is idle and the vector pipe is the bound; same operations in the same order, bit-identical results.
+// The same arithmetic on a PAIR of values: the same operations in the same order, bit-identical results.  (Two per instruction, where hipcc may emit
+// packed fp32 arithmetic; the Makefile has it off, so these are scalar instructions.)
 typedef float uc2_f2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void gelu_and_dgelu_bf2(uc2_f2v x, uc2_f2v& g, uc2_f2v& d) {
   const uc2_f2v xc = {__builtin_amdgcn_fmed3f(x.x, -9.0f, 9.0f), __builtin_amdgcn_fmed3f(x.y, -9.0f, 9.0f)};

@@ -191,7 +191,7 @@ __device__ __forceinline__ void pp16_epi_compute_q(const GemmArgs& p, const f32x
           } else if (EPI == EPI_GELU_D) {
 #if UC2_GELU_PACKED
 #pragma unroll
-            for (int e = 0; e < 4; e += 2) {              // pairs: packed fp32 arithmetic (common.h, gelu_and_dgelu_bf2)
+            for (int e = 0; e < 4; e += 2) {              // pairs (common.h, gelu_and_dgelu_bf2)
               uc2_f2v gg, dd;
               gelu_and_dgelu_bf2(uc2_f2v{v[e], v[e + 1]}, gg, dd);
               pre[k][e] = (bf16)dd.x; pre[k][e + 1] = (bf16)dd.y;
@@ -209,7 +209,7 @@ __device__ __forceinline__ void pp16_epi_compute_q(const GemmArgs& p, const f32x
           } else if (EPI == EPI_DGELU || EPI == EPI_MUL) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] *= (EPI == EPI_MUL) ? (float)axq[k][e] : dgelu_bf((float)axq[k][e]);
-            // (unconditional: under the run-time `want_cs` hipcc emitted a packed add AND a select per value -- 128 v_cndmask per
+            // (unconditional: under the run-time `want_cs` hipcc emitted an addition AND a select per value -- 128 v_cndmask per
             //  tile and wave; the sums are simply not used when no column-sum output was asked for)
 #pragma unroll
             for (int e = 0; e < 4; ++e) cs[4 * nb + e] += v[e];

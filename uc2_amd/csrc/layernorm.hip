@@ -11,6 +11,18 @@
 
 #define LN_MAXC 4     // chunks of 4 elements per lane: H <= 64*4*4 = 1024
 
+// Sums whose products are rounded before the addition.  Left open, fused or not is hipcc's choice and changes with its flags, and a last bit of a row's
+// statistics moves bf16 and e4m3 values downstream to the other side of a border
+__device__ __forceinline__ float ln_add(float x, float y) {
+#pragma clang fp contract(off)
+  return x + y;
+}
+__device__ __forceinline__ float ln_add_product(float q, float x, float y) {
+#pragma clang fp contract(off)
+  const float p = x * y;
+  return q + p;
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void ln_fwd_kernel(int M, int H, const T* __restrict__ x, const T* __restrict__ res,
                                                      const float* __restrict__ gamma, const float* __restrict__ beta,
@@ -63,7 +75,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(int M, int H, const T* __re
     const int c = lane + 64 * i;
     if (c < nch) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { const float d = v[i][e] - mean; q += d * d; }
+      for (int e = 0; e < 4; ++e) { const float d = v[i][e] - mean; q = ln_add_product(q, d, d); }
     }
   }
   const float var = wave_sum(q) / (float)H;
@@ -179,8 +191,8 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(int M, int H, const T* __re
         const float dyq = valid ? dyv[e] : 0.f;
         xh[i][e] = valid ? (xv[e] - mean) * rstd : 0.f;
         g[i][e] = dyq * gmr[i][e];
-        s1 += g[i][e];
-        s2 += g[i][e] * xh[i][e];
+        s1 = ln_add(s1, g[i][e]);
+        s2 = ln_add_product(s2, g[i][e], xh[i][e]);
         dg[i][e] += dyq * xh[i][e];
         db[i][e] += dyq;
       }
@@ -195,7 +207,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(int M, int H, const T* __re
         float dz[4], dxv[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          dz[e] = rstd * (g[i][e] - s1 - xh[i][e] * s2);
+          dz[e] = rstd * (ln_add(g[i][e], -s1) - xh[i][e] * s2);
           dxv[e] = (thresh && drop_after != 1) ? (kp[i][e] ? dz[e] * keep_scale : 0.f) : dz[e];
           dbx[i][e] += dxv[e];
         }
@@ -304,7 +316,7 @@ __global__ __launch_bounds__(256) void ln_fwd16_kernel(int M, int H, const bf16*
   for (int i = 0; i < NC8; ++i) {
     if (l32 + 32 * i < nch) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { const float d = v[i][e] - mean; q += d * d; }
+      for (int e = 0; e < 8; ++e) { const float d = v[i][e] - mean; q = ln_add_product(q, d, d); }
     }
   }
   const float var = half_sum(q) / (float)H;
