@@ -166,6 +166,19 @@ def test_cpu_tensors_are_refused():
             f()
 
 
+def test_gradients_are_refused_where_they_would_be_lost():
+    """quantisation and its product run outside autograd: an argument that wants a gradient raises, under no_grad it is a constant"""
+    x, w, bias = torch.zeros(4, 128, dtype=torch.bfloat16, requires_grad=True), torch.zeros(8, 128, requires_grad=True), torch.zeros(8, requires_grad=True)
+    a = ops.BlockRows(torch.zeros(4, 128, dtype=torch.uint8), torch.zeros(1, 4, dtype=torch.int32), 128)
+    b = ops.BlockWeight(torch.zeros(8, 128, dtype=torch.uint8), torch.zeros(1, 1, dtype=torch.uint8))
+    for f in (lambda: ops.fp8_quantize_block(x), lambda: ops.fp8_quantize_block(2 * x), lambda: ops.fp8_quantize_weight_block(w), lambda: ops.fp8_quantize_weight_block(w, transpose=True),
+              lambda: ops.gemm_fp8_block(a, b, bias=bias)):
+        with pytest.raises(_lib.Uc2Error, match="has no gradient"):
+            f()
+        with torch.no_grad(), pytest.raises(_lib.Uc2Error, match="GPU only"):            # (the next check)
+            f()
+
+
 def test_structures_match_the_header(tmp_path):
     """the binding's packed structures, these here and a C compiler's: the same sizes, and each field at the same place"""
     import os

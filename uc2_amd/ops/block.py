@@ -44,6 +44,12 @@ def _float_matrix(x, what):
     return x2 if x2.stride(1) == 1 and (x2.stride(0) >= x2.shape[1] or x2.shape[0] <= 1) else x2.contiguous()
 
 
+def _no_gradient(what, instead, *tensors):
+    """refuses tensors whose gradient would be lost without a word"""
+    if torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in tensors):
+        raise _lib.Uc2Error("%s has no gradient: call it under torch.no_grad(), or use %s" % (what, instead))
+
+
 def _rows_out(M, K, x):
     Kp = _up(K)
     return x.new_empty((M, Kp), dtype=torch.uint8), x.new_empty(((Kp + 511) // 512, M), dtype=torch.int32)
@@ -58,7 +64,8 @@ def _quant_rows(x2):
 
 
 def fp8_quantize_block(x):
-    """[..., K] (fp32 or bf16, any row stride) -> BlockRows of its rows, one launch"""
+    """[..., K] (fp32 or bf16, any row stride) -> BlockRows of its rows, one launch.  No gradient: for inference (training: linear_fp8_block)"""
+    _no_gradient("fp8_quantize_block", "linear_fp8_block", x)
     x2 = _float_matrix(x, "fp8_quantize_block")
     with device_guard(x2):
         return _quant_rows(x2)
@@ -75,7 +82,8 @@ def _quant_weight(w, transpose):
 
 def fp8_quantize_weight_block(w, transpose=False):
     """[N, K] weight (fp32 or bf16) -> BlockWeight; transpose: also that of W^T with the same values (the operand of the input gradient),
-    both from one read"""
+    both from one read.  No gradient: a parameter is quantised under torch.no_grad() (training: linear_fp8_block)"""
+    _no_gradient("fp8_quantize_weight_block", "linear_fp8_block", w)
     if not torch.is_tensor(w) or w.dim() != 2:
         raise _lib.Uc2Error("fp8_quantize_weight_block: a weight of two dimensions is needed")
     w = _float_matrix(w, "fp8_quantize_weight_block")
@@ -100,7 +108,9 @@ def _gemm(a8, sa, b8, sb, bias):
 
 def gemm_fp8_block(a, b, bias=None):
     """bf16 [M, N] = a b^T + bias of a = BlockRows [M, K] (fp8_quantize_block, rms_norm_fp8) and b = BlockWeight [N, K]
-    (fp8_quantize_weight_block; any (data, scale) pair of that layout); fp32 sums, one rounding"""
+    (fp8_quantize_weight_block; any (data, scale) pair of that layout); fp32 sums, one rounding.  No gradient, that of bias neither: for inference
+    (training: linear_fp8_block)"""
+    _no_gradient("gemm_fp8_block", "linear_fp8_block", bias)
     a8, sa, b8, sb = a[0], a[1], b[0], b[1]
     device = a8.device
     if not (a8.dtype == b8.dtype == sb.dtype == torch.uint8 and sa.dtype == torch.int32):
@@ -219,8 +229,8 @@ class LinearBlockFp8Fn(torch.autograd.Function):
 
 def linear_fp8_block(x, weight, bias=None):
     """bf16 x [..., K], weight [N, K] (fp32 or bf16), bias fp32 [N] or None -> bf16 [..., N]: a linear layer whose forward and input-gradient
-    products run on e4m3 operands with block scales.  The weight is quantised in the call (a weight that does not change: quantise it
-    once with fp8_quantize_weight_block and call gemm_fp8_block)."""
+    products run on e4m3 operands with block scales.  The weight is quantised in the call (for inference, with a weight that does not change:
+    quantise it once with fp8_quantize_weight_block and call gemm_fp8_block)."""
     if not torch.is_tensor(x) or x.dtype != torch.bfloat16 or x.dim() < 1:
         raise _lib.Uc2Error("linear_fp8_block computes on bf16 activations")
     _require_cuda(x)
@@ -324,8 +334,7 @@ def rms_norm_fp8(x, weight, eps=1e-6, residual=None):
     """the norm as an operand of gemm_fp8_block: (BlockRows of y [rows, H], s) with s as in rms_norm (x's values in its shape without a
     residual); y itself is never written.  No gradient: for inference (training: rms_norm, then linear_fp8_block)."""
     _rms_args(x, weight, residual, "rms_norm_fp8")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
-        raise _lib.Uc2Error("rms_norm_fp8 has no gradient: call it under torch.no_grad(), or use rms_norm and linear_fp8_block")
+    _no_gradient("rms_norm_fp8", "rms_norm and linear_fp8_block", x, weight, residual)
     with device_guard(x):
         s, _, _, q = _rms_fwd(x, weight, float(eps), residual, False, False, True)
     return q, x if residual is None else s.view(x.shape)
