@@ -155,6 +155,41 @@ def test_a_leaf_remembers_the_stream_of_its_first_graph(monkeypatch):
     assert bool((x.grad == 1).all()) and bool((y.grad == 2).all())
 
 
+def test_the_accumulations_below_other_operations_are_looked_at(monkeypatch):
+    """a capture is refused for a leaf behind other operations too; what has been looked at is not walked again"""
+    from uc2_amd.ops import base
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    streams, asked = {}, []
+
+    def stream_of(node):
+        asked.append(node.variable)
+        return streams.get(id(node.variable), 7)
+    monkeypatch.setattr(base, "_accumulation_stream", stream_of)
+
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return 2 * x
+
+        @staticmethod
+        @base.once
+        def backward(ctx, d):
+            return 2 * d
+    x, y = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+    f = lambda: Twice.apply(Twice.apply((x.double() * y.view(3)).float())).sum()  # noqa: E731
+    f().backward()
+    assert len(asked) == 2 and bool((x.grad == 4).all())
+    streams[id(y)] = 0
+    with pytest.raises(_lib.Uc2Error, match="eager graph"):
+        f().backward()
+
+
+def test_the_module_that_knows_the_accumulations_is_built():
+    x = torch.ones(3, requires_grad=True)
+    y = 2 * x
+    assert _lib.accumulation_stream(x) is None and y.requires_grad          # (the CPU has no streams; without the module this raises)
+
+
 def test_cpu_tensors_are_refused():
     x, w, g = torch.zeros(4, 128, dtype=torch.bfloat16), torch.zeros(8, 128), torch.ones(128)
     q = torch.zeros(1, 2, 4, 64)

@@ -742,6 +742,62 @@ def test_capture_beside_an_eager_graph_of_the_same_leaves_is_refused(monkeypatch
         assert all(torch.equal(s, t) for s, t in zip(b, torch.autograd.grad(eager, leaves, d)))
 
 
+def test_the_accumulation_of_a_leaf_is_known_whoever_made_it(monkeypatch):
+    """by another operation, held by a wrapper, behind a cast: the default stream's is refused, a stream's own is not (no real capture here)"""
+    w, x = normal((8, 96), 2), normal((4, 96), 1, BF16)
+    side = torch.cuda.Stream()
+    made = {"another operation": lambda t: t * 3, "a wrapper": lambda t: t.expand_as(t).grad_fn.next_functions[0][0], "the same operator behind a cast": lambda t: ops.linear_fp8_block(x, t.to(BF16))}
+    uses = {"direct": lambda t: ops.linear_fp8_block(x, t), "behind a cast": lambda t: ops.linear_fp8_block(x, t.to(BF16)), "behind a view of a product": lambda t: ops.linear_fp8_block(x, (2 * t).view(8, 96))}
+    for what, make in made.items():
+        for how, use in uses.items():
+            leaf = w.detach().requires_grad_()
+            assert _lib.accumulation_stream(leaf) is None
+            held = make(leaf)
+            torch.cuda.synchronize()
+            assert _lib.accumulation_stream(leaf) == 0
+            with torch.cuda.stream(side):
+                out = use(leaf)
+                with monkeypatch.context() as m:
+                    m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+                    with pytest.raises(_lib.Uc2Error, match="eager graph"):
+                        torch.autograd.grad(out, [leaf], torch.ones_like(out))
+            torch.cuda.synchronize()
+            del held, out
+            with torch.cuda.stream(side):                          # made on the stream itself: nothing to refuse
+                held = make(leaf)
+                out = use(leaf)
+                with monkeypatch.context() as m:
+                    m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+                    g, = torch.autograd.grad(out, [leaf], torch.ones_like(out))
+            torch.cuda.synchronize()
+            assert torch.isfinite(g).all(), (what, how)
+            del held, out
+
+
+def test_training_in_a_graph_behind_other_operations():
+    """a captured pass whose leaves reach the operators through a cast and a product, after another operation of the same capture has used them"""
+    x, w32, gain, dy = normal((9, 96), 1, BF16), normal((40, 96), 2), 1 + normal((96,), 3, F32, 0.1), normal((9, 40), 4, BF16)
+
+    def step(w, g):
+        squares = w * w
+        out = ops.linear_fp8_block(ops.rms_norm(x, 2 * g), w.to(BF16))
+        torch.autograd.backward([out, squares], [dy, torch.ones_like(squares)])
+        return [out.detach(), w.grad, g.grad]
+    leaves = lambda: [t.detach().requires_grad_() for t in (w32, gain)]  # noqa: E731
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(*leaves())
+    torch.cuda.synchronize()
+    own, graph = leaves(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*own)
+    for i in range(4):
+        x.copy_(normal(x.shape, 10 + i, BF16)), dy.copy_(normal(dy.shape, 20 + i, BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step(*leaves())))
+
+
 def test_saved_tensors_that_come_back_where_they_were_with_other_strides():
     buf = normal((2, 9, 3, 4, 64), 1, BF16)
     q, (_, k, v, dout) = buf[:, :, 0], attn_inputs(2, 9, 70, 4, 2, 64, BF16)[0:4]

@@ -15,6 +15,7 @@ from .config import cfg
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = cfg.lib_path      # (UC2_LIB_PATH: A/B of two builds on one box)
 _lib = None
+_streams = None
 ABI_VERSION = 14         # include/uc2_hip.h; bumped whenever a signature changes
 
 P, I, F, U64, I64, SZ = c_void_p, c_int, c_float, c_uint64, c_int64, c_size_t
@@ -174,6 +175,17 @@ def stream():
     if _raw_stream is not None and _cur_device is not None:
         return _raw_stream(_cur_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def accumulation_stream(leaf):
+    """id of the stream that a leaf's gradient is accumulated on (0: the default stream), None while no graph or wrapper holds its accumulation"""
+    global _streams
+    if _streams is None:
+        try:
+            from . import _autograd_streams as _streams
+        except ImportError as e:
+            raise Uc2Error("uc2_amd: _autograd_streams.so is missing or was built against another torch (%s): rebuild it (make -C uc2_amd/csrc)" % e) from e
+    return _streams.accumulation_stream(leaf)
 
 
 def dt(dtype):

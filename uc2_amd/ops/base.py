@@ -142,22 +142,39 @@ def device_guard(t):
     return _NO_GUARD if t.get_device() == _cur_device() else torch.cuda.device(t.device)
 
 
+def _accumulation_stream(node):
+    """stream of an AccumulateGrad node, remembered in it: torch's own record, whichever operation made the node (on a device without streams: the current one)"""
+    seen = node.metadata
+    if "uc2_stream" not in seen:
+        leaf = node.variable
+        seen["uc2_stream"] = _lib.accumulation_stream(leaf) if leaf.is_cuda else _lib.stream()
+    return seen["uc2_stream"]
+
+
 def note_leaves(ctx):
     """in a forward that will be differentiated, on the device of its tensors: each leaf among the inputs remembers the stream that its gradient's accumulation
     belongs to, that of the first of its graphs alive"""
     for node, _ in ctx.next_functions:
         if type(node).__name__ == "AccumulateGrad":
-            node.metadata.setdefault("uc2_stream", _lib.stream())
+            _accumulation_stream(node)
 
 
 def refuse_foreign_capture(ctx):
-    """A captured backward pass hands its gradients to the accumulations of its leaves.  While an eager graph of a leaf from the default stream lives, that
-    accumulation belongs to the default stream, which no capture may reach over to: torch ends the process there, so it is refused before.  (A warm-up on
-    a stream of its own leaves nothing of the kind.)"""
-    for node, _ in ctx.next_functions:
-        if type(node).__name__ == "AccumulateGrad" and node.metadata.get("uc2_stream") == 0:
-            raise _lib.Uc2Error("a backward pass cannot be captured while an eager graph of the same leaves from the default stream is alive: delete its outputs "
-                                "first, warm up on a stream of its own, or capture with leaves of its own (x.detach().requires_grad_())")
+    """A captured backward pass hands its gradients to the accumulations of its leaves, those behind other operations (a cast) among them.  While an eager
+    graph of a leaf from the default stream lives, or a wrapper holds the leaf's accumulation from there, the accumulation belongs to the default stream, which no
+    capture may reach over to: torch ends the process there, so it is refused before.  (A warm-up on a stream of its own leaves nothing of the kind.)"""
+    todo = [node for node, _ in ctx.next_functions]
+    while todo:
+        node = todo.pop()
+        if node is None or "uc2_clear" in node.metadata:          # (what lies below has been looked at: a graph does not change)
+            continue
+        if type(node).__name__ == "AccumulateGrad":
+            if _accumulation_stream(node) == 0:
+                raise _lib.Uc2Error("a backward pass cannot be captured while an eager graph of the same leaves from the default stream is alive: delete its outputs "
+                                    "first, warm up on a stream of its own, or capture with leaves of its own (x.detach().requires_grad_())")
+        else:
+            node.metadata["uc2_clear"] = True
+            todo.extend(below for below, _ in node.next_functions)
 
 
 def once(backward):
