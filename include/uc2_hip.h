@@ -195,7 +195,7 @@ int uc2_linear_wgrad(int M, int N, int K, const void* dy, long long lddy, const 
 
 /* ---- root-mean-square norm of a residual stream (beside LayerNorm below) ------------------------------------------------------------------
  *   sum = x + residual rounded to the tensors' type (both NULL: the norm reads x);  y = sum rstd gamma,  rstd = 1 / sqrt(mean(sum^2) + eps)
- *   rows contiguous, any alignment, H <= 16384.  y, rstd optional (y or q_out is given); q_out / q_scale: y as a rows operand of
+ *   rows contiguous, any alignment, M <= 2^30, H <= 16384.  y, rstd optional (y or q_out is given); q_out / q_scale: y as a rows operand of
  *   uc2_gemm_fp8_block, quantised from the fp32 values.
  *   backward: dx = rstd (g - h mean(g h)) + dsum, g = dy gamma, h = sum rstd -- the gradient of x and of residual alike; dsum (gradient that
  *   reaches the stream itself) may be NULL; dgamma [H] = sum over rows of dy h (written; may be NULL), in a fixed order through ws (uc2_rms_bwd_workspace bytes; 0: may be NULL). */

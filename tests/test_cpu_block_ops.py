@@ -115,6 +115,19 @@ def test_linear_wgrad_argument_errors():
     assert lib.uc2_linear_wgrad_workspace(0, 40, 72) == 0 and lib.uc2_linear_wgrad_workspace(4000, 1 << 30, 1 << 30) == 0
 
 
+def test_sizes_beyond_a_launch_are_argument_errors():
+    """2^32 work items along a dimension, 65535 workgroups along the second: refused before a launch that cannot be"""
+    lib = _lib.load()
+    g = dict(dout=P, dout_sb=64, dq=P, dk=P, dv=P, dq_sb=64, dk_sb=65 * 64, dk_sl=64, dv_sb=65 * 64, dv_sl=64)
+    many = attn(B=1 << 23, Lq=1, Lk=65, nh=1, nkv=1, q_sb=64, k_sb=65 * 64, k_sl=64, v_sb=65 * 64, v_sl=64, o_sb=64)
+    assert lib.uc2_xattn_workspace(ctypes.byref(many), 1) == 0
+    assert lib.uc2_xattn_bwd(ctypes.byref(many), ctypes.byref(_CrossAttnGrad(**g)), None, 0, None) == -1
+    assert lib.uc2_xattn_fwd(ctypes.byref(attn(B=(1 << 24) - 1, Lq=300, nh=1, nkv=1)), None, 0, None) == -1
+    assert lib.uc2_fp8_quant_square(1, 65535 * 128 + 1, 128, P, 128, P, P, None, None, None) == -1
+    assert lib.uc2_gemm_fp8_block((1 << 31) - 1, 8, 128, P, 128, P, (1 << 31) - 1, P, 128, P, None, P, 8, None) == -1
+    assert lib.uc2_linear_wgrad((1 << 31) - 1, 8, 8, P, 8, P, 8, P, 8, None, P, 1 << 40, None) == -1
+
+
 def test_a_leaf_remembers_the_stream_of_its_first_graph(monkeypatch):
     """note_leaves and refuse_foreign_capture on the streams and captures they are told of"""
     from uc2_amd.ops.base import note_leaves, once

@@ -309,6 +309,32 @@ def test_rms_norm_fp8_is_the_norm_quantised(dtype, M, H):
     assert torch.equal(b.data, a.data) and torch.equal(b.scale, a.scale) and s1 is s
 
 
+def test_rows_beyond_one_launch():
+    """2^26 rows of the norm and 2^28 of the quantisation are a launch's most: the rows around the border and the last ones as if they were alone"""
+    M, w = (1 << 26) + 5, 1 + normal((8,), 2, F32, 0.2)
+    at = torch.cat([torch.arange(3), torch.arange((1 << 26) - 8, M)]).to(DEV)
+    x, res = normal((M, 8), 1, BF16), normal((M, 8), 3, BF16)
+    a, s = ops.rms_norm_fp8(x, w, residual=res)
+    y, s2 = ops.rms_norm(x, w, residual=res)
+    a1, s1 = ops.rms_norm_fp8(x[at], w, residual=res[at])
+    assert torch.equal(s[at], s1) and torch.equal(s2[at], s1) and torch.equal(y[at], ops.rms_norm(x[at], w, residual=res[at])[0])
+    assert torch.equal(a.data[at], a1.data) and torch.equal(a.scale[:, at], a1.scale)
+    assert torch.equal(s, x + res) and bool(torch.isfinite(y).all())
+    xg = x.requires_grad_()
+    dx, = torch.autograd.grad(ops.rms_norm(xg, w), [xg], res)
+    xs = xg.detach()[at].requires_grad_()
+    assert torch.equal(dx[at], torch.autograd.grad(ops.rms_norm(xs, w), [xs], res[at])[0])
+    del x, xg, res, a, s, y, s2, dx
+    M = (1 << 28) + 5
+    at = torch.cat([torch.arange(3), torch.arange((1 << 28) - 8, M)]).to(DEV)
+    x = torch.empty(M, 8, device=DEV, dtype=BF16).normal_(generator=gen(5))
+    a = ops.fp8_quantize_block(x)
+    a1 = ops.fp8_quantize_block(x[at])
+    assert torch.equal(a.data[at], a1.data) and torch.equal(a.scale[:, at], a1.scale)
+    del a, x
+    torch.cuda.empty_cache()
+
+
 # ---- cross attention ------------------------------------------------------------------------------------------------------------
 def attn_inputs(B, Lq, Lk, nh, nkv, D, dtype, seed=0, std=1.0):
     q = normal((B, Lq, nh, D), seed + 1, dtype, std)

@@ -951,7 +951,7 @@ static bool xa_side(const XaArgs& a, XaSide& side, int cols, int ns, int splits)
   side.splits = splits;
   const long long n = (long long)(a.BH >= 8 ? (a.BH + 7) / 8 * 8 : a.BH) * side.tiles * splits;
   side.blocks = (int)n;
-  return n < (1ll << 30);
+  return n <= UC2_MOST_BLOCKS(64 * ns);
 }
 #define XA_LAUNCH(KERN, TT_, DD_, NN_, grid)                                                                                        \
   do {                                                                                                                              \
@@ -1000,7 +1000,7 @@ extern "C" int uc2_xattn_fwd(const Uc2CrossAttn* attn, void* ws, size_t ws_bytes
     // four waves per row from 8 splits on
     const bool wide = pl.s_fwd >= 8;
     const long long rows = (long long)a.BH * a.R, blocks = wide ? rows : (rows + 3) / 4;
-    UC2_CHECK_ARG(blocks < (1ll << 31));
+    UC2_CHECK_ARG(blocks <= UC2_MOST_BLOCKS(256));
 #define XA_GO(T_, D_)                                                                                                               \
   if (wide) hipLaunchKernelGGL((xattn_join_kernel<T_, D_, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a);                         \
   else hipLaunchKernelGGL((xattn_join_kernel<T_, D_, 1>), dim3((unsigned)blocks), dim3(256), 0, st, a)
@@ -1039,11 +1039,12 @@ extern "C" int uc2_xattn_bwd(const Uc2CrossAttn* attn, const Uc2CrossAttnGrad* g
   a.delta = (float*)ws;
   a.dkv.part = (float*)((char*)ws + pl.delta);
   a.dq.part = (float*)((char*)ws + pl.delta + pl.part_dkv);
+  UC2_CHECK_ARG((long long)a.dkv.blocks + a.dq.blocks <= UC2_MOST_BLOCKS(64 * ns));
   const int grid = a.dkv.blocks + a.dq.blocks;
   if (grid == 0) return 0;                                        // (neither queries nor keys)
   if (pl.pre && a.R > 0) {
     const long long lanes = (long long)a.BH * a.R * (p->D * el / 16), n = (lanes + 255) / 256;
-    UC2_CHECK_ARG(n < (1ll << 31));
+    UC2_CHECK_ARG(n <= UC2_MOST_BLOCKS(256));
 #define XA_GO(T_, D_) hipLaunchKernelGGL((xattn_delta_kernel<T_, D_>), dim3((unsigned)n), dim3(256), 0, st, a);                    \
     if (a.thresh) hipLaunchKernelGGL((xattn_bwd_kernel<T_, D_, 4, true, true>), dim3(grid), dim3(256), 0, st, a);                   \
     else hipLaunchKernelGGL((xattn_bwd_kernel<T_, D_, 4, false, true>), dim3(grid), dim3(256), 0, st, a)
@@ -1056,7 +1057,7 @@ extern "C" int uc2_xattn_bwd(const Uc2CrossAttn* attn, const Uc2CrossAttnGrad* g
   }
   UC2_LAUNCH_CHECK();
   const long long rows = (pl.s_dkv > 1 ? 2ll * a.BH * a.Lk : 0) + (pl.s_dq > 1 ? (long long)a.BH * a.R : 0), blocks = (rows * (p->D / 4) + 255) / 256;
-  UC2_CHECK_ARG(blocks < (1ll << 31));
+  UC2_CHECK_ARG(blocks <= UC2_MOST_BLOCKS(256));
   if (blocks > 0) {
 #define XA_GO(T_, D_) hipLaunchKernelGGL((xattn_sum_kernel<T_, D_>), dim3((unsigned)blocks), dim3(256), 0, st, a)
     XA_TD(XA_GO);

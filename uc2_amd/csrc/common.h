@@ -17,6 +17,8 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 #define UC2_CHECK_ARG(cond) do { if (!(cond)) { uc2_set_error(__FILE__, __LINE__, #cond); return -1; } } while (0)
 #define UC2_LAUNCH_CHECK() do { hipError_t e__ = hipGetLastError(); if (e__ != hipSuccess) { uc2_set_error(__FILE__, __LINE__, hipGetErrorString(e__)); return (int)e__; } } while (0)
 extern "C" void uc2_set_error(const char* file, int line, const char* what);
+// a launch has fewer than 2^32 work items along a dimension
+#define UC2_MOST_BLOCKS(threads) ((int)((1ll << 32) / (threads)) - 1)
 
 // ---- dtype helpers ----
 template <typename T> __device__ __forceinline__ float to_f(T v);

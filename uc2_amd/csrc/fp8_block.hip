@@ -9,7 +9,7 @@
 // a wave takes 512 columns of R rows: R loads in flight, then R reductions over 16 lanes
 template <typename T, int R, bool WHOLE>
 __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(int M, int K, int Kp, const T* __restrict__ x, long long ldx, unsigned char* __restrict__ q,
-                                                             unsigned* __restrict__ scale, int groups, long long items) {
+                                                             unsigned* __restrict__ scale, int lds, int groups, long long items) {
   const int lane = threadIdx.x & 63;
   const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (item >= items) return;
@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(int M, int K, int K
     const int row = rb * R + r;
     float v[8];
     x8[r].template get<WHOLE>(v, c, K);
-    if (row < M) blk_quant_row(v, c, Kp, q + (size_t)row * Kp, scale + (size_t)g * M + row, lane);
+    if (row < M) blk_quant_row(v, c, Kp, q + (size_t)row * Kp, scale + (size_t)g * lds + row, lane);
   }
 }
 extern "C" int uc2_fp8_quant_rows(int dtype, int M, int K, const void* x, long long ldx, void* out, void* scale, void* stream) {
@@ -33,13 +33,17 @@ extern "C" int uc2_fp8_quant_rows(int dtype, int M, int K, const void* x, long l
   const int Kp = (K + 127) / 128 * 128, groups = (Kp + 511) / 512;
   // four rows per wave once that leaves two waves for every SIMD (2048), one row below
   const int R = (long long)M * groups >= 8192 ? 4 : 1;
-  const long long items = (long long)((M + R - 1) / R) * groups, blocks = (items + 3) / 4;
-  UC2_CHECK_ARG(blocks < (1ll << 31));
+  const int most = (int)(UC2_MOST_BLOCKS(256) * 4ll / groups) * R, el = dtype == 1 ? 2 : 4;      // rows of a launch: 2^28 of 512 columns
   hipStream_t st = (hipStream_t)stream;
-#define QROWS_(T_, R_, W_) hipLaunchKernelGGL((fp8_quant_rows_kernel<T_, R_, W_>), dim3((unsigned)blocks), dim3(256), 0, st, M, K, Kp, (const T_*)x, ldx, (unsigned char*)out, (unsigned*)scale, groups, items)
+#define QROWS_(T_, R_, W_) hipLaunchKernelGGL((fp8_quant_rows_kernel<T_, R_, W_>), dim3((unsigned)blocks), dim3(256), 0, st, n, K, Kp, (const T_*)xp, ldx, (unsigned char*)out + (size_t)m0 * Kp, (unsigned*)scale + m0, M, groups, items)
 #define QROWS(T_, R_) do { if (K % 8 == 0) QROWS_(T_, R_, true); else QROWS_(T_, R_, false); } while (0)
-  if (dtype == 1) { if (R == 4) QROWS(bf16, 4); else QROWS(bf16, 1); } else { if (R == 4) QROWS(float, 4); else QROWS(float, 1); }
-  UC2_LAUNCH_CHECK();
+  for (long long m0 = 0; m0 < M; m0 += most) {
+    const int n = (int)(M - m0 < most ? M - m0 : most);
+    const char* xp = (const char*)x + (size_t)m0 * ldx * el;
+    const long long items = (long long)((n + R - 1) / R) * groups, blocks = (items + 3) / 4;
+    if (dtype == 1) { if (R == 4) QROWS(bf16, 4); else QROWS(bf16, 1); } else { if (R == 4) QROWS(float, 4); else QROWS(float, 1); }
+    UC2_LAUNCH_CHECK();
+  }
   return 0;
 }
 
@@ -95,7 +99,7 @@ __global__ __launch_bounds__(256) void fp8_quant_square_kernel(int N, int K, int
 }
 extern "C" int uc2_fp8_quant_square(int dtype, int N, int K, const void* w, long long ldw, void* out, void* scale, void* out_t, void* scale_t, void* stream) {
   UC2_CHECK_ARG(dtype == 0 || dtype == 1);
-  UC2_CHECK_ARG(N >= 0 && K >= 1 && N <= (1 << 23) && K <= (1 << 23) && ldw >= K);
+  UC2_CHECK_ARG(N >= 0 && K >= 1 && N <= 65535 * 128 && K <= (1 << 23) && ldw >= K);      // (65535: a launch's second grid dimension)
   if (N == 0) return 0;
   UC2_CHECK_ARG(w && out && scale && (out_t == nullptr) == (scale_t == nullptr) && (((uintptr_t)out | (uintptr_t)out_t) & 7) == 0);
   const int Kp = (K + 127) / 128 * 128, Np = (N + 127) / 128 * 128;

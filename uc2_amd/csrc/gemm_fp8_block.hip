@@ -201,7 +201,7 @@ static void blk_launch(BlkGemm p, hipStream_t st) {
 
 extern "C" int uc2_gemm_fp8_block(int M, int N, int K, const void* A8, int lda, const void* scale_a, int rows_a, const void* B8, int ldb,
                                   const void* scale_b, const float* bias, void* C, int ldc, void* stream) {
-  UC2_CHECK_ARG(M >= 0 && N >= 0 && K >= 1 && K <= (1 << 30));
+  UC2_CHECK_ARG(M >= 0 && M < 0x7FFFFF00 && N >= 0 && K >= 1 && K <= (1 << 30));
   if (M == 0 || N == 0) return 0;
   const int Kp = (K + 127) / 128 * 128;
   UC2_CHECK_ARG((N + 63) / 64 < 65536);                            // (a launch's second grid dimension)

@@ -16,7 +16,7 @@ struct RmsArgs {
   int M, H; float eps;
   const void *x, *res, *s, *dy, *ds; const float* w; const float* rstd_in;
   void *y, *s_out, *dx; float* rstd; float* part;
-  unsigned char* q; unsigned* qs; int Kp;
+  unsigned char* q; unsigned* qs; int Kp, ldqs;       // ldqs: the operand's rows
 };
 
 // sum over the NW waves of a row (the workgroup holds whole rows: NW = 1 needs no LDS)
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(NW == 16 ? 1024 : 256) void rms_fwd_kernel(RmsArgs 
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * r * g[e];
     if (a.y) blk_store8((T*)a.y + (size_t)row * a.H, c, a.H, v[i]);
-    if (Q) blk_quant_row(v[i], c, a.Kp, a.q + (size_t)row * a.Kp, a.qs + (size_t)(i * NW + w) * a.M + row, lane);
+    if (Q) blk_quant_row(v[i], c, a.Kp, a.q + (size_t)row * a.Kp, a.qs + (size_t)(i * NW + w) * a.ldqs + row, lane);
   }
 }
 
@@ -210,10 +210,10 @@ extern "C" int uc2_rms_fwd(int dtype, int M, int H, const void* x, const void* r
   UC2_CHECK_ARG(((uintptr_t)q_out & 7) == 0 && ((uintptr_t)q_scale & 3) == 0);
   RmsArgs a{};
   a.M = M; a.H = H; a.eps = eps; a.x = x; a.res = residual; a.w = gamma; a.s_out = sum; a.y = y; a.rstd = rstd;
-  a.q = (unsigned char*)q_out; a.qs = (unsigned*)q_scale; a.Kp = (H + 127) / 128 * 128;
+  a.q = (unsigned char*)q_out; a.qs = (unsigned*)q_scale; a.Kp = (H + 127) / 128 * 128; a.ldqs = M;
   int nw, nv;
   rms_shape(H, nw, nv);
-  const int blocks = nw == 1 ? (M + 3) / 4 : M, threads = nw == 16 ? 1024 : 256;
+  const int rpb = nw == 1 ? 4 : 1, threads = nw == 16 ? 1024 : 256, most = UC2_MOST_BLOCKS(threads) * rpb, el = dtype == 1 ? 2 : 4;
   hipStream_t st = (hipStream_t)stream;
   const bool whole = H % 8 == 0;
 #define RMS_F(T_, NW_, NV_, Q_)                                                                                                     \
@@ -221,9 +221,19 @@ extern "C" int uc2_rms_fwd(int dtype, int M, int H, const void* x, const void* r
     if (whole) hipLaunchKernelGGL((rms_fwd_kernel<T_, NW_, NV_, Q_, true>), dim3(blocks), dim3(threads), 0, st, a);                  \
     else hipLaunchKernelGGL((rms_fwd_kernel<T_, NW_, NV_, Q_, false>), dim3(blocks), dim3(threads), 0, st, a);                       \
   } while (0)
-  if (dtype == 1) { if (q_out) RMS_GO(RMS_F, bf16, true); else RMS_GO(RMS_F, bf16, false); }
-  else { if (q_out) RMS_GO(RMS_F, float, true); else RMS_GO(RMS_F, float, false); }
-  UC2_LAUNCH_CHECK();
+  for (int m0 = 0; m0 < M; m0 += most) {                           // (one launch below 2^26 rows of 2048)
+    a.M = M - m0 < most ? M - m0 : most;
+    const int blocks = (a.M + rpb - 1) / rpb;
+    const size_t at = (size_t)m0 * H * el;
+    a.x = (const char*)x + at;
+    if (residual) { a.res = (const char*)residual + at; a.s_out = (char*)sum + at; }
+    if (y) a.y = (char*)y + at;
+    if (rstd) a.rstd = rstd + m0;
+    if (q_out) { a.q = (unsigned char*)q_out + (size_t)m0 * a.Kp; a.qs = (unsigned*)q_scale + m0; }
+    if (dtype == 1) { if (q_out) RMS_GO(RMS_F, bf16, true); else RMS_GO(RMS_F, bf16, false); }
+    else { if (q_out) RMS_GO(RMS_F, float, true); else RMS_GO(RMS_F, float, false); }
+    UC2_LAUNCH_CHECK();
+  }
   return 0;
 }
 extern "C" size_t uc2_rms_bwd_workspace(int M, int H) {

@@ -249,7 +249,7 @@ static int wgrad_cols_splits(int M, int N) {
   const int s = want < most ? want : most;
   return s < 1 ? 1 : s > 32 ? 32 : s;
 }
-static bool wgrad_sizes_ok(int M, int N, int K) { return M >= 1 && N >= 1 && K >= 1 && N <= (1 << 23) && K <= (1 << 23) && (long long)((N + 127) / 128) * ((K + 127) / 128) < (1ll << 30); }
+static bool wgrad_sizes_ok(int M, int N, int K) { return M >= 1 && M < 0x7FFFFF00 && N >= 1 && K >= 1 && N <= (1 << 23) && K <= (1 << 23) && (long long)((N + 127) / 128) * ((K + 127) / 128) < (1ll << 30); }
 static size_t wgrad_up(size_t n) { return (n + 255) & ~(size_t)255; }
 extern "C" size_t uc2_linear_wgrad_workspace(int M, int N, int K) {
   if (!wgrad_sizes_ok(M, N, K)) return 0;
