@@ -59,6 +59,13 @@ def test_cross_attention_backward_argument_errors():
     assert lib.uc2_xattn_workspace(ctypes.byref(attn(D=7)), 0) == 0
 
 
+def test_cross_attention_backward_without_queries_checks_its_keys():
+    lib = _lib.load()
+    g = _CrossAttnGrad(dout=P, dout_sb=768, dout_sl=256, dout_sh=64, dq=P, dk=P, dv=P, dq_sb=768, dq_sl=256, dq_sh=64, dk_sb=640, dk_sl=128, dk_sh=64, dv_sb=640, dv_sl=128, dv_sh=64)
+    for bad in (dict(k=0), dict(v=0), dict(k=P + 8), dict(v=P + 2), dict(k_sl=129), dict(v_sh=1 << 22)):
+        assert lib.uc2_xattn_bwd(ctypes.byref(attn(Lq=0, **bad)), ctypes.byref(g), None, 0, None) == -1, bad
+
+
 def test_empty_calls_launch_nothing():
     lib = _lib.load()
     assert lib.uc2_xattn_fwd(ctypes.byref(attn(B=0)), None, 0, None) == 0

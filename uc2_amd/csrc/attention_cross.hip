@@ -922,14 +922,20 @@ static int xa_check(const Uc2CrossAttn* p) {
   UC2_CHECK_ARG(p->drop_p >= 0.f && p->drop_p < 1.f);
   return 0;
 }
+static int xa_keys(const Uc2CrossAttn* p) {
+  const int el = p->dtype ? 2 : 4;
+  UC2_CHECK_ARG(p->Lk == 0 || (p->k && p->v));
+  UC2_CHECK_ARG(xa_str_ok(p->k_sb, p->k_sl, p->k_sh, el) && xa_str_ok(p->v_sb, p->v_sl, p->v_sh, el));
+  UC2_CHECK_ARG((((uintptr_t)p->k | (uintptr_t)p->v) & 15) == 0);
+  return 0;
+}
 static int xa_ptrs(const Uc2CrossAttn* p, bool backward) {
   const int el = p->dtype ? 2 : 4;
-  UC2_CHECK_ARG(p->q && (p->out || (backward && p->dtype == 1 && p->out_f32)) && (p->Lk == 0 || (p->k && p->v)));
+  UC2_CHECK_ARG(p->q && (p->out || (backward && p->dtype == 1 && p->out_f32)));
   UC2_CHECK_ARG(!backward || p->dtype == 0 || p->out_f32);
-  UC2_CHECK_ARG(xa_str_ok(p->q_sb, p->q_sl, p->q_sh, el) && xa_str_ok(p->k_sb, p->k_sl, p->k_sh, el) && xa_str_ok(p->v_sb, p->v_sl, p->v_sh, el));
-  UC2_CHECK_ARG(xa_str_ok(p->o_sb, p->o_sl, p->o_sh, el));
-  UC2_CHECK_ARG((((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->out | (uintptr_t)p->out_f32) & 15) == 0);
-  return 0;
+  UC2_CHECK_ARG(xa_str_ok(p->q_sb, p->q_sl, p->q_sh, el) && xa_str_ok(p->o_sb, p->o_sl, p->o_sh, el));
+  UC2_CHECK_ARG((((uintptr_t)p->q | (uintptr_t)p->out | (uintptr_t)p->out_f32) & 15) == 0);
+  return xa_keys(p);
 }
 static XaArgs xa_args(const Uc2CrossAttn* p) {
   const int el = p->dtype ? 2 : 4;
@@ -1025,7 +1031,7 @@ extern "C" int uc2_xattn_bwd(const Uc2CrossAttn* attn, const Uc2CrossAttnGrad* g
   UC2_CHECK_ARG(xa_str_ok(g->dout_sb, g->dout_sl, g->dout_sh, el) && xa_str_ok(g->dq_sb, g->dq_sl, g->dq_sh, el));
   UC2_CHECK_ARG(xa_str_ok(g->dk_sb, g->dk_sl, g->dk_sh, el) && xa_str_ok(g->dv_sb, g->dv_sl, g->dv_sh, el));
   UC2_CHECK_ARG((((uintptr_t)g->dout | (uintptr_t)g->dq | (uintptr_t)g->dk | (uintptr_t)g->dv) & 15) == 0);
-  if (p->Lq > 0) { if (int e = xa_ptrs(p, true)) return e; }
+  if (int e = p->Lq > 0 ? xa_ptrs(p, true) : xa_keys(p)) return e;      // (without queries the keys are read all the same)
   const XaPlan pl = xa_plan(p);
   UC2_CHECK_ARG(pl.bwd == 0 || (ws && ws_bytes >= pl.bwd && ((uintptr_t)ws & 15) == 0));
   hipStream_t st = (hipStream_t)stream;
