@@ -843,6 +843,33 @@ def test_saved_tensors_that_come_back_where_they_were_with_other_strides():
     assert torch.equal(torch.autograd.grad(o, [qg], dout)[0], want[1])
 
 
+def test_saved_tensors_that_come_back_with_gaps():
+    """saved-tensor hooks that bring every tensor back with a stride of two in its last dimension, or as columns: the gradients of the tensors themselves"""
+    def gaps(t):
+        return torch.stack([t, t], -1)[..., 0]
+
+    def columns(t):
+        return t.transpose(0, -1).contiguous().transpose(0, -1)
+    q, k, v, dout = attn_inputs(2, 9, 70, 4, 2, 64, BF16)
+    mask, lens = normal((2, 70), 9), torch.tensor([70, 33], device=DEV, dtype=torch.int32)
+    x, w, b, dy = normal((9, 96), 1, BF16), normal((40, 96), 2), normal((40,), 3), normal((9, 40), 4, BF16)
+    gain, dn = 1 + normal((96,), 5, F32, 0.1), normal((9, 96), 6, BF16)
+
+    def run(unpack):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), unpack):
+            leaves = [t.detach().requires_grad_() for t in (q, k, v, x, w, b, gain, x)]
+            o16 = ops.cross_attention(*leaves[:3], key_mask=mask, k_lens=lens)
+            o32 = ops.cross_attention(*(t.float() for t in leaves[:3]), key_mask=mask, k_lens=lens, drop_p=0.2)
+            y = ops.linear_fp8_block(*leaves[3:6])
+            n, s = ops.rms_norm(leaves[7], leaves[6], residual=x)
+        return torch.autograd.grad([o16, o32, y, n, s], leaves, [dout, dout.float(), dy, dn, dn])
+    ops.rng.manual_seed(4)
+    want = run(lambda t: t)
+    for unpack in (gaps, columns):
+        ops.rng.manual_seed(4)
+        assert all(torch.equal(a, c) for a, c in zip(run(unpack), want)), unpack.__name__
+
+
 def test_saved_tensors_that_come_back_as_copies():
     """saved-tensor hooks (offloading): the backward reads what they bring, not the tensors of the forward"""
     q, k, v, dout = attn_inputs(2, 9, 70, 4, 2, 64, BF16)

@@ -205,6 +205,10 @@ class LinearBlockFp8Fn(torch.autograd.Function):
         shp, (N, K), wtype, n = ctx.cfg
         need_dx, need_dw, need_db = ctx.needs_input_grad
         dy2 = _float_matrix(dy, "linear_fp8_block")
+        if need_dw:                                       # (saved-tensor hooks may bring other strides than the forward's)
+            x2 = _float_matrix(x2, "linear_fp8_block")
+        if need_dx:
+            wt = wt.contiguous()
         M = dy2.shape[0]
         dx = dw = db = None
         with device_guard(dy2):
@@ -299,7 +303,7 @@ class RMSNormFn(torch.autograd.Function):
     @staticmethod
     @once
     def backward(ctx, dy, ds=None):
-        s, weight, rstd = ctx.saved_tensors
+        s, weight, rstd = (t.contiguous() for t in ctx.saved_tensors)       # (saved-tensor hooks may bring other strides than the forward's)
         M, H = s.shape
         if dy is None:                                   # only the stream is used
             return ds, torch.zeros_like(weight) if ctx.needs_input_grad[1] else None, None, ds

@@ -88,8 +88,10 @@ class CrossAttentionFn(torch.autograd.Function):
             dout = _rows16(dout)
             # saved-tensor hooks may bring copies: elsewhere, or where the tensor itself had been with other strides
             p = _PTRS.unpack(desc)
-            if (*p[:5], p[7] or p[5], p[6], p[8]) != tuple([0 if t is None else t.data_ptr() for t in saved]) or strides != _strides(q, k, v, key_mask):
+            if ((*p[:5], p[7] or p[5], p[6], p[8]) != tuple([0 if t is None else t.data_ptr() for t in saved]) or strides != _strides(q, k, v, key_mask)
+                    or not (out.is_contiguous() and lse.is_contiguous() and (k_lens is None or k_lens.is_contiguous()))):
                 q, k, v, lse = _rows16(q), _rows16(k), _rows16(v), lse.contiguous()
+                key_mask, k_lens = (None if t is None else t.contiguous() for t in (key_mask, k_lens))
                 out, out_f32 = (None, out.clone(memory_format=torch.contiguous_format)) if q.dtype == torch.bfloat16 else (_rows16(out), None)
                 desc = _describe(q, k, v, out, key_mask, k_lens, scale, drop_p, lse, out_f32, seed, site)
             dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
