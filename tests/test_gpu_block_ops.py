@@ -100,6 +100,41 @@ def test_gemm_block(M, N, K, bias):
     assert torch.equal(got, ops.gemm_fp8_block(a, q, bias=b))
 
 
+@pytest.mark.parametrize("M,N,K", [(8460, 2310, 256), (8460, 2310, 1024), (8448, 2304, 3840), (8460, 2310, 4096), (16896, 1024, 7424)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_gemm_block_more_tiles_than_compute_units(M, N, K, bias):
+    """more than 256 whole 256 x 256 tiles: workgroups of the persistent kernel take a second one (2, 8, 30, 32 and 58 blocks of K: with one, two and three fills
+    of the scales, and the next tile's first fill after a refill), nine columns of tiles, with and without remainders.  Each row and each
+    128 columns have a scale of their own, so a tile that took another's scales would be off by a power of two"""
+    g = gen(M + N + K)
+    x = normal((M, K), 1, BF16) * torch.exp2(torch.randint(-6, 7, (M, 1), generator=g, device=DEV).float()).to(BF16)
+    x *= torch.exp2(torch.randint(-3, 4, (1, K // 128, 1), generator=g, device=DEV).float()).expand(1, K // 128, 128).reshape(1, K).to(BF16)
+    w = normal((N, K), 3, F32, K ** -0.5) * torch.exp2(torch.randint(-6, 7, ((N + 127) // 128, 1, K // 128, 1), generator=g, device=DEV).float()).expand(-1, 128, -1, 128).reshape(-1, K)[:N]
+    b = normal((N,), 5) if bias else None
+    a, q = ops.fp8_quantize_block(x), ops.fp8_quantize_weight_block(w)
+    got = ops.gemm_fp8_block(a, q, bias=b)
+    assert torch.equal(got, ops.gemm_fp8_block(a, q, bias=b))
+    for r0 in range(0, M, 2112):                             # (the 64-bit product in parts)
+        part = ops.BlockRows(a.data[r0:r0 + 2112], a.scale[:, r0:r0 + 2112], K)
+        A, B = R.rows_values(part)[0], R.weight_values(q, K)
+        R.assert_gemm(got[r0:r0 + 2112], A, B, b, "%d x %d x %d from row %d" % (M, N, K, r0))
+
+
+def test_gemm_block_a_row_has_the_same_bits_among_others():
+    """the operand bytes of a row do not depend on the rows beside it, nor do the product's bits where the same kernel runs: few rows, 64 x 64 tiles, 128 x 128
+    tiles, whole 256 x 256 tiles, and with other values in the rows behind"""
+    for N, K, sizes in ((640, 768, (3, 16)), (1024, 1024, (33, 50)), (2048, 512, (640, 700)), (4096, 384, (1280, 1400)), (2048, 512, (4096, 4352))):
+        x, w = normal((sizes[1], K), 1, BF16), normal((N, K), 2)
+        q = ops.fp8_quantize_weight_block(w)
+        full, m = ops.fp8_quantize_block(x), sizes[0]
+        some = ops.fp8_quantize_block(x[:m])
+        assert torch.equal(some.data, full.data[:m]) and torch.equal(some.scale, full.scale[:, :m])
+        want = ops.gemm_fp8_block(full, q)
+        assert torch.equal(ops.gemm_fp8_block(some, q), want[:m]), (N, K, sizes)
+        x[m:] = math.inf
+        assert torch.equal(ops.gemm_fp8_block(ops.fp8_quantize_block(x), q)[:m], want[:m])
+
+
 def test_gemm_block_rows_do_not_depend_on_the_others():
     """a row alone and among others: the same operand bytes; where both run the same kernel the same bits"""
     K, N = 768, 640
@@ -249,6 +284,25 @@ def test_rms_norm_forward_and_gradients(dtype, M, H, with_res):
     c, cm = (g * h).mean(-1, keepdim=True), (g * h).abs().mean(-1, keepdim=True)
     want = r * (g - h * c) + (0 if ds is None else ds.double())
     mag = r * (g.abs() + h.abs() * cm)
+    R.assert_within(dx, want, u * want.abs() + (2 * r1 + (H + 8) * u32) * mag + u32 * want.abs(), "dx")
+    want, mag = (dy.double() * h).sum(0), (dy.double() * h).abs().sum(0)
+    R.assert_within(dw, want, (M + 4) * u32 * mag + r1 * mag, "dw")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,H", [(2049, 768), (5003, 1000), (9000, 130), (1100, 2500), (700, 9000)])
+def test_rms_norm_gradient_of_more_rows_than_workgroups(dtype, M, H):
+    """more rows than the backward's 512 workgroups take at once: each goes over several, of every width of row"""
+    x, w, res = normal((M, H), 1, dtype, 3.0), 1 + normal((H,), 2, F32, 0.2), normal((M, H), 3, dtype)
+    dy, ds = normal((M, H), 4, dtype), normal((M, H), 5, dtype)
+    eps, u, u32, r1 = 1e-5, R.U[dtype], R.U[F32], R.rms_rel(H)
+    _, s, r = R.rms(x, w, eps, res)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y, sg = ops.rms_norm(xg, wg, eps, residual=res)
+    dx, dw = torch.autograd.grad([y, sg], [xg, wg], [dy, ds])
+    g, h = dy.double() * w.double(), s.double() * r
+    c, cm = (g * h).mean(-1, keepdim=True), (g * h).abs().mean(-1, keepdim=True)
+    want, mag = r * (g - h * c) + ds.double(), r * (g.abs() + h.abs() * cm)
     R.assert_within(dx, want, u * want.abs() + (2 * r1 + (H + 8) * u32) * mag + u32 * want.abs(), "dx")
     want, mag = (dy.double() * h).sum(0), (dy.double() * h).abs().sum(0)
     R.assert_within(dw, want, (M + 4) * u32 * mag + r1 * mag, "dw")
