@@ -18,10 +18,12 @@
 // partials (outputs with maximum and sum; gradients), joined by a second small kernel.
 // Roundings below fp32: the weights (forward, dV) and the score gradients (dQ, dK) to bf16 where they enter the second product, results to T; each at most half
 // a step of its value, so they leave the results off by 2.2e-3 to 2.5e-3 of their norm where one rounding of the result makes 1.7e-3.
-// Measured, bf16: 2 x 2048 x 4096, 16 heads of 64: forward 101 - 110 us (0.62 - 0.68 PF/s), backward 260 - 286 (0.60 - 0.66, 0.84 - 0.92 with the products that
-// it makes twice); the vector pipe is busy half of that, the matrix pipe 28 % (forward) and 41 %, and two waves per SIMD, all that the registers
-// hold, overlap them little (products between the vector instructions of one wave, raised priorities: no gain).  104 x 60 x 100, 12 heads of 64:
-// 18 + 43 us (its bytes at a copy's rate: 14 + 23).  16 x 1 x 16384, 16 heads over 4 key heads: 26 us and 5 for the join (4.8 TB/s).  fp32, 8 x 77 x 211: 14 + 6 and 35 + 6 us.
+// Measured, bf16 (the least and the median of 23 launches in a row, under which the clock falls): 2 x 2048 x 4096, 16 heads of 64: forward 103 - 115 us (0.60 - 0.67
+// PF/s), backward 271 - 296 (0.58 - 0.63, 0.81 - 0.89 with the products that it makes twice); the vector pipe is busy 50 % (forward) and 44 % of that, the
+// matrix pipe 28 % and 40 %, and two waves per SIMD, all that the registers hold, overlap them little (products between the vector instructions of one
+// wave, raised priorities: no gain).  With dropout, which draws a hash per weight and loads no fragment ahead: 147 - 154 and 379 - 402.  104 x 60 x 100, 12
+// heads of 64: 17 + 42 us (its bytes at a copy's rate: 14 + 23).  16 x 1 x 16384, 16 heads over 4 key heads: 26 us and 5 for the join (4.8 TB/s).  fp32, 8 x 77 x 211: 13 + 5
+// and 35 + 6 us.
 #include "../../include/uc2_hip.h"
 #include "common.h"
 
@@ -893,8 +895,9 @@ static XaPlan xa_plan(const Uc2CrossAttn* p) {
   r.s_dq = xa_splits(p, r.ns_bwd, (int)R, p->Lk);
   r.s_dkv = xa_splits(p, r.ns_bwd, p->Lk, (int)R);
   r.part_dkv = r.s_dkv > 1 ? xa_up((size_t)r.s_dkv * 2 * bh * p->Lk * p->D * 4) : 0;
-  // delta by a kernel of its own where five workgroups or more stream the same rows and there is work to hide a launch in (2 x 2048 x 4096, 16 heads, forward
-  // and backward 377 us against 398; 8 x 100 x 600, 12 heads 46.5 against 47; 128 x 2000, 4 heads 25 against 23.6)
+  // delta by a kernel of its own where five workgroups or more stream the same rows and there is work to hide a launch in: from 2^22 scores on.  Forward and
+  // backward with it / without, us: 2^20 scores (128 x 2000, 4 heads) 24.7 / 23.2 for bf16 heads of 64, 41.0 / 39.5 for heads of 128, fp32 53.4 / 51.8; 2^22 (512 x 2048, 4
+  // heads) 37.3 / 36.0, 59.6 / 61.8, 78.0 / 78.4; 2^24 (2 x 1024 x 1024, 8 heads) 56.2 / 55.5, 103.8 / 110.3, 210 / 215; 2^27 (2 x 2048 x 2048, 16 heads) 186 / 192, 446 / 503, 1370 / 1428
   r.pre = r.ns_bwd == 4 && p->Lk > 512 && bh * R * p->Lk >= (1 << 22);
   r.delta = r.pre ? xa_up((size_t)bh * R * 4) : 0;
   r.bwd = r.delta + r.part_dkv + (r.s_dq > 1 ? (size_t)r.s_dq * bh * R * p->D * 4 : 0);

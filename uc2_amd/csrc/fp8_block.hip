@@ -1,7 +1,8 @@
 // Quantisation to e4m3 under power-of-two block scales (fp8_block.h): rows in blocks of 1 x 128 (activations, output gradients), weights in
 // blocks of 128 x 128, in both orientations from one read -- a square block has the same scale in W and in W^T, so the input gradient's
 // operand holds the very bytes of the forward's.  HBM-bound: x once in, one byte per element (two for a weight) out.
-// Measured: rows 66560 x 1024 bf16 36 us (5.7 TB/s), 9984 x 2304 15 us (4.6); a 2304 x 768 fp32 weight in both orientations 6 us (108 workgroups).
+// Measured (medians): rows 66560 x 1024 bf16 37 us (5.6 TB/s), 9984 x 2304 15 us (4.6); a 2304 x 768 fp32 weight in both orientations 6 us: one round of memory
+// latency and a reduction on 108 workgroups, one per block, which is what a block's maximum needs (its bytes at a copy's rate: 2.2).
 #include "../../include/uc2_hip.h"
 #include "common.h"
 #include "fp8_block.h"

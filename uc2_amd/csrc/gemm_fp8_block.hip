@@ -3,8 +3,9 @@
 //   C[m][n] = bias[n] + sum over k-blocks b of 2^(ea[m][b] + eb[n / 128][b]) sum_{k in b} a[m][k] b[n][k]
 // The scales are powers of two, so v_mfma_scale_f32_16x16x128_f8f6f4 applies both inside the matrix instruction (one k-block of 128 per
 // instruction): no second accumulator, no multiply per block; sums are fp32 throughout and rounded to bf16 once.
-// Measured: 66560 x 4096 x 1024 272 us (2.05 PF/s in the persistent kernel, eight k-tiles a tile; 8192^3 2.7), 9984 x 768 x 2304 29 us,
-// 1237 x 777 x 1000 8.7 us, 8 x 4096 x 1024 3.4 us, 1 x 1024 x 4096 4.9 us (latency: every wave four blocks, one after the other).
+// Measured: 66560 x 4096 x 1024 282 us at the least and 321 as the median of 23 in a row, under which the clock falls (1.98, 1.74 PF/s in the persistent kernel,
+// eight k-tiles a tile; 8192^3 2.7 PF/s); medians: 9984 x 2304 x 768 31 us, 9984 x 768 x 2304 30 us, 1237 x 777 x 1000 8.5 us, 8 x 4096 x 1024 3.4 us, 1 x 1024 x 4096
+// 4.9 us (latency: every wave four blocks, one after the other).
 #include "../../include/uc2_hip.h"
 #include "common.h"
 #include "fp8_block.h"

@@ -6,8 +6,8 @@
 // 4 M H (s, dy, ds in; dx out).  A row stays in registers between its reduction and its use: NW waves per row, NV chunks of 8 elements
 // per lane (rows up to 64 * 8 * NV * NW wide).  Rows need no alignment: the vector loads are unaligned ones (legal for global memory on
 // gfx950), a row's last partial chunk goes element by element.
-// Measured: 66560 x 1024 bf16 with a residual: forward 84 us (6.5 TB/s), backward 108 and 5 for dw's sum over the 512 workgroups (4.9 TB/s: it lives on three
-// streams in and one out, as a copy does); 33280 x 1024 to e4m3 36 us (6.6 TB/s); 4099 x 1000 fp32 12 + 14 + 4 us (5.4, 4.7 TB/s).
+// Measured (medians): 66560 x 1024 bf16 with a residual: forward 84 us (6.5 TB/s), backward 112 and 5 for dw's sum over the 512 workgroups (4.9 TB/s: it lives on
+// three streams in and one out, as a copy does); 33280 x 1024 to e4m3 37 us (6.5 TB/s); 4099 x 1000 fp32 12 + 14 + 4 us (5.4, 4.7 TB/s).
 #include "../../include/uc2_hip.h"
 #include "common.h"
 #include "fp8_block.h"
