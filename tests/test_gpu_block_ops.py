@@ -520,6 +520,18 @@ def test_cross_attention_one_key_has_no_gradient_of_its_scores(dtype, Lq, Lk, nh
         assert Lk < 2 or bool(dq[4].any()) and bool(dk[4, :2].any())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("Lq,Lk,nh,nkv,D,left", [(3, 300, 4, 4, 32, [10, 290]), (70, 300, 4, 2, 64, range(5, 300, 32)), (2, 5000, 4, 1, 128, [10, 4990]), (2, 5000, 4, 1, 64, [4998, 4999]),
+                                                 (600, 1500, 3, 3, 32, range(31, 1500, 64)), (40, 64, 2, 2, 64, [0, 33])])
+def test_cross_attention_keys_far_apart(dtype, Lq, Lk, nh, nkv, D, left):
+    """two keys and more, one of them at most in a tile, a split or a wave's share: none is taken for the only one"""
+    q, k, v, dout = attn_inputs(2, Lq, Lk, nh, nkv, D, dtype)
+    mask = torch.full((2, Lk), -1e30, device=DEV)
+    mask[:, list(left)] = normal((2, len(left)), 9)
+    got = check_attn(q, k, v, dout, key_mask=mask)
+    assert bool(got[1].any()) and all(bool(got[2][:, j].any()) for j in left)
+
+
 def test_cross_attention_views():
     """heads before positions, fused projections, expanded keys, unaligned slices (copied), a gradient that is a broadcast"""
     B, Lq, Lk, nh, D = 2, 19, 70, 4, 64

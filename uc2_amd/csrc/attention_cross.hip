@@ -367,12 +367,20 @@ __device__ __forceinline__ float xa_max2(float x) {
 }
 __device__ __forceinline__ int xa_len(const XaArgs& a, int b) { return a.klens ? max(0, min(a.klens[b], a.Lk)) : a.Lk; }
 // Whether just one key of the sequence takes part.  The softmax over one key is constant, so dq and dk are zero; p (dp - delta) would leave fp32's rounding
-// noise there, dp and delta being sums of the same products in two orders.  Their last factor, the scale, is zero then (NaN stays NaN).  seen: the keys
-// that the wave has met (two: nothing is read; otherwise the mask is, up to its second key).
-__device__ __forceinline__ bool xa_alone(const XaArgs& a, int b, int len, int lane, int seen) {
+// noise there, dp and delta being sums of the same products in two orders.  Their last factor, the scale, is zero then (NaN stays NaN).  seen: keys that take part
+// among those that the wave has met, `all`: it has met every one; the mask is read, up to its second key, by a wave that met one of them only (one that met
+// none has zeros to scale).
+__device__ __forceinline__ bool xa_alone(const XaArgs& a, int b, int len, int lane, int seen, bool all) {
   if (!a.kmask) return len == 1;
-  int n = seen < 2 ? 0 : seen;
-  for (int j0 = 0; n < 2 && j0 < len; j0 += 64) n += __popcll(__ballot(j0 + lane < len && !(xa_key_raw(a, b, j0 + lane, len) <= XA_REMOVED)));
+  if (seen != 1 || all) return seen == 1;
+  int n = 0;
+  for (int j0 = 0; n < 2 && j0 < len; j0 += 256) {
+    float raw[4];                                                 // (four loads in flight)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) raw[u] = xa_key_raw(a, b, j0 + 64 * u + lane, len);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) n += __popcll(__ballot(j0 + 64 * u + lane < len && !(raw[u] <= XA_REMOVED)));
+  }
   return n == 1;
 }
 
@@ -665,7 +673,7 @@ __device__ __forceinline__ void xa_dq(const XaArgs& a, int blk, XaLds<T, D, DROP
     __syncthreads();
     buf ^= 1;
   }
-  const float scale = xa_alone(a, b, len, lane, seen) ? 0.f : a.scale;
+  const float scale = xa_alone(a, b, len, lane, seen, a.dq.splits == 1) ? 0.f : a.scale;
   if (!mine) return;
   if (a.dq.splits == 1) {
     int i, g;
@@ -781,7 +789,7 @@ __device__ __forceinline__ void xa_dkv(const XaArgs& a, int blk, XaLds<T, D, DRO
     __syncthreads();
     buf ^= 1;
   }
-  const float scale = xa_alone(a, b, len, lane, __popcll(__ballot(part && lane < 32))) ? 0.f : a.scale;
+  const float scale = xa_alone(a, b, len, lane, __popcll(__ballot(part && lane < 32)), false) ? 0.f : a.scale;
   if (key >= a.Lk) return;
   if (!part) {                                                     // (without a mask its column was computed: on zero vectors, into this lane alone)
 #pragma unroll
