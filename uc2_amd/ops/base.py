@@ -163,18 +163,21 @@ def refuse_foreign_capture(ctx):
     """A captured backward pass hands its gradients to the accumulations of its leaves, those behind other operations (a cast) among them.  While an eager
     graph of a leaf from the default stream lives, or a wrapper holds the leaf's accumulation from there, the accumulation belongs to the default stream, which no
     capture may reach over to: torch ends the process there, so it is refused before.  (A warm-up on a stream of its own leaves nothing of the kind.)"""
-    todo = [node for node, _ in ctx.next_functions]
+    todo, walk, seen = [node for node, _ in ctx.next_functions], object(), []
     while todo:
         node = todo.pop()
-        if node is None or "uc2_clear" in node.metadata:          # (what lies below has been looked at: a graph does not change)
+        if node is None or node.metadata.get("uc2_walk") in (walk, "clear"):          # (clear: a graph does not change)
             continue
         if type(node).__name__ == "AccumulateGrad":
             if _accumulation_stream(node) == 0:
                 raise _lib.Uc2Error("a backward pass cannot be captured while an eager graph of the same leaves from the default stream is alive: delete its outputs "
                                     "first, warm up on a stream of its own, or capture with leaves of its own (x.detach().requires_grad_())")
         else:
-            node.metadata["uc2_clear"] = True
+            node.metadata["uc2_walk"] = walk
+            seen.append(node)
             todo.extend(below for below, _ in node.next_functions)
+    for node in seen:
+        node.metadata["uc2_walk"] = "clear"
 
 
 def once(backward):
